@@ -222,6 +222,72 @@ REAX_API int reax_sliced_i8_static(const int8_t* A, const int8_t* W, const void*
                                    const float* sw, const float* bias, void* partials, int M, int N, int G, int HP,
                                    int P, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- gated delta rule --------------------------------------------------------------------------------
+ * No counterpart in the reference, whose engine calls a library for it: the token mixer behind the grouped
+ * projection of q, k, v and z (runtime/split_gated_projection.py:73-137).  For each value head, with a float32
+ * state S [Dk, Dv] and row by row:
+ *   S <- exp(g) S;  u = beta (v - k^T S);  S <- S + k u^T;  out = scale q^T S
+ * with q and k divided by sqrt(sum of squares + 1e-6) first when `normalize` is set.  Value head h uses key head
+ * h / (v_heads / k_heads).
+ * q, k bf16 [rows, k_heads, Dk] and v bf16 [rows, v_heads, Dv] with row strides ldq, ldk, ldv (elements, multiples
+ * of 8; heads contiguous); g, beta float32 [rows, v_heads]; state float32 [n_slots, v_heads, Dk, Dv], updated in
+ * place; out bf16 [rows, v_heads, Dv].  Sequence b keeps its state in slot slots[b] (int32 [batch]; NULL: b); a
+ * slot outside [0, n_slots) marks a sequence that keeps none: its outputs are zeros.  No two sequences of a call
+ * may share a slot.  Dk and Dv are 64 or 128 each.
+ *
+ * reax_gdn_prefill: sequence b has rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1 (int32 [batch + 1] on the device;
+ * NULL: one sequence of all rows); one without rows keeps its state as it is, or gets zeros when `carry` is 0.
+ * carry: 1 = start from the states kept, 0 = from zeros, and the states are only written. */
+REAX_API int reax_gdn_prefill(const void* q, const void* k, const void* v, const float* g, const float* beta,
+                              float* state, const int32_t* cu_seqlens, const int32_t* slots, void* out, int rows,
+                              int batch, int k_heads, int v_heads, int Dk, int Dv, int n_slots, long long ldq,
+                              long long ldk, long long ldv, float scale, int normalize, int carry, void* stream);
+
+/* One row for each of `batch` sequences, from the states kept. */
+REAX_API int reax_gdn_decode(const void* q, const void* k, const void* v, const float* g, const float* beta,
+                             float* state, const int32_t* slots, void* out, int batch, int k_heads, int v_heads, int Dk,
+                             int Dv, int n_slots, long long ldq, long long ldk, long long ldv, float scale,
+                             int normalize, void* stream);
+
+/* ---- paged INT8 cache of keys and values ------------------------------------------------------------------
+ * No counterpart in the reference, whose cache is bf16.  Codes int8 [pages, heads, page, dim] and scales float32
+ * [pages, heads], one for each page and head, for k and for v; a code stands for code * scale.  Row i of sequence
+ * b lies in page tables[b, i / page] (int32 [batch, table_ld]), place i % page.  page is 16, 32 or 64 and dim 64,
+ * 128 or 256.  Places past the table, and pages outside [0, pages), are neither read nor written.
+ *
+ * reax_kv8_append: rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1 of k and v (bf16 [rows, heads, dim], row strides ldk
+ * and ldv; cu_seqlens NULL: one row a sequence) become rows lengths[b], lengths[b] + 1 .. of sequence b.  A page's
+ * scale is the largest |x| / 127 it has held (at least 1e-12 / 127; it starts anew when place 0 is written);
+ * codes are round-to-nearest-even(x / scale) in [-127, 127], and where a scale grows from s to t the page's older
+ * codes become round-to-nearest-even(code * (s / t)).  Infinities take no part in a scale and become +-127, NaN
+ * becomes 0.  No two sequences of a call may append to one page. */
+REAX_API int reax_kv8_append(const void* k, const void* v, int8_t* k_codes, int8_t* v_codes, float* k_scales,
+                             float* v_scales, const int32_t* tables, const int32_t* lengths, const int32_t* cu_seqlens,
+                             int rows, int batch, int table_ld, int pages, int heads, int page, int dim, long long ldk,
+                             long long ldv, void* stream);
+
+/* Rows starts[b], starts[b] + 1 .. of each sequence, cu_seqlens[b + 1] - cu_seqlens[b] of them, as bf16 [rows, heads,
+ * dim] k and v (zeros for places that the cache does not have). */
+REAX_API int reax_kv8_read(const int8_t* k_codes, const int8_t* v_codes, const float* k_scales, const float* v_scales,
+                           const int32_t* tables, const int32_t* starts, const int32_t* cu_seqlens, void* k, void* v,
+                           int rows, int batch, int table_ld, int pages, int heads, int page, int dim, void* stream);
+
+/* Bytes of workspace that reax_kv8_attend needs on `device` (-1 = current device); 0 on failure. */
+REAX_API size_t reax_kv8_workspace_bytes(int device);
+
+/* Softmax attention of q (bf16 [rows, heads * group, dim], row stride ldq) over the cache.  Sequence b has lengths[b]
+ * cached rows, of which its cu_seqlens[b + 1] - cu_seqlens[b] query rows (cu_seqlens NULL: one) are the last: query row
+ * i of n sees cached rows 0 .. lengths[b] - n + i.  A row that sees none gives zeros, and -inf in lse.  Query head h
+ * reads cached head h / group.  out bf16 [rows, heads * group, dim]; lse float32 [rows, heads * group] (may be NULL):
+ * the natural log of the sum of exp(scale q.k).  max_rows: at least the most query rows of a sequence (a hint for the
+ * launch; the result does not depend on it).  The workspace (reax_kv8_workspace_bytes(), zeroed once; one for each
+ * stream, as the GEMMs') holds the parts of rows whose cache several blocks share. */
+REAX_API int reax_kv8_attend(const void* q, const int8_t* k_codes, const int8_t* v_codes, const float* k_scales,
+                             const float* v_scales, const int32_t* tables, const int32_t* lengths,
+                             const int32_t* cu_seqlens, void* out, float* lse, int rows, int max_rows, int batch,
+                             int table_ld, int pages, int heads, int group, int page, int dim, long long ldq, float scale,
+                             void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- failure detection -------------------------------------------------------------------------------
  * Runs one kernel that waits on a barrier nothing arrives on, bounded by timeout_ns, and ORs
  * REAX_STATUS_SELFTEST into the status word at `workspace` (a GEMM workspace, or NULL for the status word

@@ -26,6 +26,7 @@ STATUS_BITS = {0x1: "timeout waiting for a TMA stage", 0x2: "timeout waiting for
 _P = C.c_void_p
 _I = C.c_int
 _LL = C.c_longlong
+_F = C.c_float
 _SZ = C.c_size_t
 _ULL = C.c_ulonglong
 
@@ -50,6 +51,12 @@ SIGNATURES = {
     "reax_bf16_partials": ([_P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _SZ, _P], _I),
     "reax_sliced_i8": ([_P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _SZ, _P], _I),
     "reax_sliced_i8_static": ([_P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _SZ, _P], _I),
+    "reax_gdn_prefill": ([_P] * 9 + [_I] * 7 + [_LL] * 3 + [_F, _I, _I, _P], _I),
+    "reax_gdn_decode": ([_P] * 8 + [_I] * 6 + [_LL] * 3 + [_F, _I, _P], _I),
+    "reax_kv8_append": ([_P] * 9 + [_I] * 7 + [_LL] * 2 + [_P], _I),
+    "reax_kv8_read": ([_P] * 9 + [_I] * 7 + [_P], _I),
+    "reax_kv8_attend": ([_P] * 10 + [_I] * 9 + [_LL, _F, _P, _SZ, _P], _I),
+    "reax_kv8_workspace_bytes": ([_I], _SZ),
     "reax_selftest_wait": ([_P, _ULL, _P], _I),
     "reax_noalloc_status": ([C.POINTER(C.c_uint), _I, _P], _I),
     "reax_set_stream_sms": ([_P, _I], _I),
@@ -115,8 +122,29 @@ def require_cuda(*tensors: torch.Tensor) -> None:
 
 
 # ------------------------------------------------------------------------------------------------------ workspace
-_workspaces: dict[tuple[int, int], torch.Tensor] = {}
+_workspaces: dict[tuple[int, int, str], torch.Tensor] = {}
 _ws_lock = threading.Lock()
+
+
+def _stream_workspace(device: torch.device, kind: str) -> torch.Tensor:
+    index = device.index if device.index is not None else torch.cuda.current_device()
+    key = (index, stream_handle(device), kind)
+    ws = _workspaces.get(key)
+    if ws is None:
+        with _ws_lock:
+            ws = _workspaces.get(key)
+            if ws is None:
+                size = getattr(load(), kind)(index)
+                if size == 0:
+                    raise RuntimeError(f"{kind} failed (no CUDA device?)")
+                ws = torch.zeros(size, dtype=torch.uint8, device=torch.device("cuda", index))
+                _workspaces[key] = ws
+    return ws
+
+
+def kv8_workspace(device: torch.device) -> torch.Tensor:
+    """Zero-initialised workspace of the attention over the INT8 cache for (device, current stream)."""
+    return _stream_workspace(device, "reax_kv8_workspace_bytes")
 
 
 def workspace(device: torch.device) -> torch.Tensor:
@@ -126,19 +154,7 @@ def workspace(device: torch.device) -> torch.Tensor:
     lanes replaying graphs concurrently apart (the reference keys its workspaces by stream too,
     runtime/native_core.py:102-115).
     """
-    index = device.index if device.index is not None else torch.cuda.current_device()
-    key = (index, stream_handle(device))
-    ws = _workspaces.get(key)
-    if ws is None:
-        with _ws_lock:
-            ws = _workspaces.get(key)
-            if ws is None:
-                size = load().reax_workspace_bytes(index)
-                if size == 0:
-                    raise RuntimeError("reax_workspace_bytes failed (no CUDA device?)")
-                ws = torch.zeros(size, dtype=torch.uint8, device=torch.device("cuda", index))
-                _workspaces[key] = ws
-    return ws
+    return _stream_workspace(device, "reax_workspace_bytes")
 
 
 def read_status(ws: torch.Tensor) -> int:

@@ -9,8 +9,8 @@ from pathlib import Path
 PKG = Path(__file__).resolve().parent
 ROOT = PKG.parent
 LIB = PKG / "libreax_b200.so"
-SOURCES = [PKG / "csrc" / "abi.cu"]
-HEADERS = sorted((PKG / "csrc").glob("*.cuh")) + [ROOT / "include" / "reax_b200.h"]
+SOURCES = [PKG / "csrc" / "abi.cu", PKG / "csrc" / "mixers.cu"]
+HEADERS = sorted((PKG / "csrc").glob("*.cuh")) + sorted((PKG / "csrc").glob("*.h")) + [ROOT / "include" / "reax_b200.h"]
 
 
 def nvcc() -> str:
@@ -21,7 +21,7 @@ def nvcc() -> str:
 
 def command(out: Path = LIB, extra: list[str] | None = None) -> list[str]:
     return [nvcc(), "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
-            "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden", "-shared",
+            "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden", "-shared", "--threads", "0",
             "-I", str(ROOT / "include"), "-I", str(PKG / "csrc"),
             *(extra or []), *[str(s) for s in SOURCES], "-o", str(out)]
 

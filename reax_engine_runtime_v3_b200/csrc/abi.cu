@@ -14,6 +14,7 @@
 
 #include <cudaTypedefs.h>
 
+#include "abi_shared.h"
 #include "gate_up_tc.cuh"
 #include "reax_b200.h"
 #include "rowwise.cuh"
@@ -788,6 +789,36 @@ int quant_rows_dense(const void* x, int8_t* low, float* scales, int M, int K, in
     }
 }
 }  // namespace
+
+namespace reax_abi {
+
+int fail(int code, const char* fmt, ...) {
+    char buf[512];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(buf, sizeof(buf), fmt, ap);
+    va_end(ap);
+    g_last_error = buf;
+    return code;
+}
+
+int cuda_fail(cudaError_t e, const char* what) { return ::cuda_fail(e, what); }
+
+int current_sms(int* sms) {
+    int dev = 0;
+    DeviceInfo* info = nullptr;
+    const int rc = current_device(&dev, &info);
+    if (rc == REAX_OK) *sms = info->sms;
+    return rc;
+}
+
+int device_sms(int device) {
+    int dev = device, sms = 0;
+    if (dev < 0 && cudaGetDevice(&dev) != cudaSuccess) return -1;
+    return cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess ? sms : -1;
+}
+
+}  // namespace reax_abi
 
 extern "C" {
 

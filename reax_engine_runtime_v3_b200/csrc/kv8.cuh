@@ -1,0 +1,269 @@
+// A paged INT8 cache of keys and values, and attention over it.
+//
+// Page p of head h holds `page` rows of D codes (codes [pages, heads, page, D]) and one scale
+// (scales [pages, heads]); a code c stands for c * scale.  Sequence b's row i lies in page
+// tables[b, i / page], place i % page.
+#pragma once
+
+#include "common.cuh"
+
+namespace reax {
+
+struct Kv8Cache {
+    int8_t* k;
+    int8_t* v;
+    float* k_scale;
+    float* v_scale;
+    int pages, heads, page, dim;
+};
+
+struct Kv8Append {
+    Kv8Cache c;
+    const __nv_bfloat16* k;   // [rows, heads, dim], row stride ldk
+    const __nv_bfloat16* v;
+    long long ldk, ldv;
+    const int32_t* tables;    // [batch, table_ld]
+    const int32_t* lengths;   // [batch]: rows cached before this call
+    const int32_t* cu;        // [batch + 1] (NULL: one row a sequence)
+    int rows, batch, table_ld;
+};
+
+REAX_DEVI void kv8_span(const int32_t* cu, int b, int rows, int* lo, int* hi) {
+    int l = cu ? cu[b] : b, h = cu ? cu[b + 1] : b + 1;
+    *lo = min(max(l, 0), rows);
+    *hi = min(max(h, *lo), rows);
+}
+
+REAX_DEVI float warp_max(float v) {
+#pragma unroll
+    for (int m = 16; m > 0; m >>= 1) v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, m));
+    return v;
+}
+
+// |x| of a bf16 pair's two values, infinities and NaN left out.
+REAX_DEVI float absmax_finite(float m, uint32_t w) {
+    const uint32_t a = (w << 16) & 0x7FFF0000u, b = w & 0x7FFF0000u;
+    if (a < 0x7F800000u) m = fmaxf(m, __uint_as_float(a));
+    if (b < 0x7F800000u) m = fmaxf(m, __uint_as_float(b));
+    return m;
+}
+
+// rint(x / scale) kept in [-127, 127]; NaN gives 0.
+REAX_DEVI int kv8_code(float x, float scale) {
+    const float q = rintf(__fdiv_rn(x, scale));
+    return q != q ? 0 : static_cast<int>(fminf(fmaxf(q, -127.0f), 127.0f));
+}
+
+// One block writes the new rows of one page, one head, of k (blockIdx.z = 0) or v (1).  Block x is the x-th
+// page touched, counted over the sequences in order: a warp's prefix sum over the batch finds whose it is,
+// so the host need not know the lengths.
+constexpr int kAppendThreads = 256;
+
+__global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const Kv8Append a) {
+    __shared__ int s_seq, s_page;
+    __shared__ float s_max[kAppendThreads / 32];
+    const int tid = threadIdx.x, lane = tid % 32;
+    if (tid < 32) {
+        int before = 0, seq = -1, page = 0;
+        for (int b0 = 0; b0 < a.batch; b0 += 32) {
+            int n = 0, first = 0;
+            if (b0 + lane < a.batch) {
+                int lo, hi;
+                kv8_span(a.cu, b0 + lane, a.rows, &lo, &hi);
+                const int len = max(a.lengths[b0 + lane], 0);
+                first = len / a.c.page;
+                n = hi > lo ? (len + hi - lo - 1) / a.c.page - first + 1 : 0;
+            }
+            int sum = n;
+#pragma unroll
+            for (int m = 1; m < 32; m <<= 1) {
+                const int t = __shfl_up_sync(0xFFFFFFFFu, sum, m);
+                if (lane >= m) sum += t;
+            }
+            const int x = static_cast<int>(blockIdx.x) - before;
+            const bool mine = x >= sum - n && x < sum;
+            const unsigned who = __ballot_sync(0xFFFFFFFFu, mine);
+            if (who) {
+                const int l = __ffs(who) - 1;
+                seq = b0 + l;
+                page = __shfl_sync(0xFFFFFFFFu, first + x - (sum - n), l);
+                break;
+            }
+            before += __shfl_sync(0xFFFFFFFFu, sum, 31);
+        }
+        if (lane == 0) s_seq = seq, s_page = page;
+    }
+    __syncthreads();
+    const int b = s_seq, pg = s_page;
+    if (b < 0 || pg >= a.table_ld) return;
+    const int id = a.tables[static_cast<long long>(b) * a.table_ld + pg];
+    if (id < 0 || id >= a.c.pages) return;
+    int lo, hi;
+    kv8_span(a.cu, b, a.rows, &lo, &hi);
+    const int len = max(a.lengths[b], 0), h = blockIdx.y, dim = a.c.dim;
+    const int from = max(len - pg * a.c.page, 0);                     // places of the page held before
+    const int to = min(len + hi - lo - pg * a.c.page, a.c.page);
+    const bool is_v = blockIdx.z != 0;
+    const long long ld = is_v ? a.ldv : a.ldk;
+    const __nv_bfloat16* src = (is_v ? a.v : a.k) + (lo + static_cast<long long>(pg) * a.c.page + from - len) * ld + h * dim;
+    const long long at = static_cast<long long>(id) * a.c.heads + h;
+    int8_t* dst = (is_v ? a.c.v : a.c.k) + at * a.c.page * dim;
+    float* scale = (is_v ? a.c.v_scale : a.c.k_scale) + at;
+    const int per_row = dim / 8, total = (to - from) * per_row;       // pieces of 8 values
+    constexpr int kHeld = 64 * 256 / 8 / kAppendThreads;              // a whole page of the largest size
+    uint4 x[kHeld];
+    float m = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+        const int e = tid + i * kAppendThreads;
+        if (e < total) {
+            x[i] = *reinterpret_cast<const uint4*>(src + (e / per_row) * ld + (e % per_row) * 8);
+            m = absmax_finite(absmax_finite(absmax_finite(absmax_finite(m, x[i].x), x[i].y), x[i].z), x[i].w);
+        }
+    }
+    m = warp_max(m);
+    if (lane == 0) s_max[tid / 32] = m;
+    const float was = from > 0 ? *scale : 0.0f;
+    __syncthreads();
+    m = s_max[0];
+#pragma unroll
+    for (int i = 1; i < kAppendThreads / 32; ++i) m = fmaxf(m, s_max[i]);
+    const float now = fmaxf(was, __fdiv_rn(fmaxf(m, 1e-12f), 127.0f));
+    if (tid == 0) *scale = now;
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+        const int e = tid + i * kAppendThreads;
+        if (e < total) {
+            const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+            uint32_t o[2] = {};
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float f = __uint_as_float(j % 2 ? w[j / 2] & 0xFFFF0000u : w[j / 2] << 16);
+                o[j / 4] |= (static_cast<uint32_t>(kv8_code(f, now)) & 0xFFu) << (8 * (j % 4));
+            }
+            *reinterpret_cast<uint2*>(dst + (from + e / per_row) * dim + (e % per_row) * 8) = uint2{o[0], o[1]};
+        }
+    }
+    if (now > was && from > 0) {
+        const float r = __fdiv_rn(was, now);
+        uint32_t* old = reinterpret_cast<uint32_t*>(dst);
+        for (int e = tid; e < from * dim / 4; e += kAppendThreads) {
+            const uint32_t w = old[e];
+            uint32_t o = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float f = static_cast<float>(static_cast<int8_t>(w >> (8 * j)));
+                o |= (static_cast<uint32_t>(static_cast<int>(rintf(__fmul_rn(f, r)))) & 0xFFu) << (8 * j);
+            }
+            old[e] = o;
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------- read back
+struct Kv8Read {
+    Kv8Cache c;
+    const int32_t* tables;
+    const int32_t* starts;    // [batch]: first cached row read
+    const int32_t* cu;        // [batch + 1]: rows read, packed
+    __nv_bfloat16* k;         // [rows, heads, dim]
+    __nv_bfloat16* v;
+    int rows, batch, table_ld;
+};
+
+// 8 codes a thread; row r of the output belongs to the last sequence that starts at or before it.
+__global__ void __launch_bounds__(256) kv8_read_kernel(const Kv8Read a) {
+    const int per_row = a.c.heads * a.c.dim / 8;
+    const long long total = static_cast<long long>(a.rows) * per_row;
+    const bool is_v = blockIdx.y != 0;
+    const int8_t* codes = is_v ? a.c.v : a.c.k;
+    const float* scales = is_v ? a.c.v_scale : a.c.k_scale;
+    __nv_bfloat16* out = is_v ? a.v : a.k;
+    for (long long e = blockIdx.x * 256ll + threadIdx.x; e < total; e += gridDim.x * 256ll) {
+        const int r = static_cast<int>(e / per_row), x = static_cast<int>(e % per_row) * 8;
+        const int h = x / a.c.dim, d = x % a.c.dim;
+        int lo = 0, hi = a.batch;                                     // cu[lo] <= r < cu[hi]
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            if (a.cu[mid] <= r) lo = mid; else hi = mid;
+        }
+        const int place = a.starts[lo] + r - a.cu[lo];
+        uint4 o = {};
+        if (place >= 0 && r < a.cu[a.batch] && place / a.c.page < a.table_ld) {
+            const int id = a.tables[static_cast<long long>(lo) * a.table_ld + place / a.c.page];
+            if (id >= 0 && id < a.c.pages) {
+                const long long at = static_cast<long long>(id) * a.c.heads + h;
+                const uint2 w = *reinterpret_cast<const uint2*>(codes + (at * a.c.page + place % a.c.page) * a.c.dim + d);
+                const float s = scales[at];
+                uint32_t y[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t b = j < 2 ? w.x : w.y;
+                    y[j] = bf16x2_rn(f2(static_cast<int8_t>(b >> (16 * (j % 2))) * s, static_cast<int8_t>(b >> (16 * (j % 2) + 8)) * s));
+                }
+                o = uint4{y[0], y[1], y[2], y[3]};
+            }
+        }
+        *reinterpret_cast<uint4*>(out + r * static_cast<long long>(a.c.heads) * a.c.dim + x) = o;
+    }
+}
+
+// ------------------------------------------------------------------------------------------------- attention
+struct Kv8Attend {
+    Kv8Cache c;
+    const __nv_bfloat16* q;   // [rows, heads * group, dim], row stride ldq
+    long long ldq;
+    const int32_t* tables;
+    const int32_t* lengths;   // [batch]: rows cached, the new ones among them
+    const int32_t* cu;        // [batch + 1] (NULL: one row a sequence)
+    __nv_bfloat16* out;       // [rows, heads * group, dim]
+    float* lse;               // [rows, heads * group] or NULL
+    int rows, batch, table_ld, group;
+    float scale;
+};
+
+// One warp a row and query head, one cached row at a time; lane l holds elements l * D/32 .. of the row.
+template <int D>
+__global__ void __launch_bounds__(128) kv8_attend_rows_kernel(const Kv8Attend a) {
+    constexpr int kPer = D / 32;
+    const int lane = threadIdx.x % 32, hq = blockIdx.y, h = hq / a.group;
+    const int r = blockIdx.x * 4 + threadIdx.x / 32;
+    if (r >= a.rows) return;
+    int b = 0;
+    if (a.cu) {
+        int hi = a.batch;
+        while (hi - b > 1) {
+            const int mid = (b + hi) / 2;
+            if (a.cu[mid] <= r) b = mid; else hi = mid;
+        }
+    } else b = r;
+    int lo, hi;
+    kv8_span(a.cu, b, a.rows, &lo, &hi);
+    const int heads_q = a.c.heads * a.group;
+    const int seen = r < hi ? min(a.lengths[b] - (hi - lo) + (r - lo) + 1, a.table_ld * a.c.page) : 0;
+    float q[kPer], o[kPer] = {}, m = -INFINITY, l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) q[i] = __bfloat162float(a.q[r * a.ldq + hq * D + lane * kPer + i]) * a.scale;
+    for (int t = 0; t < seen; ++t) {
+        const int id = a.tables[static_cast<long long>(b) * a.table_ld + t / a.c.page];
+        if (id < 0 || id >= a.c.pages) continue;
+        const long long at = static_cast<long long>(id) * a.c.heads + h;
+        const long long e = (at * a.c.page + t % a.c.page) * D + lane * kPer;
+        float s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) s += q[i] * static_cast<float>(a.c.k[e + i]);
+        s = warp_sum(s) * a.c.k_scale[at];
+        const float top = fmaxf(m, s), keep = __expf(m - top), w = __expf(s - top), ws = w * a.c.v_scale[at];
+        l = l * keep + w;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) o[i] = o[i] * keep + ws * static_cast<float>(a.c.v[e + i]);
+        m = top;
+    }
+    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    const long long at = static_cast<long long>(r) * heads_q + hq;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) a.out[at * D + lane * kPer + i] = __float2bfloat16_rn(o[i] * inv);
+    if (lane == 0 && a.lse) a.lse[at] = l > 0.0f ? m + logf(l) : -INFINITY;
+}
+
+}  // namespace reax

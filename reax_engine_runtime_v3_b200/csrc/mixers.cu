@@ -1,0 +1,187 @@
+// C ABI of the token mixers: the gated delta rule and the paged INT8 cache with its attention
+// (declarations and contracts: include/reax_b200.h).  As in abi.cu, nothing here allocates or synchronizes.
+#include <algorithm>
+#include <utility>
+
+#include "abi_shared.h"
+#include "gdn.cuh"
+#include "kv8.cuh"
+#include "reax_b200.h"
+
+namespace {
+
+using reax_abi::fail;
+
+constexpr int kGridYz = 65535;
+
+bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
+
+template <typename P>
+int launch(const char* what, void (*kernel)(P), dim3 grid, int threads, size_t smem, void* stream, const P& p) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads, 1, 1);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = static_cast<cudaStream_t>(stream);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
+    return e == cudaSuccess ? REAX_OK : reax_abi::cuda_fail(e, what);
+}
+
+int check_gdn(const char* who, const reax::GdnParams& p, int Dk, int Dv) {
+    if (p.rows < 0 || p.batch < 0 || p.k_heads <= 0 || p.v_heads <= 0 || p.v_heads % p.k_heads || p.n_slots < 0)
+        return fail(REAX_ERR_INVALID, "%s: rows %d, batch %d, heads %d and %d (the second a multiple of the first), "
+                    "slots %d", who, p.rows, p.batch, p.k_heads, p.v_heads, p.n_slots);
+    if ((Dk != 64 && Dk != 128) || (Dv != 64 && Dv != 128))
+        return fail(REAX_ERR_INVALID, "%s: head widths %d and %d: each must be 64 or 128", who, Dk, Dv);
+    if (p.ldq < static_cast<long long>(p.k_heads) * Dk || p.ldk < static_cast<long long>(p.k_heads) * Dk ||
+        p.ldv < static_cast<long long>(p.v_heads) * Dv)
+        return fail(REAX_ERR_INVALID, "%s: a row stride is shorter than its row", who);
+    if (p.v_heads > kGridYz || p.batch > kGridYz)
+        return fail(REAX_ERR_INVALID, "%s: at most %d heads and sequences", who, kGridYz);
+    if (p.rows == 0 || p.batch == 0) return REAX_OK;
+    if (!p.q || !p.k || !p.v || !p.g || !p.beta || !p.state || !p.out)
+        return fail(REAX_ERR_INVALID, "%s: NULL pointer", who);
+    if (!aligned(p.q, 16) || !aligned(p.k, 16) || !aligned(p.v, 16) || !aligned(p.state, 16) || !aligned(p.out, 16) ||
+        p.ldq % 8 || p.ldk % 8 || p.ldv % 8)
+        return fail(REAX_ERR_ALIGN, "%s: q, k, v, state and out must be 16-byte aligned, row strides multiples of 8", who);
+    return REAX_OK;
+}
+
+#define REAX_GDN_DISPATCH(Dk, Dv, X)               \
+    (Dk == 128 ? (Dv == 128 ? X(128, 128) : X(128, 64)) : (Dv == 128 ? X(64, 128) : X(64, 64)))
+
+int gdn_rows(const char* who, const reax::GdnParams& p, int Dk, int Dv, void* stream) {
+#define X(K, V) reax::gdn_rows_kernel<K, V>
+    return launch(who, REAX_GDN_DISPATCH(Dk, Dv, X), dim3(Dv / 16, p.v_heads, p.batch), 128, 0, stream, p);
+#undef X
+}
+
+int check_cache(const char* who, const reax::Kv8Cache& c) {
+    if (c.pages < 0 || c.heads <= 0 || c.heads > kGridYz)
+        return fail(REAX_ERR_INVALID, "%s: %d pages of %d heads", who, c.pages, c.heads);
+    if ((c.page != 16 && c.page != 32 && c.page != 64) || (c.dim != 64 && c.dim != 128 && c.dim != 256))
+        return fail(REAX_ERR_INVALID, "%s: pages of %d rows must have 16, 32 or 64, heads of %d values 64, 128 or 256", who,
+                    c.page, c.dim);
+    if (!c.k || !c.v || !c.k_scale || !c.v_scale) return fail(REAX_ERR_INVALID, "%s: NULL pointer in the cache", who);
+    if (!aligned(c.k, 16) || !aligned(c.v, 16)) return fail(REAX_ERR_ALIGN, "%s: codes must be 16-byte aligned", who);
+    return REAX_OK;
+}
+
+int check_rows(const char* who, const int32_t* tables, const int32_t* lengths, const int32_t* cu, int rows, int batch,
+               int table_ld) {
+    if (rows < 0 || batch < 0 || table_ld < 0) return fail(REAX_ERR_INVALID, "%s: negative size", who);
+    if (rows == 0 || batch == 0) return REAX_OK;
+    if (!tables || !lengths) return fail(REAX_ERR_INVALID, "%s: NULL pointer", who);
+    if (!cu && rows != batch)
+        return fail(REAX_ERR_INVALID, "%s: %d rows for %d sequences: without cu_seqlens each has one", who, rows, batch);
+    return REAX_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int reax_gdn_prefill(const void* q, const void* k, const void* v, const float* g, const float* beta, float* state,
+                     const int32_t* cu_seqlens, const int32_t* slots, void* out, int rows, int batch, int k_heads,
+                     int v_heads, int Dk, int Dv, int n_slots, long long ldq, long long ldk, long long ldv, float scale,
+                     int normalize, int carry, void* stream) {
+    using bf16 = __nv_bfloat16;
+    const reax::GdnParams p = {static_cast<const bf16*>(q), static_cast<const bf16*>(k), static_cast<const bf16*>(v), g,
+                               beta, state, cu_seqlens, slots, static_cast<bf16*>(out), ldq, ldk, ldv, rows, batch, k_heads,
+                               v_heads, n_slots, scale, normalize, carry};
+    int rc = check_gdn("reax_gdn_prefill", p, Dk, Dv), sms = 0;
+    if (rc != REAX_OK || rows == 0 || batch == 0) return rc;
+    if (!cu_seqlens && batch != 1)
+        return fail(REAX_ERR_INVALID, "reax_gdn_prefill: %d sequences need cu_seqlens", batch);
+    if ((rc = reax_abi::current_sms(&sms)) != REAX_OK) return rc;
+    return gdn_rows("reax_gdn_prefill", p, Dk, Dv, stream);
+}
+
+int reax_gdn_decode(const void* q, const void* k, const void* v, const float* g, const float* beta, float* state,
+                    const int32_t* slots, void* out, int batch, int k_heads, int v_heads, int Dk, int Dv, int n_slots,
+                    long long ldq, long long ldk, long long ldv, float scale, int normalize, void* stream) {
+    using bf16 = __nv_bfloat16;
+    const reax::GdnParams p = {static_cast<const bf16*>(q), static_cast<const bf16*>(k), static_cast<const bf16*>(v), g,
+                               beta, state, nullptr, slots, static_cast<bf16*>(out), ldq, ldk, ldv, batch, batch, k_heads,
+                               v_heads, n_slots, scale, normalize, 1};
+    int rc = check_gdn("reax_gdn_decode", p, Dk, Dv), sms = 0;
+    if (rc != REAX_OK || batch == 0) return rc;
+    if ((rc = reax_abi::current_sms(&sms)) != REAX_OK) return rc;
+#define X(K, V) reax::gdn_step_kernel<K, V>
+    return launch("reax_gdn_decode", REAX_GDN_DISPATCH(Dk, Dv, X), dim3(v_heads, batch), reax::kStepThreads, 0, stream, p);
+#undef X
+}
+
+int reax_kv8_append(const void* k, const void* v, int8_t* k_codes, int8_t* v_codes, float* k_scales, float* v_scales,
+                    const int32_t* tables, const int32_t* lengths, const int32_t* cu_seqlens, int rows, int batch,
+                    int table_ld, int pages, int heads, int page, int dim, long long ldk, long long ldv, void* stream) {
+    const char* who = "reax_kv8_append";
+    using bf16 = __nv_bfloat16;
+    const reax::Kv8Append a = {{k_codes, v_codes, k_scales, v_scales, pages, heads, page, dim},
+                               static_cast<const bf16*>(k), static_cast<const bf16*>(v), ldk, ldv, tables, lengths,
+                               cu_seqlens, rows, batch, table_ld};
+    int rc = check_rows(who, tables, lengths, cu_seqlens, rows, batch, table_ld), sms = 0;
+    if (rc != REAX_OK || rows == 0 || batch == 0) return rc;
+    if ((rc = check_cache(who, a.c)) != REAX_OK) return rc;
+    if (!k || !v) return fail(REAX_ERR_INVALID, "%s: NULL pointer", who);
+    if (ldk < static_cast<long long>(heads) * dim || ldv < static_cast<long long>(heads) * dim)
+        return fail(REAX_ERR_INVALID, "%s: a row stride is shorter than its row", who);
+    if (!aligned(k, 16) || !aligned(v, 16) || ldk % 8 || ldv % 8)
+        return fail(REAX_ERR_ALIGN, "%s: k and v must be 16-byte aligned, row strides multiples of 8", who);
+    if ((rc = reax_abi::current_sms(&sms)) != REAX_OK) return rc;
+    // n new rows touch at most (n - 1) / page + 2 pages: the most that any split of `rows` over the batch gives
+    const long long most = cu_seqlens ? static_cast<long long>(rows) / page + 2ll * std::min(rows, batch) : batch;
+    return launch(who, reax::kv8_append_kernel, dim3(static_cast<unsigned>(most), heads, 2), reax::kAppendThreads, 0, stream,
+                  a);
+}
+
+int reax_kv8_read(const int8_t* k_codes, const int8_t* v_codes, const float* k_scales, const float* v_scales,
+                  const int32_t* tables, const int32_t* starts, const int32_t* cu_seqlens, void* k, void* v, int rows,
+                  int batch, int table_ld, int pages, int heads, int page, int dim, void* stream) {
+    const char* who = "reax_kv8_read";
+    const reax::Kv8Read a = {{const_cast<int8_t*>(k_codes), const_cast<int8_t*>(v_codes), const_cast<float*>(k_scales),
+                              const_cast<float*>(v_scales), pages, heads, page, dim},
+                             tables, starts, cu_seqlens, static_cast<__nv_bfloat16*>(k), static_cast<__nv_bfloat16*>(v), rows,
+                             batch, table_ld};
+    int rc = check_rows(who, tables, starts, cu_seqlens, rows, batch, table_ld), sms = 0;
+    if (rc != REAX_OK || rows == 0 || batch == 0) return rc;
+    if ((rc = check_cache(who, a.c)) != REAX_OK) return rc;
+    if (!cu_seqlens || !k || !v) return fail(REAX_ERR_INVALID, "%s: NULL pointer", who);
+    if (!aligned(k, 16) || !aligned(v, 16)) return fail(REAX_ERR_ALIGN, "%s: k and v must be 16-byte aligned", who);
+    if ((rc = reax_abi::current_sms(&sms)) != REAX_OK) return rc;
+    const long long work = (static_cast<long long>(rows) * heads * dim / 8 + 255) / 256;
+    return launch(who, reax::kv8_read_kernel, dim3(static_cast<unsigned>(std::min<long long>(work, sms * 8ll)), 2), 256, 0,
+                  stream, a);
+}
+
+size_t reax_kv8_workspace_bytes(int device) {
+    const int sms = reax_abi::device_sms(device);
+    return sms < 0 ? 0 : 256;
+}
+
+int reax_kv8_attend(const void* q, const int8_t* k_codes, const int8_t* v_codes, const float* k_scales,
+                    const float* v_scales, const int32_t* tables, const int32_t* lengths, const int32_t* cu_seqlens,
+                    void* out, float* lse, int rows, int max_rows, int batch, int table_ld, int pages, int heads, int group,
+                    int page, int dim, long long ldq, float scale, void* workspace, size_t workspace_bytes, void* stream) {
+    const char* who = "reax_kv8_attend";
+    const reax::Kv8Attend a = {{const_cast<int8_t*>(k_codes), const_cast<int8_t*>(v_codes), const_cast<float*>(k_scales),
+                                const_cast<float*>(v_scales), pages, heads, page, dim},
+                               static_cast<const __nv_bfloat16*>(q), ldq, tables, lengths, cu_seqlens,
+                               static_cast<__nv_bfloat16*>(out), lse, rows, batch, table_ld, group, scale};
+    int rc = check_rows(who, tables, lengths, cu_seqlens, rows, batch, table_ld), sms = 0;
+    if (rc != REAX_OK || rows == 0 || batch == 0) return rc;
+    if ((rc = check_cache(who, a.c)) != REAX_OK) return rc;
+    if (!q || !out) return fail(REAX_ERR_INVALID, "%s: NULL pointer", who);
+    if (group <= 0 || heads * static_cast<long long>(group) > kGridYz)
+        return fail(REAX_ERR_INVALID, "%s: %d query heads a cached head, %d cached heads", who, group, heads);
+    if (ldq < static_cast<long long>(heads) * group * dim) return fail(REAX_ERR_INVALID, "%s: row stride shorter than a row", who);
+    if (!aligned(q, 16) || !aligned(out, 16) || ldq % 8)
+        return fail(REAX_ERR_ALIGN, "%s: q and out must be 16-byte aligned, the row stride a multiple of 8", who);
+    if ((rc = reax_abi::current_sms(&sms)) != REAX_OK) return rc;
+    const dim3 grid((rows + 3) / 4, heads * group);
+    if (dim == 64) return launch(who, reax::kv8_attend_rows_kernel<64>, grid, 128, 0, stream, a);
+    if (dim == 128) return launch(who, reax::kv8_attend_rows_kernel<128>, grid, 128, 0, stream, a);
+    return launch(who, reax::kv8_attend_rows_kernel<256>, grid, 128, 0, stream, a);
+}
+
+}  // extern "C"
