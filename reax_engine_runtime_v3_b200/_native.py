@@ -53,6 +53,7 @@ SIGNATURES = {
     "reax_sliced_i8_static": ([_P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _SZ, _P], _I),
     "reax_gdn_prefill": ([_P] * 9 + [_I] * 7 + [_LL] * 3 + [_F, _I, _I, _P], _I),
     "reax_gdn_decode": ([_P] * 8 + [_I] * 6 + [_LL] * 3 + [_F, _I, _P], _I),
+    "reax_mixer_status": ([C.POINTER(C.c_uint), _I, _P], _I),
     "reax_kv8_append": ([_P] * 9 + [_I] * 7 + [_LL] * 2 + [_P], _I),
     "reax_kv8_read": ([_P] * 9 + [_I] * 7 + [_P], _I),
     "reax_kv8_attend": ([_P] * 10 + [_I] * 9 + [_LL, _F, _P, _SZ, _P], _I),
@@ -167,6 +168,14 @@ def noalloc_status(clear: bool = False) -> int:
     current stream's work (synchronizes that stream)."""
     v = C.c_uint(0)
     check(load().reax_noalloc_status(C.byref(v), 1 if clear else 0, stream_handle()))
+    return int(v.value)
+
+
+def mixer_status(clear: bool = False) -> int:
+    """Status word of the gated delta rule's prompt form on the current device, after the current stream's work
+    (synchronizes that stream); non-zero means a bounded wait expired."""
+    v = C.c_uint(0)
+    check(load().reax_mixer_status(C.byref(v), 1 if clear else 0, stream_handle()))
     return int(v.value)
 
 

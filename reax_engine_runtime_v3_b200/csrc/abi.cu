@@ -818,6 +818,8 @@ int device_sms(int device) {
     return cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess ? sms : -1;
 }
 
+unsigned long long wait_timeout_ns() { return g_timeout_ns; }
+
 }  // namespace reax_abi
 
 extern "C" {

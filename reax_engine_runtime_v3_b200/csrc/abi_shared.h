@@ -14,4 +14,7 @@ int current_sms(int* sms);
 // Multiprocessors of `device` (-1: the current one); -1 on failure.
 int device_sms(int device);
 
+// Bound of device-side waits (reax_set_wait_timeout_ns).
+unsigned long long wait_timeout_ns();
+
 }  // namespace reax_abi

@@ -1,10 +1,12 @@
 // C ABI of the token mixers: the gated delta rule and the paged INT8 cache with its attention
 // (declarations and contracts: include/reax_b200.h).  As in abi.cu, nothing here allocates or synchronizes.
 #include <algorithm>
+#include <atomic>
 #include <utility>
 
 #include "abi_shared.h"
 #include "gdn.cuh"
+#include "gdn_chunk.cuh"
 #include "kv8.cuh"
 #include "reax_b200.h"
 
@@ -16,14 +18,14 @@ constexpr int kGridYz = 65535;
 
 bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
 
-template <typename P>
-int launch(const char* what, void (*kernel)(P), dim3 grid, int threads, size_t smem, void* stream, const P& p) {
+template <typename... P>
+int launch(const char* what, void (*kernel)(P...), dim3 grid, int threads, size_t smem, void* stream, const P&... p) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(threads, 1, 1);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = static_cast<cudaStream_t>(stream);
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p...);
     return e == cudaSuccess ? REAX_OK : reax_abi::cuda_fail(e, what);
 }
 
@@ -49,6 +51,29 @@ int check_gdn(const char* who, const reax::GdnParams& p, int Dk, int Dv) {
 
 #define REAX_GDN_DISPATCH(Dk, Dv, X)               \
     (Dk == 128 ? (Dv == 128 ? X(128, 128) : X(128, 64)) : (Dv == 128 ? X(64, 128) : X(64, 64)))
+
+// Shared memory of a kernel above the default limit, set once for each device.
+constexpr int kMaxDevices = 64;
+int allow_smem(const void* kernel, std::atomic<bool> (&done)[kMaxDevices], size_t bytes) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return reax_abi::cuda_fail(e, "cudaGetDevice");
+    if (dev >= kMaxDevices) return fail(REAX_ERR_DEVICE, "device ordinal %d out of range", dev);
+    if (done[dev].load(std::memory_order_acquire)) return REAX_OK;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+    if (e != cudaSuccess) return reax_abi::cuda_fail(e, "cudaFuncSetAttribute(shared memory)");
+    done[dev].store(true, std::memory_order_release);
+    return REAX_OK;
+}
+
+template <int DK, int DV>
+int gdn_chunks(const char* who, const reax::GdnParams& p, void* stream) {
+    static std::atomic<bool> done[kMaxDevices];
+    const int rc = allow_smem(reinterpret_cast<const void*>(reax::gdn_chunk_kernel<DK, DV>), done, reax::gdn_chunk_smem());
+    if (rc != REAX_OK) return rc;
+    return launch(who, reax::gdn_chunk_kernel<DK, DV>, dim3(p.v_heads, p.batch), reax::kChunkThreads, reax::gdn_chunk_smem(),
+                  stream, p, reax_abi::wait_timeout_ns());
+}
 
 int gdn_rows(const char* who, const reax::GdnParams& p, int Dk, int Dv, void* stream) {
 #define X(K, V) reax::gdn_rows_kernel<K, V>
@@ -94,7 +119,20 @@ int reax_gdn_prefill(const void* q, const void* k, const void* v, const float* g
     if (!cu_seqlens && batch != 1)
         return fail(REAX_ERR_INVALID, "reax_gdn_prefill: %d sequences need cu_seqlens", batch);
     if ((rc = reax_abi::current_sms(&sms)) != REAX_OK) return rc;
-    return gdn_rows("reax_gdn_prefill", p, Dk, Dv, stream);
+#define X(K, V) gdn_chunks<K, V>("reax_gdn_prefill", p, stream)
+    return REAX_GDN_DISPATCH(Dk, Dv, X);
+#undef X
+}
+
+int reax_mixer_status(unsigned* status, int clear, void* stream) {
+    if (!status) return fail(REAX_ERR_INVALID, "reax_mixer_status: NULL pointer");
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    unsigned zero = 0;
+    cudaError_t e = cudaMemcpyFromSymbolAsync(status, reax::g_mixer_status, sizeof(unsigned), 0, cudaMemcpyDeviceToHost, s);
+    if (e == cudaSuccess && clear)
+        e = cudaMemcpyToSymbolAsync(reax::g_mixer_status, &zero, sizeof(unsigned), 0, cudaMemcpyHostToDevice, s);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+    return e == cudaSuccess ? REAX_OK : reax_abi::cuda_fail(e, "reax_mixer_status");
 }
 
 int reax_gdn_decode(const void* q, const void* k, const void* v, const float* g, const float* beta, float* state,
