@@ -1,6 +1,7 @@
 // Host helpers of the C ABI that its translation units share (defined in abi.cu).
 #pragma once
 
+#include <cuda.h>
 #include <cuda_runtime.h>
 
 namespace reax_abi {
@@ -14,6 +15,10 @@ int current_sms(int* sms);
 // Multiprocessors of `device` (-1: the current one); -1 on failure.
 int device_sms(int device);
 
+// Tensor map of row-major bf16 [rows, cols], row stride ld elements; boxes of box_rows x box_cols, zeros outside;
+// swizzle: the 128-byte one (box_cols 64).
+int encode_rows(CUtensorMap* map, const void* base, int cols, int rows, long long ld, int box_cols, int box_rows,
+                bool swizzle);
 // Bound of device-side waits (reax_set_wait_timeout_ns).
 unsigned long long wait_timeout_ns();
 

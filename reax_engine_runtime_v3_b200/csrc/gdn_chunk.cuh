@@ -7,23 +7,25 @@
 //   out_i = e^(G_i) q_i^T S + sum_(j <= i) P_ij V'_j,   P_ij = e^(G_i - G_j) q_i.k_j
 //   S    <- e^(G_63) S + sum_j e^(G_63 - G_j) k_j V'_j^T
 //
-// With T = (I + A)^-1 diag(beta) and W = P T, both found without S, a chunk is a chain of three products:
+// With T = (I + A)^-1 diag(beta) and P, both found without S, a chunk is a chain of three products (and one beside it):
 //
-//   [X_k | X_q] = S^T [k | q]^T      ->  R      (rows j of X_k)
-//   [V' | Y]    = R^T [T | W]^T      ->  V'     (out = e^G X_q + Y)
-//   D           = V'^T diag(..) k    ->  S
+//   [X_k | X_q] = S^T [k | q]^T      ->  R      (from X_k)
+//   V'          = R^T T^T            ->  V'
+//   D           = V'^T diag(..) k    ->  S      and  Y = V'^T P^T, out = e^G X_q + Y
 //
 // Layout.  Everything is transposed so that the 128 TMEM lanes are the columns of the state (dv): S, R and V' are then
-// the A operands, in TMEM, and a thread owns one state column (a half of it: two warpgroups share the lanes), which it
+// the A operands, in TMEM, and a thread owns a half of one state column (two warpgroups share the lanes), which it
 // keeps in registers in float32 and reads from and writes to TMEM without any exchange but a row maximum.  The B
-// operands k, q, T and W are shared-memory tiles; k serves K-major (X) and MN-major (D) from one copy.
+// operands k, q, T and P are shared-memory tiles; k serves K-major (X) and MN-major (D) from one copy.
 //
 // Precision.  The state has to stay a float32 one, and the tensor cores take 16 bits.  An operand is scaled by a power of
 // two to a largest value in [2^13, 2^14) in its row and split into two fp16 numbers, hi + lo, with 22 bits; k and q
 // have 8 bits and are exact in one.  X_k, V' and D, which the state depends on, take all terms down to 2^-22; X_q and Y
 // only reach the bf16 output and take the hi terms.  Sums are float32.
 //
-// Roles (13 warps): 0-7 carry the state; 8-11 prepare T and W of the chunks ahead; 12 issues the chain's MMAs.
+// Roles (16 warps): 0-7 carry the state; 8-11 find T and P of the chunks ahead; 12 issues the chain's MMAs; 13-15 load
+// rows and turn k and q into fp16 tiles.  No role may spill: beside this much shared memory little is left of the L1
+// cache, and a spilled value comes back from L2.
 #pragma once
 
 #include <cuda_fp16.h>
@@ -34,49 +36,75 @@
 namespace reax {
 
 constexpr int kChunk = 64;
-constexpr int kChunkThreads = 13 * 32;
-constexpr int kGdnStages = 2;
+constexpr int kChunkThreads = 16 * 32;
+constexpr int kKqSlots = 3;                   // chunks of k and q tiles in flight
+constexpr int kLoaders = 3 * 32;
+constexpr float kGdnDown = 0x1p-20f, kGdnUp = 0x1p20f;
 
-// TMEM columns.  S hi and lo (64 each) share the columns of D, and V' hi and lo those of X_k: each is written after the
-// other has been read.
-constexpr uint32_t kTmS = 0, kTmXk = 128, kTmXq = 192, kTmR = 256, kTmY = 320, kTmW = 384, kTmPrep = 448;
+// TMEM columns.  S hi and lo (64 each) share the columns of D, and the decayed V' hi and lo those of X_k, V' hi those of R:
+// each is written after the other has been read.
+constexpr uint32_t kTmS = 0, kTmXk = 128, kTmXq = 192, kTmR = 256, kTmV = 320, kTmY = 384, kTmPrep = 448;
 
-struct GdnStage {
-    uint8_t kq[2][128 * 128];                 // [half of dk][64 rows of k, then of q][64 fp16], 128-byte swizzle
-    uint8_t t_hi[64 * 128], t_lo[64 * 128];   // rows i, columns j of T
-    uint8_t w[64 * 128];
-    __nv_bfloat16 v[kChunk][128];
-    float4 c[kChunk];                         // factors of X_k, V', X_q and Y for each row
-    float gamma;
-    float pad[255];
+// Tensor maps of q and k (boxes of 64 rows of 64 values, 128-byte swizzle), v (64 rows of one head) and the output (32 rows
+// of 32 columns).
+struct GdnMaps {
+    CUtensorMap q, k, v, out;
 };
-static_assert(sizeof(GdnStage) % 1024 == 0, "tiles start on swizzle atoms");
+
+// What the loaders bring of a chunk.
+struct GdnRows {
+    uint8_t kq[2][128 * 128];                 // [half of dk][64 rows of k, then of q][64 fp16], 128-byte swizzle
+    float g_hi[kChunk], g_lo[kChunk];         // G in log2, as hi + lo
+    float row_k[kChunk], row_q[kChunk];       // scales of the rows of k and q
+    float beta[kChunk];
+    float pad[192];
+};
+// What the solvers find for it: tiles and the factors of each row.
+struct GdnTiles {
+    uint8_t t_hi[64 * 128], t_lo[64 * 128];   // rows i, columns j of T
+    uint8_t p[64 * 128];                      // of P
+    float c_x[kChunk], c_b[kChunk];           // R = c_b v + c_x X_k
+    float c_v[kChunk], c_u[kChunk];           // V' decayed to the chunk's end, and for Y
+    float c_q[kChunk], c_p[kChunk];           // out = c_q X_q + c_p Y
+    float gamma;
+    float pad[127];
+};
+static_assert(sizeof(GdnRows) % 1024 == 0 && sizeof(GdnTiles) % 1024 == 0, "tiles start on swizzle atoms");
 
 struct GdnShared {
-    GdnStage stage[kGdnStages];
+    GdnRows rows[kKqSlots];
+    GdnTiles tiles[2];
     uint8_t a21[2][32 * 128];                 // A[32.., ..31] hi and lo: rows of 64 fp16, of which 32 are used
-    uint8_t raw[128 * 256];                   // k and q rows as they come
-    float a11[32 * 32], a22[32 * 32];         // 16-byte pieces of a row xor-ed with row % 8
-    float4 tok[kChunk];                       // G as hi + lo (log2), row scale of k, beta
-    float row_q[kChunk];                      // row scale of q
-    float a21_inv[32];
+    __nv_bfloat16 v[2][kChunk * 128];         // rows of DV values
+    __nv_bfloat16 out[8][32 * 32];            // a warp's 32 rows of 32 output columns
+    float a11[32 * 32], a22[32 * 32];         // -A's diagonal blocks; 16-byte pieces of a row xor-ed with row % 8
     float xch[2][8][32];
-    uint64_t full[kGdnStages], empty[kGdnStages], s_ready, r_ready, v_ready, x_done, y_done, d_done, kk_done, z_done;
+    uint64_t kq_in[kKqSlots], rows_full[kKqSlots], rows_free[kKqSlots], v_in[2], v_free[2], tiles_full[2], tiles_free[2];
+    uint64_t s_ready, r_ready, v_ready, x_done, v_done, d_done, y_done, kk_done, kk_free, z_done;
     uint32_t tmem;
-    int abort;
+    uint32_t abort;
 };
 
 static __device__ unsigned g_mixer_status;    // REAX_STATUS_* bits of waits that expired
 
+REAX_DEVI uint32_t timer_lo() {
+    uint32_t t;
+    asm volatile("mov.u32 %0, %%globaltimer_lo;" : "=r"(t));
+    return t;
+}
+// Wait for a phase, for at most limit_ns.  Once a wait of the block has expired all of them return at once, so that the
+// block runs on to its end; the flag then goes to the status word, which says that the results are invalid.  (Few
+// instructions: the roles' code has to fit the instruction cache.)
 struct GdnWait {
-    volatile int* abort;
-    unsigned long long limit_ns;
-    // Wait for a phase; once any wait of the block has expired all of them return at once, so that the block runs on to
-    // its end (with results that the status word marks as invalid).
+    volatile uint32_t* abort;
+    uint32_t limit_ns;
     REAX_DEVI void operator()(uint64_t* bar, uint32_t parity, uint32_t bit) const {
-        if (mbar_wait_bounded(bar, parity, limit_ns, abort)) return;
-        if (!*abort) atomicOr(&g_mixer_status, bit);
-        *abort = 1;
+        if (mbar_try_wait_suspend(bar, parity, 2000u)) return;
+        const uint32_t t0 = timer_lo();
+        while (!mbar_try_wait_suspend(bar, parity, 2000u)) {
+            if (*abort) return;
+            if (timer_lo() - t0 > limit_ns) *abort = bit;
+        }
     }
 };
 
@@ -134,40 +162,78 @@ REAX_DEVI uint64_t sw128_mn_desc(uint32_t smem_addr, uint32_t lbo) {
     return d | static_cast<uint64_t>(lbo >> 4) << 16;
 }
 
-REAX_DEVI void cp_async16_zfill(uint32_t dst, const void* src, bool real) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
-}
-
-// One row's solve z (I + a) = p in place, z and p of 32 columns, `a` strictly lower [32][32]: columns from the last to the
-// first, each finished value taken out of the ones before it (the row of `a` is the same for all lanes: a broadcast).
-REAX_DEVI void solve32(uint64_t (&z)[16], const float* a) {
+// One row's solve z (I + a) = p in place, z and p of 32 columns; `neg` holds -a, of which the part below the diagonal is
+// used (and zeros on it).  Four columns at a time from the last to the first: solved among themselves, then taken out of
+// the columns before them.  The rows of `neg` are the same for all lanes (broadcasts) and do not depend on z, so that
+// their loads run ahead of the chain.
+REAX_DEVI void solve32(uint64_t (&z)[16], const float* neg) {
 #pragma unroll
-    for (int j = 31; j > 0; --j) {
-        const float zj = j % 2 ? f2_hi(z[j / 2]) : f2_lo(z[j / 2]);
-        const uint64_t neg = f2(-zj, -zj);
+    for (int b = 7; b >= 0; --b) {
+        auto row = [&](int r, int c) {
+            return *reinterpret_cast<const ulonglong2*>(neg + (4 * b + r) * 32 + ((c ^ ((4 * b + r) & 7)) * 4));
+        };
+        auto twice = [](float x) { return f2(x, x); };
+        const ulonglong2 a3 = row(3, b), a2 = row(2, b), a1 = row(1, b);
+        z[2 * b + 1] = fma2_rn(twice(f2_hi(z[2 * b + 1])), a3.y, z[2 * b + 1]);
+        z[2 * b] = fma2_rn(twice(f2_hi(z[2 * b + 1])), a3.x, z[2 * b]);
+        z[2 * b] = fma2_rn(twice(f2_lo(z[2 * b + 1])), a2.x, z[2 * b]);
+        z[2 * b] = fma2_rn(twice(f2_hi(z[2 * b])), a1.x, z[2 * b]);
 #pragma unroll
-        for (int c = 0; c < (j + 3) / 4; ++c) {
-            const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(a + j * 32 + ((c ^ (j & 7)) * 4));
-            z[2 * c] = fma2_rn(neg, x.x, z[2 * c]);
-            if (4 * c + 2 < j) z[2 * c + 1] = fma2_rn(neg, x.y, z[2 * c + 1]);
-        }
+        for (int c = b - 1; c >= 0; --c)
+#pragma unroll
+            for (int r = 3; r >= 0; --r) {
+                const ulonglong2 x = row(r, c);
+                const uint64_t zz = twice(r % 2 ? f2_hi(z[2 * b + r / 2]) : f2_lo(z[2 * b + r / 2]));
+                z[2 * c] = fma2_rn(zz, x.x, z[2 * c]);
+                z[2 * c + 1] = fma2_rn(zz, x.y, z[2 * c + 1]);
+            }
     }
 }
 
+// Two float32 of a packed pair, times `f`, as fp16 pairs hi + lo.
+REAX_DEVI void split2(uint64_t x, uint64_t f, uint32_t& hi, uint32_t& lo) {
+    const uint64_t y = mul2_rn(x, f);
+    const __half2 h = __floats2half2_rn(f2_lo(y), f2_hi(y));
+    const float2 back = __half22float2(h);
+    const uint64_t rest = sub2_rn(y, f2(back.x, back.y));
+    const __half2 l = __floats2half2_rn(f2_lo(rest), f2_hi(rest));
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    lo = *reinterpret_cast<const uint32_t*>(&l);
+}
+REAX_DEVI uint32_t half2_of(uint64_t x) { return half2_bits(f2_lo(x), f2_hi(x)); }
+REAX_DEVI float max3(float m, uint64_t x) { return fmaxf(m, fmaxf(fabsf(f2_lo(x)), fabsf(f2_hi(x)))); }
+
+REAX_DEVI uint64_t u2(uint32_t lo, uint32_t hi) { return (static_cast<uint64_t>(hi) << 32) | lo; }
+REAX_DEVI void tmem_st_x8(uint32_t taddr, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
+                 "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+}
+REAX_DEVI void tmem_ld_x16_sync(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
+
 template <int DK, int DV>
-__global__ void __launch_bounds__(kChunkThreads, 1) gdn_chunk_kernel(const GdnParams p, unsigned long long limit_ns) {
+__global__ void __launch_bounds__(kChunkThreads, 1) gdn_chunk_kernel(const __grid_constant__ GdnParams p,
+                                                                     const __grid_constant__ GdnMaps maps, uint32_t limit_ns) {
     extern __shared__ uint8_t smem_raw[];
-    GdnShared& sh = *reinterpret_cast<GdnShared*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    // (an offset into the array, not an integer made a pointer: the accesses stay known as shared-memory ones)
+    GdnShared& sh = *reinterpret_cast<GdnShared*>(smem_raw + (-smem_u32(smem_raw) & 1023u));
     const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
     const int hv = blockIdx.x, b = blockIdx.y, hk = hv / (p.v_heads / p.k_heads);
     int r0, r1;
     gdn_rows(p, b, &r0, &r1);
     const int slot = gdn_slot(p, b), rows = r1 - r0, chunks = (rows + kChunk - 1) / kChunk;
-    __nv_bfloat16* out = p.out + (static_cast<long long>(r0) * p.v_heads + hv) * DV;
-    const long long ldo = static_cast<long long>(p.v_heads) * DV;
     if (slot < 0) {
-        for (long long e = tid; e < static_cast<long long>(rows) * (DV / 8); e += kChunkThreads)
-            *reinterpret_cast<uint4*>(out + e / (DV / 8) * ldo + e % (DV / 8) * 8) = uint4{};
+        __nv_bfloat16* out = p.out + (static_cast<long long>(r0) * p.v_heads + hv) * DV;
+        for (int e = tid; e < rows * (DV / 8); e += kChunkThreads)
+            *reinterpret_cast<uint4*>(out + static_cast<long long>(e / (DV / 8)) * p.v_heads * DV + e % (DV / 8) * 8) = uint4{};
         return;
     }
     float* state = p.state + (static_cast<long long>(slot) * p.v_heads + hv) * DK * DV;
@@ -179,449 +245,592 @@ __global__ void __launch_bounds__(kChunkThreads, 1) gdn_chunk_kernel(const GdnPa
 
     if (warp == 12) tmem_alloc(&sh.tmem, 512);
     if (tid == 0) {
-        for (int i = 0; i < kGdnStages; ++i) mbar_init(&sh.full[i], 128), mbar_init(&sh.empty[i], 256);
-        mbar_init(&sh.s_ready, 256), mbar_init(&sh.r_ready, 256), mbar_init(&sh.v_ready, 256);
-        mbar_init(&sh.x_done, 1), mbar_init(&sh.y_done, 1), mbar_init(&sh.d_done, 1);
-        mbar_init(&sh.kk_done, 1), mbar_init(&sh.z_done, 1);
+        for (int i = 0; i < kKqSlots; ++i) mbar_init(&sh.kq_in[i], 1), mbar_init(&sh.rows_full[i], 3), mbar_init(&sh.rows_free[i], 1);
+        for (int i = 0; i < 2; ++i) mbar_init(&sh.v_in[i], 1), mbar_init(&sh.v_free[i], 8);
+        for (int i = 0; i < 2; ++i) mbar_init(&sh.tiles_full[i], 4), mbar_init(&sh.tiles_free[i], 8);
+        mbar_init(&sh.s_ready, 8), mbar_init(&sh.r_ready, 8), mbar_init(&sh.v_ready, 8);
+        mbar_init(&sh.x_done, 1), mbar_init(&sh.v_done, 1), mbar_init(&sh.d_done, 1), mbar_init(&sh.y_done, 1);
+        mbar_init(&sh.kk_done, 1), mbar_init(&sh.kk_free, 4), mbar_init(&sh.z_done, 1);
         sh.abort = 0;
         fence_mbar_init();
     }
-    if (DV < 128)
-        for (int e = tid; e < kGdnStages * kChunk * 128; e += kChunkThreads)
-            sh.stage[e / (kChunk * 128)].v[e / 128 % kChunk][e % 128] = __float2bfloat16_rn(0.0f);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tm = sh.tmem;
     const GdnWait wait{&sh.abort, limit_ns};
+    const int quarter = warp % 4;
+    const uint32_t lanes = tm + (static_cast<uint32_t>(quarter * 32) << 16);
+    // One arrival for the warp, after what all its lanes have done.
+    auto arrive = [&](uint64_t* bar) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar);
+    };
 
     if (warp < 8) {
         // ------------------------------------------------------------------------------------ the state's warps
-        const int quarter = warp % 4, half = warp / 4, n = quarter * 32 + lane;
-        const uint32_t lanes = tm + (static_cast<uint32_t>(quarter * 32) << 16);
+        const int part = warp / 4, n = quarter * 32 + lane;       // rows 32 part .. of a chunk, S's DK / 2 part ..
         constexpr int kS = DK / 2;
-        float s[kS];
+        uint64_t s[kS / 2];
 #pragma unroll
-        for (int i = 0; i < kS; ++i) s[i] = p.carry && n < DV ? state[(half * kS + i) * DV + n] : 0.0f;
+        for (int i = 0; i < kS / 2; ++i) {
+            const float* at = state + (part * kS + 2 * i) * DV + n;
+            s[i] = p.carry && n < DV ? f2(at[0], at[DV]) : 0;
+        }
         int turn = 0;
-        // Largest of both halves of this thread's row (the two warps of a quarter meet).
+        // Largest of both parts of this thread's row (the two warps of a quarter meet).
         auto row_max = [&](float m) {
-            sh.xch[turn][warp][lane] = m;
+            float* x = &sh.xch[turn][quarter * 2][lane];
+            x[part * 32] = m;
             named_bar_sync(1 + quarter, 64);
-            m = fmaxf(m, sh.xch[turn][warp ^ 4][lane]);
             turn ^= 1;
-            return m;
+            return fmaxf(x[0], x[32]);
         };
-        float xq[32], sq = 0.0f, sr = 0.0f;
-        auto output = [&](int c) {
-            const GdnStage& st = sh.stage[c & 1];
-            uint32_t y[32];
-            tmem_ld_x32_sync(lanes + kTmW + half * 32, y);
-            const int left = rows - c * kChunk - half * 32;
-            __nv_bfloat16* o = out + (static_cast<long long>(c) * kChunk + half * 32) * ldo + n;
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-                const float4 f = st.c[half * 32 + i];
-                const float x = xq[i] * (f.z * sq) + __uint_as_float(y[i]) * (f.w * sr);
-                if (i < left && n < DV) o[i * ldo] = __float2bfloat16_rn(x);
-            }
-            mbar_arrive(&sh.empty[c & 1]);
-        };
-        for (int c = 0; c < chunks; ++c) {
+        auto pair_of = [](const float* f) { return *reinterpret_cast<const uint64_t*>(f); };
+        const uint16_t* vcol = reinterpret_cast<const uint16_t*>(sh.v[0]) + part * 32 * DV + (n < DV ? n : 0);
+        float sq = 0.0f, sv = 0.0f;          // scales of the S behind X_q and the V' behind Y
+#pragma unroll 1
+        for (int c = 0;; ++c) {
             const uint32_t par = c & 1;
-            const GdnStage& st = sh.stage[c & 1];
-            // S -> two fp16 operands
-            float m = 0.0f;
+            float2 ss = {};
+            if (c < chunks) {
+                // S -> two fp16 operands
+                float m = 0.0f;
 #pragma unroll
-            for (int i = 0; i < kS; ++i) m = fmaxf(m, fabsf(s[i]));
-            const float2 ss = scale_of(row_max(m));
+                for (int i = 0; i < kS / 2; ++i) m = max3(m, s[i]);
+                ss = scale_of(row_max(m));
 #pragma unroll
-            for (int x = 0; x < kS / 32; ++x) {
-                uint32_t hi[16], lo[16];
+                for (int x = 0; x < kS / 16; ++x) {
+                    uint32_t hi[8], lo[8];
 #pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    split2(s[x * 32 + 2 * i] * ss.x, s[x * 32 + 2 * i + 1] * ss.x, hi[i], lo[i]);
-                tmem_st_x16(lanes + kTmS + half * (kS / 2) + x * 16, hi);
-                tmem_st_x16(lanes + kTmS + 64 + half * (kS / 2) + x * 16, lo);
+                    for (int i = 0; i < 8; ++i) split2(s[x * 8 + i], f2(ss.x, ss.x), hi[i], lo[i]);
+                    tmem_st_x8(lanes + kTmS + part * (kS / 2) + x * 8, hi);
+                    tmem_st_x8(lanes + kTmS + 64 + part * (kS / 2) + x * 8, lo);
+                }
+                tmem_wait_st();
+                tc_fence_before();
+                arrive(&sh.s_ready);
             }
-            tmem_wait_st();
-            tc_fence_before();
-            mbar_arrive(&sh.s_ready);
-            if (c > 0) output(c - 1);
+            if (c > 0) {
+                // the rows out of the chunk before, through shared memory: 32 rows of 32 columns a warp
+                const GdnTiles& st = sh.tiles[par ^ 1];
+                wait(&sh.y_done, par ^ 1, kStatusTimeoutAccFull);
+                tc_fence_after();
+                if (lane == 0) bulk_wait_read_all();
+                __syncwarp();
+                uint16_t* o = reinterpret_cast<uint16_t*>(sh.out[warp]) + lane;
+#pragma unroll
+                for (int e = 0; e < 32; e += 16) {
+                    uint32_t x[16], y[16];
+                    tmem_ld2_x16_sync(lanes + kTmXq + part * 32 + e, lanes + kTmY + part * 32 + e, x, y);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int at = part * 32 + e + 2 * i;
+                        const uint64_t z = mul2_rn(u2(x[2 * i], x[2 * i + 1]), mul2_rn(pair_of(st.c_q + at), f2(sq, sq)));
+                        const uint32_t w = bf16x2_rn(fma2_rn(u2(y[2 * i], y[2 * i + 1]), mul2_rn(pair_of(st.c_p + at), f2(sv, sv)), z));
+                        o[(e + 2 * i) * 32] = static_cast<uint16_t>(w);
+                        o[(e + 2 * i + 1) * 32] = static_cast<uint16_t>(w >> 16);
+                    }
+                }
+                tc_fence_before();
+                arrive(&sh.tiles_free[par ^ 1]);
+                const int row = (c - 1) * kChunk + part * 32, left = rows - row;
+                if (quarter * 32 < DV) {
+                    if (left >= 32) {
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                        if (lane == 0) {
+                            tma_store_2d(&maps.out, sh.out[warp], hv * DV + quarter * 32, r0 + row);
+                            bulk_commit_group();
+                        }
+                    } else {
+                        uint16_t* to = reinterpret_cast<uint16_t*>(p.out);
+#pragma unroll 1
+                        for (int i = 0; i < left; ++i) to[(static_cast<long long>(r0 + row + i) * p.v_heads + hv) * DV + n] = o[i * 32];
+                    }
+                }
+            }
+            if (c == chunks) break;
+            const GdnTiles& st = sh.tiles[par];
             sq = ss.y;
             // X_k -> R
-            wait(&sh.full[c & 1], (c >> 1) & 1, kStatusTimeoutFull);
+            wait(&sh.tiles_full[par], (c >> 1) & 1, kStatusTimeoutFull);
+            wait(&sh.v_in[par], (c >> 1) & 1, kStatusTimeoutFull);
             wait(&sh.x_done, par, kStatusTimeoutAccFull);
             tc_fence_after();
-            uint32_t x[32], hi[16], lo[16];
-            tmem_ld_x32_sync(lanes + kTmXk + half * 32, x);
-            float r[32];
-            m = 0.0f;
+            uint32_t x[32];
+            float m = 0.0f;
+            {
+                uint64_t r[16];
+                tmem_ld_x32_sync(lanes + kTmXk + part * 32, x);
+                const uint16_t* v = vcol + par * (kChunk * 128);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-                const int j = half * 32 + i;
-                r[i] = __bfloat162float(st.v[j][n]) - __uint_as_float(x[i]) * (st.c[j].x * ss.y);
-                m = fmaxf(m, fabsf(r[i]));
+                for (int i = 0; i < 16; ++i) {
+                    const int at = part * 32 + 2 * i;
+                    const uint64_t y = u2(static_cast<uint32_t>(v[2 * i * DV]) << 16, static_cast<uint32_t>(v[(2 * i + 1) * DV]) << 16);
+                    r[i] = fma2_rn(u2(x[2 * i], x[2 * i + 1]), mul2_rn(pair_of(st.c_x + at), f2(ss.y, ss.y)), mul2_rn(pair_of(st.c_b + at), y));
+                }
+                if (rows - c * kChunk < kChunk)            // rows past the end, which the box takes from what follows
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const int left = rows - c * kChunk - part * 32 - 2 * i;
+                        r[i] = f2(left > 0 ? f2_lo(r[i]) : 0.0f, left > 1 ? f2_hi(r[i]) : 0.0f);
+                    }
+                arrive(&sh.v_free[par]);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) m = max3(m, r[i]);
+                const float2 rs = scale_of(row_max(m));
+                sv = rs.y;
+#pragma unroll
+                for (int e = 0; e < 16; e += 8) {
+                    uint32_t hi[8], lo[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) split2(r[e + i], f2(rs.x, rs.x), hi[i], lo[i]);
+                    tmem_st_x8(lanes + kTmR + part * 16 + e, hi);
+                    tmem_st_x8(lanes + kTmR + 32 + part * 16 + e, lo);
+                }
             }
-            const float2 rs = scale_of(row_max(m));
-#pragma unroll
-            for (int i = 0; i < 16; ++i) split2(r[2 * i] * rs.x, r[2 * i + 1] * rs.x, hi[i], lo[i]);
-            tmem_st_x16(lanes + kTmR + half * 16, hi);
-            tmem_st_x16(lanes + kTmR + 32 + half * 16, lo);
             tmem_wait_st();
             tc_fence_before();
-            mbar_arrive(&sh.r_ready);
-            sr = rs.y;
-            // V'
-            wait(&sh.y_done, par, kStatusTimeoutAccFull);
+            arrive(&sh.r_ready);
+            // V', decayed to the chunk's end for D and as it is for Y
+            wait(&sh.v_done, par, kStatusTimeoutAccFull);
             tc_fence_after();
-            tmem_ld_x32_sync(lanes + kTmY + half * 32, x);
+            tmem_ld_x32_sync(lanes + kTmV + part * 32, x);
+            float mu = 0.0f;
             m = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-                r[i] = __uint_as_float(x[i]) * (st.c[half * 32 + i].y * rs.y);
-                m = fmaxf(m, fabsf(r[i]));
+            for (int i = 0; i < 16; ++i) {
+                const int at = part * 32 + 2 * i;
+                m = max3(m, mul2_rn(u2(x[2 * i], x[2 * i + 1]), pair_of(st.c_v + at)));
+                mu = max3(mu, mul2_rn(u2(x[2 * i], x[2 * i + 1]), pair_of(st.c_u + at)));
             }
+            sh.xch[turn ^ 1][quarter * 2 + part][lane] = mu;      // read behind row_max's barrier
             const float2 vs = scale_of(row_max(m));
+            const float2 us = scale_of(fmaxf(sh.xch[turn][quarter * 2][lane], sh.xch[turn][quarter * 2 + 1][lane]));
 #pragma unroll
-            for (int i = 0; i < 16; ++i) split2(r[2 * i] * vs.x, r[2 * i + 1] * vs.x, hi[i], lo[i]);
-            tmem_st_x16(lanes + kTmXk + half * 16, hi);
-            tmem_st_x16(lanes + kTmXk + 32 + half * 16, lo);
+            for (int e = 0; e < 16; e += 8) {
+                uint32_t hi[8], lo[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int at = part * 32 + 2 * (e + i);
+                    split2(mul2_rn(u2(x[2 * (e + i)], x[2 * (e + i) + 1]), pair_of(st.c_v + at)), f2(vs.x, vs.x), hi[i], lo[i]);
+                }
+                tmem_st_x8(lanes + kTmXk + part * 16 + e, hi);
+                tmem_st_x8(lanes + kTmXk + 32 + part * 16 + e, lo);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int at = part * 32 + 2 * (e + i);
+                    hi[i] = half2_of(mul2_rn(mul2_rn(u2(x[2 * (e + i)], x[2 * (e + i) + 1]), pair_of(st.c_u + at)), f2(us.x, us.x)));
+                }
+                tmem_st_x8(lanes + kTmR + part * 16 + e, hi);
+            }
             tmem_wait_st();
             tc_fence_before();
-            mbar_arrive(&sh.v_ready);
-            // X_q is overwritten once the next state is handed over
-            tmem_ld_x32_sync(lanes + kTmXq + half * 32, x);
-#pragma unroll
-            for (int i = 0; i < 32; ++i) xq[i] = __uint_as_float(x[i]);
+            arrive(&sh.v_ready);
+            // (R's scale is that of V' until here)
+            const float back = vs.y * sv, gamma = st.gamma;
+            sv *= us.y;
             // D -> S
+#pragma unroll
+            for (int i = 0; i < kS / 2; ++i) s[i] = mul2_rn(s[i], f2(gamma, gamma));
             wait(&sh.d_done, par, kStatusTimeoutAccFull);
             tc_fence_after();
-            const float gamma = st.gamma;
 #pragma unroll
             for (int y = 0; y < kS / 32; ++y) {
-                tmem_ld_x32_sync(lanes + kTmS + half * kS + y * 32, x);
+                tmem_ld_x32_sync(lanes + kTmS + part * kS + y * 32, x);
 #pragma unroll
-                for (int i = 0; i < 32; ++i) s[y * 32 + i] = gamma * s[y * 32 + i] + vs.y * __uint_as_float(x[i]);
+                for (int i = 0; i < 16; ++i) s[y * 16 + i] = fma2_rn(f2(back, back), u2(x[2 * i], x[2 * i + 1]), s[y * 16 + i]);
             }
         }
-        output(chunks - 1);
         if (n < DV)
 #pragma unroll
-            for (int i = 0; i < kS; ++i) state[(half * kS + i) * DV + n] = s[i];
-    } else if (warp == 12) {
-        // ------------------------------------------------------------------------------- issuer of the chain's MMAs
-        if (lane == 0) {
-            constexpr uint32_t id64 = idesc_f16_f32(128, 64, false), id_d = idesc_f16_f32(128, DK, true);
-            for (int c = 0; c < chunks; ++c) {
-                const uint32_t par = c & 1;
-                GdnStage& st = sh.stage[c & 1];
-                const uint32_t kq = smem_u32(st.kq), thi = smem_u32(st.t_hi), tlo = smem_u32(st.t_lo), w = smem_u32(st.w);
-                wait(&sh.full[c & 1], (c >> 1) & 1, kStatusTimeoutFull);
-                wait(&sh.s_ready, par, kStatusTimeoutEmpty);
-                tc_fence_after();
-#pragma unroll
-                for (int e = 0; e < 2 * (DK / 16); ++e) {
-                    const int ks = e % (DK / 16);
-                    umma_f16_ts(tm + kTmXk, tm + kTmS + (e / (DK / 16)) * 64 + ks * 8,
-                                sw128_kmajor_desc(kq + (ks / 4) * 16384 + (ks % 4) * 32), id64, e > 0);
-                }
-                umma_commit(&sh.x_done);
-#pragma unroll
-                for (int ks = 0; ks < DK / 16; ++ks)
-                    umma_f16_ts(tm + kTmXq, tm + kTmS + ks * 8, sw128_kmajor_desc(kq + 8192 + (ks / 4) * 16384 + (ks % 4) * 32), id64,
-                                ks > 0);
-                wait(&sh.r_ready, par, kStatusTimeoutEmpty);
-                tc_fence_after();
-#pragma unroll
-                for (int e = 0; e < 12; ++e) {
-                    const int ks = e % 4, term = e / 4;      // hi hi, lo hi, hi lo
-                    umma_f16_ts(tm + kTmY, tm + kTmR + (term == 1 ? 32 : 0) + ks * 8,
-                                sw128_kmajor_desc((term == 2 ? tlo : thi) + ks * 32), id64, e > 0);
-                }
-                umma_commit(&sh.y_done);
-#pragma unroll
-                for (int ks = 0; ks < 4; ++ks)
-                    umma_f16_ts(tm + kTmW, tm + kTmR + ks * 8, sw128_kmajor_desc(w + ks * 32), id64, ks > 0);
-                wait(&sh.v_ready, par, kStatusTimeoutEmpty);
-                tc_fence_after();
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    umma_f16_ts(tm + kTmS, tm + kTmXk + (e / 4) * 32 + (e % 4) * 8, sw128_mn_desc(kq + (e % 4) * 2048, 16384), id_d,
-                                e > 0);
-                umma_commit(&sh.d_done);
+            for (int i = 0; i < kS / 2; ++i) {
+                float* at = state + (part * kS + 2 * i) * DV + n;
+                at[0] = f2_lo(s[i]), at[DV] = f2_hi(s[i]);
             }
-            // TMEM may be freed once the MMAs are done, also after a wait that expired
-            mbar_wait_bounded(&sh.d_done, (chunks - 1) & 1, limit_ns, nullptr);
-        }
-        __syncwarp();
-    } else {
-        // ---------------------------------------------------------------------------------- T and W of the chunks ahead
-        const int t = tid - 256, quarter = warp % 4, i = t % 64;      // lane t of TMEM: row i of k (t < 64) or q
-        const bool is_q = t >= 64, upper = (quarter & 1) != 0;        // upper: rows 32.. of the chunk
-        const uint32_t lanes = tm + (static_cast<uint32_t>(quarter * 32) << 16);
-        const __nv_bfloat16* kg = p.k + static_cast<long long>(r0) * p.ldk + hk * DK;
-        const __nv_bfloat16* qg = p.q + static_cast<long long>(r0) * p.ldq + hk * DK;
-        const __nv_bfloat16* vg = p.v + static_cast<long long>(r0) * p.ldv + hv * DV;
-        constexpr int kPieces = DK / 8;                               // 16-byte pieces of a row
-        auto load_kq = [&](int c) {
-#pragma unroll 4
-            for (int e = t; e < 128 * kPieces; e += 128) {
-                const int r = e / kPieces, x = e % kPieces, row = c * kChunk + r % 64;
-                const bool real = row < rows;
-                const __nv_bfloat16* src = r < 64 ? kg + (real ? row * p.ldk : 0) : qg + (real ? row * p.ldq : 0);
-                cp_async16_zfill(smem_u32(sh.raw) + r * (DK * 2) + x * 16, src + x * 8, real);
+        if (lane == 0) bulk_wait_all();
+    } else if (warp < 12) {
+        // ---------------------------------------------------------------------------------- T and P of the chunks ahead
+        const int l = lane;
+        const bool is_q = quarter >= 2, upper = (quarter & 1) != 0;   // upper: rows 32.. of the chunk
+        const int i = upper ? 32 + l : l;                             // this lane's row, of k (warps 8, 9) or q (10, 11)
+        auto piece = [&](int j) { return (j ^ (l & 7)); };
+        // [k; q] k^T of a chunk, once its tiles are there
+        auto products = [&](int c) {
+            if (lane == 0) {
+                GdnRows& in = sh.rows[c % kKqSlots];
+                wait(&sh.rows_full[c % kKqSlots], (c / kKqSlots) & 1, kStatusTimeoutFull);
+                if (c > 0) wait(&sh.kk_free, (c - 1) & 1, kStatusTimeoutAccEmpty);
+                tc_fence_after();
+                const uint64_t d = sw128_kmajor_desc(smem_u32(in.kq));
+#pragma unroll 1
+                for (int ks = 0; ks < DK / 16; ++ks) {
+                    const uint64_t y = d + (ks / 4) * 1024 + (ks % 4) * 2;
+                    umma_f16(tm + kTmPrep, y, y, idesc_f16_f32(128, 64, false), ks > 0);
+                }
+                umma_commit(&sh.kk_done);
             }
+            __syncwarp();
         };
-        load_kq(0);
-        for (int c = 0; c < chunks; ++c) {
+        if (warp == 8) products(0);
+#pragma unroll 1
+        for (int c = 0, slot_k = 0; c < chunks; ++c, slot_k = slot_k == kKqSlots - 1 ? 0 : slot_k + 1) {
             const uint32_t par = c & 1;
-            GdnStage& st = sh.stage[c & 1];
-            if (c >= kGdnStages) wait(&sh.empty[c & 1], ((c >> 1) - 1) & 1, kStatusTimeoutEmpty);
-#pragma unroll 4
-            for (int e = t; e < kChunk * (DV / 8); e += 128) {
-                const int r = e / (DV / 8), x = e % (DV / 8), row = c * kChunk + r;
-                const bool real = row < rows;
-                cp_async16_zfill(smem_u32(&st.v[r][x * 8]), vg + (real ? row * p.ldv : 0) + x * 8, real);
+            const GdnRows& in = sh.rows[slot_k];
+            GdnTiles& st = sh.tiles[par];
+            wait(&sh.rows_full[slot_k], (c / kKqSlots) & 1, kStatusTimeoutFull);
+            wait(&sh.kk_done, par, kStatusTimeoutAccFull);
+            if (c > 1) wait(&sh.tiles_free[par], ((c >> 1) - 1) & 1, kStatusTimeoutEmpty);
+            tc_fence_after();
+            const float g_hi = in.g_hi[i], g_lo = in.g_lo[i], row_k = in.row_k[i], beta = in.beta[i];
+            if (!is_q) named_bar_sync(5, 64);      // the chunk before has been solved: a11, a22 and a21 are free
+            // The row's products with the rows of k before it, with their decays, 8 at a time.  k and q have 2-norms below
+            // 2^14, so that products times kGdnDown fit fp16 (with room for a g above 0) and need no look at the row first:
+            // the scales of P's columns go with V', those of A[32.., ..31] with what it is multiplied by.
+#pragma unroll 1
+            for (int o = 0; o < (upper ? 64 : 32); o += 16) {
+                uint32_t x[16];
+                uint64_t y[8];
+                tmem_ld_x16_sync(lanes + kTmPrep + o, x);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const uint64_t h = sub2_rn(f2(g_hi, g_hi), *reinterpret_cast<const uint64_t*>(in.g_hi + o + 2 * e));
+                    const uint64_t d = add2_rn(h, sub2_rn(f2(g_lo, g_lo), *reinterpret_cast<const uint64_t*>(in.g_lo + o + 2 * e)));
+                    y[e] = mul2_rn(f2(ex2(f2_lo(d)), ex2(f2_hi(d))), u2(x[2 * e], x[2 * e + 1]));
+                }
+                if (is_q) {
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        uint32_t hi[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int at = o + 8 * q + 2 * e;
+                            const uint64_t w = mul2_rn(y[4 * q + e], f2(kGdnDown, kGdnDown));
+                            hi[e] = half2_bits(at <= i ? f2_lo(w) : 0.0f, at + 1 <= i ? f2_hi(w) : 0.0f);
+                        }
+                        *reinterpret_cast<uint4*>(st.p + i * 128 + piece(o / 8 + q) * 16) = uint4{hi[0], hi[1], hi[2], hi[3]};
+                    }
+                } else if (o < 32 && upper) {
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        uint32_t hi[4], lo[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) split2(y[4 * q + e], f2(kGdnDown, kGdnDown), hi[e], lo[e]);
+                        *reinterpret_cast<uint4*>(sh.a21[0] + l * 128 + piece(o / 8 + q) * 16) = uint4{hi[0], hi[1], hi[2], hi[3]};
+                        *reinterpret_cast<uint4*>(sh.a21[1] + l * 128 + piece(o / 8 + q) * 16) = uint4{lo[0], lo[1], lo[2], lo[3]};
+                    }
+                } else {
+                    const float f = -row_k * beta;
+                    float* a = (upper ? sh.a22 : sh.a11) + l * 32;
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+#pragma unroll
+                        for (int e = 2 * q; e < 2 * q + 2; ++e)
+                            y[e] = mul2_rn(y[e], mul2_rn(f2(f, f), *reinterpret_cast<const uint64_t*>(in.row_k + o + 2 * e)));
+                        *reinterpret_cast<ulonglong2*>(a + piece((o & 31) / 4 + q) * 4) = ulonglong2{y[2 * q], y[2 * q + 1]};
+                    }
+                }
             }
-            // running sums of g in log2 units: multiples of 2^-8 (exact in float32) and the rest, so that differences
-            // of far running sums keep their low bits; decays below 2^-128 count as 0
-            if (quarter == 0) {
-                float hi[2], lo[2], beta[2];
+            if (is_q) {
+                tc_fence_before();
+                if (!upper) {
+#pragma unroll
+                    for (int e = 4; e < 8; ++e) *reinterpret_cast<uint4*>(st.p + i * 128 + piece(e) * 16) = uint4{};
+                } else {
+                    asm volatile("bar.arrive 6, 64;" ::: "memory");     // columns 32.. may be written
+                }
+                const float f = in.row_q[i];
+                st.c_q[i] = f * ex2(g_hi + g_lo);
+                st.c_p[i] = f * kGdnUp;
+                if (i == 0) st.gamma = ex2(in.g_hi[kChunk - 1] + in.g_lo[kChunk - 1]);
+                fence_proxy_async_smem();
+                arrive(&sh.kk_free);
+                arrive(&sh.tiles_full[par]);
+                continue;
+            }
+            (upper ? sh.a22 : sh.a11)[l * 32 + piece(l / 4) * 4 + l % 4] = 0.0f;
+            if (!upper) {
+                tc_fence_before();
+                arrive(&sh.kk_free);
+            }
+            fence_proxy_async_smem();
+            uint64_t z[16], z1[16];                   // T's row: columns ..31 and 32..
+#pragma unroll
+            for (int j = 0; j < 16; ++j) z[j] = f2(2 * j == l ? 1.0f : 0.0f, 2 * j + 1 == l ? 1.0f : 0.0f), z1[j] = 0;
+            named_bar_sync(5, 64);
+#pragma unroll 1
+            for (int pass = upper ? 0 : 1; pass < 2; ++pass) {
+                solve32(z, pass == 0 ? sh.a22 : sh.a11);
+                if (pass == 0) {
+                    // z (columns 32..) is done; its product with A[32.., ..31] on the tensor cores, then columns ..31
+                    uint64_t y[16];
+                    float m = 0.0f;
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        y[j] = mul2_rn(z[j], mul2_rn(*reinterpret_cast<const uint64_t*>(in.beta + 32 + 2 * j),
+                                                     *reinterpret_cast<const uint64_t*>(in.row_k + 32 + 2 * j)));
+                        m = max3(m, y[j]);
+                    }
+                    const float2 f = scale_of(m);
+                    uint32_t hi[16], lo[16];
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) split2(y[j], f2(f.x, f.x), hi[j], lo[j]);
+                    tmem_st_x16(lanes + kTmPrep, hi);
+                    tmem_st_x16(lanes + kTmPrep + 16, lo);
+                    tmem_wait_st();
+                    tc_fence_before();
+                    asm volatile("bar.sync 6, 64;" ::: "memory");
+                    if (lane == 0) {
+                        tc_fence_after();
+#pragma unroll 1
+                        for (int e = 0; e < 6; ++e) {
+                            const int ks = e % 2, term = e / 2;
+                            umma_f16_ts(tm + kTmPrep + 32, tm + kTmPrep + (term == 1 ? 16 : 0) + ks * 8,
+                                        sw128_mn_desc(smem_u32(sh.a21[term == 2]) + ks * 2048, 4096), idesc_f16_f32(128, 32, true),
+                                        e > 0);
+                        }
+                        umma_commit(&sh.z_done);
+                    }
+                    __syncwarp();
+                    wait(&sh.z_done, par, kStatusTimeoutAccFull);
+                    tc_fence_after();
+                    uint32_t x[32];
+                    tmem_ld_x32_sync(lanes + kTmPrep + 32, x);
+                    tc_fence_before();
+                    arrive(&sh.kk_free);
+                    const float g = -f.y * kGdnUp;
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        z1[j] = z[j];
+                        z[j] = mul2_rn(u2(x[2 * j], x[2 * j + 1]), mul2_rn(f2(g, g), *reinterpret_cast<const uint64_t*>(in.row_k + 2 * j)));
+                    }
+                }
+            }
+            float m = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) m = max3(max3(m, z[j]), z1[j]);
+            const float2 f = scale_of(m);
+            st.c_x[i] = -row_k * beta * ex2(g_hi + g_lo);
+            st.c_b[i] = beta;
+            st.c_v[i] = row_k * ex2((in.g_hi[kChunk - 1] - g_hi) + (in.g_lo[kChunk - 1] - g_lo)) * f.y;
+            st.c_u[i] = row_k * f.y;
+#pragma unroll 1
+            for (int o = 0; o < 8; o += 4) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    uint32_t hi[4], lo[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) split2(z[4 * j + e], f2(f.x, f.x), hi[e], lo[e]);
+                    *reinterpret_cast<uint4*>(st.t_hi + i * 128 + piece(o + j) * 16) = uint4{hi[0], hi[1], hi[2], hi[3]};
+                    *reinterpret_cast<uint4*>(st.t_lo + i * 128 + piece(o + j) * 16) = uint4{lo[0], lo[1], lo[2], lo[3]};
+                }
+#pragma unroll
+                for (int j = 0; j < 16; ++j) z[j] = z1[j];
+            }
+            fence_proxy_async_smem();
+            arrive(&sh.tiles_full[par]);
+            if (warp == 8 && c + 1 < chunks) products(c + 1);
+        }
+        if (warp == 9 && lane == 0) mbar_wait_bounded(&sh.z_done, (chunks - 1) & 1, limit_ns, nullptr);
+        if (warp == 8 && lane == 0) mbar_wait_bounded(&sh.kk_done, (chunks - 1) & 1, limit_ns, nullptr);
+    } else {
+        if (warp == 12) {
+            // --------------------------------------------------------------------------- issuer of the chain's MMAs
+            if (lane == 0) {
+                constexpr uint32_t id64 = idesc_f16_f32(128, 64, false);
+                constexpr uint32_t id_d = idesc_f16_f32(128, DK, true);
+#pragma unroll 1
+                for (int c = 0, slot_k = 0; c < chunks; ++c, slot_k = slot_k == kKqSlots - 1 ? 0 : slot_k + 1) {
+                    const uint32_t par = c & 1;
+                    GdnTiles& st = sh.tiles[par];
+                    const uint32_t kq_at = smem_u32(sh.rows[slot_k].kq);
+                    const uint64_t kq = sw128_kmajor_desc(kq_at), kmn = sw128_mn_desc(kq_at, 16384);
+                    const uint64_t thi = sw128_kmajor_desc(smem_u32(st.t_hi)), tlo = sw128_kmajor_desc(smem_u32(st.t_lo));
+                    const uint64_t pd = sw128_kmajor_desc(smem_u32(st.p));
+                    wait(&sh.rows_full[slot_k], (c / kKqSlots) & 1, kStatusTimeoutFull);
+                    wait(&sh.s_ready, par, kStatusTimeoutEmpty);
+                    tc_fence_after();
+                    // descriptor addresses count in units of 16 bytes
+#pragma unroll 1
+                    for (int e = 0; e < 2 * (DK / 16); ++e) {
+                        const int ks = e % (DK / 16);
+                        umma_f16_ts(tm + kTmXk, tm + kTmS + (e / (DK / 16)) * 64 + ks * 8, kq + (ks / 4) * 1024 + (ks % 4) * 2, id64, e > 0);
+                    }
+                    umma_commit(&sh.x_done);
+                    // the chunk before's X_q has been read
+                    if (c > 0) wait(&sh.tiles_free[par ^ 1], ((c - 1) >> 1) & 1, kStatusTimeoutEmpty);
+                    tc_fence_after();
+#pragma unroll 1
+                    for (int ks = 0; ks < DK / 16; ++ks)
+                        umma_f16_ts(tm + kTmXq, tm + kTmS + ks * 8, kq + 512 + (ks / 4) * 1024 + (ks % 4) * 2, id64, ks > 0);
+                    wait(&sh.tiles_full[par], (c >> 1) & 1, kStatusTimeoutFull);
+                    wait(&sh.r_ready, par, kStatusTimeoutEmpty);
+                    tc_fence_after();
+#pragma unroll 1
+                    for (int e = 0; e < 12; ++e) {
+                        const int ks = e % 4, term = e / 4;      // hi hi, lo hi, hi lo
+                        umma_f16_ts(tm + kTmV, tm + kTmR + (term == 1 ? 32 : 0) + ks * 8, (term == 2 ? tlo : thi) + ks * 2, id64, e > 0);
+                    }
+                    umma_commit(&sh.v_done);
+                    wait(&sh.v_ready, par, kStatusTimeoutEmpty);
+                    tc_fence_after();
+#pragma unroll 1
+                    for (int e = 0; e < 8; ++e)
+                        umma_f16_ts(tm + kTmS, tm + kTmXk + (e / 4) * 32 + (e % 4) * 8, kmn + (e % 4) * 128, id_d, e > 0);
+                    umma_commit(&sh.d_done);
+                    umma_commit(&sh.rows_free[slot_k]);
+#pragma unroll 1
+                    for (int ks = 0; ks < 4; ++ks) umma_f16_ts(tm + kTmY, tm + kTmR + ks * 8, pd + ks * 2, id64, ks > 0);
+                    umma_commit(&sh.y_done);
+                }
+                // TMEM may be freed once the MMAs are done, also after a wait that expired
+                mbar_wait_bounded(&sh.y_done, (chunks - 1) & 1, limit_ns, nullptr);
+            }
+            __syncwarp();
+        } else {
+            // ----------------------------------------------------------------------------------------- rows in
+            const int t = tid - 13 * 32, w = warp - 13;
+            constexpr int kPieces = DK / 8;                               // 16-byte pieces of a row
+            const uint64_t policy = l2_policy_evict_normal();
+            auto load_kq = [&](int c, int slot_k) {
+                if (t == 0) {
+                    uint64_t* bar = &sh.kq_in[slot_k];
+                    fence_proxy_async_smem();
+                    mbar_arrive_expect_tx(bar, kChunk * 4 * DK);
+#pragma unroll 1
+                    for (int h = 0; h < DK / 64; ++h) {
+                        tma_load_2d(sh.rows[slot_k].kq[h], &maps.k, bar, hk * DK + h * 64, r0 + c * kChunk, policy);
+                        tma_load_2d(sh.rows[slot_k].kq[h] + kChunk * 128, &maps.q, bar, hk * DK + h * 64, r0 + c * kChunk, policy);
+                    }
+                }
+            };
+            auto gates = [&](int c, float (&g)[2], float (&beta)[2]) {
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     const int row = c * kChunk + lane * 2 + j;
                     const long long at = (static_cast<long long>(r0) + row) * p.v_heads + hv;
-                    const float g = row < rows ? p.g[at] * 1.44269504f : 0.0f;
+                    g[j] = row < rows ? p.g[at] : 0.0f;
                     beta[j] = row < rows ? p.beta[at] : 0.0f;
-                    const float x = g < -128.0f ? -128.0f : g;
-                    hi[j] = rintf(x * 256.0f) * 0.00390625f;
-                    lo[j] = x - hi[j];
                 }
-                float sh_ = hi[0] + hi[1], sl = lo[0] + lo[1];
+            };
+            // Each lane's pieces of its row, in an order that the row's number turns, so that the eight lanes of a
+            // shared-memory pass meet all banks.
+            int at[kPieces / 4];
 #pragma unroll
-                for (int m = 1; m < 32; m <<= 1) {
-                    const float a = __shfl_up_sync(0xFFFFFFFFu, sh_, m), l = __shfl_up_sync(0xFFFFFFFFu, sl, m);
-                    if (lane >= m) sh_ += a, sl += l;
-                }
-                sh.tok[lane * 2 + 1].x = sh_, sh.tok[lane * 2 + 1].y = sl, sh.tok[lane * 2 + 1].w = beta[1];
-                sh.tok[lane * 2].x = sh_ - hi[1], sh.tok[lane * 2].y = sl - lo[1], sh.tok[lane * 2].w = beta[0];
-                if (lane == 31) st.gamma = ex2(sh_ + sl);
+            for (int x = 0; x < kPieces / 4; ++x) {
+                const int r = lane / 4, y = ((x + r) % (kPieces / 4)) * 4 + lane % 4;
+                at[x] = (y / 8) * 16384 + r * 128 + ((y % 8) ^ r) * 16;
             }
-            cp_async_wait_all();
-            named_bar_sync(5, 128);
-            // k and q rows -> fp16 scaled to [2^13, 2^14): four lanes a row
+            load_kq(0, 0);
+            if (chunks > 1) load_kq(1, 1);
+            float g[2] = {}, beta[2] = {};
+            if (w == 0) gates(0, g, beta);
+#pragma unroll 1
+            for (int c = 0, slot_k = 0; c < chunks; ++c, slot_k = slot_k == kKqSlots - 1 ? 0 : slot_k + 1) {
+                const uint32_t par = c & 1;
+                GdnRows& in = sh.rows[slot_k];
+                // running sums of g in log2 units: multiples of 2^-8 (exact in float32) and the rest, so that differences
+                // of far running sums keep their low bits; decays below 2^-128 count as 0
+                if (w == 0) {
+                    float hi[2], lo[2];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const int r = quarter * 32 + u * 8 + lane / 4, c4 = lane % 4;
-                uint4 w[kPieces / 4];
-                uint32_t top = 0;
-                uint64_t sum = 0;
-#pragma unroll
-                for (int x = 0; x < kPieces / 4; ++x) {
-                    const int piece = ((x + r) % (kPieces / 4)) * 4 + c4;
-                    w[x] = *reinterpret_cast<const uint4*>(sh.raw + r * (DK * 2) + piece * 16);
-                    const uint32_t y[4] = {w[x].x, w[x].y, w[x].z, w[x].w};
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        top = __vmaxu2(top, y[j] & 0x7FFF7FFFu);
-                        const uint64_t f = bf16x2_to_f2(y[j]);
-                        sum = fma2_rn(f, f, sum);
+                    for (int j = 0; j < 2; ++j) {
+                        const float y = g[j] * 1.44269504f, x = y < -128.0f ? -128.0f : y;
+                        hi[j] = rintf(x * 256.0f) * 0.00390625f;
+                        lo[j] = x - hi[j];
                     }
-                }
-                top = max(top & 0xFFFFu, top >> 16);
-                float sq = f2_lo(sum) + f2_hi(sum);
-#pragma unroll
-                for (int m = 1; m < 4; m <<= 1) {
-                    top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, m));
-                    sq += __shfl_xor_sync(0xFFFFFFFFu, sq, m);
-                }
-                const float2 f = scale_of(__uint_as_float(top << 16));
-                const uint64_t f_2 = f2(f.x, f.x);
-#pragma unroll
-                for (int x = 0; x < kPieces / 4; ++x) {
-                    const int piece = ((x + r) % (kPieces / 4)) * 4 + c4;
-                    const uint32_t y[4] = {w[x].x, w[x].y, w[x].z, w[x].w};
-                    uint32_t o[4];
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const uint64_t g = mul2_rn(bf16x2_to_f2(y[j]), f_2);
-                        o[j] = half2_bits(f2_lo(g), f2_hi(g));
+                    float sum_h = hi[0] + hi[1], sum_l = lo[0] + lo[1];
+#pragma unroll 1
+                    for (int m = 1; m < 32; m <<= 1) {
+                        const float a = __shfl_up_sync(0xFFFFFFFFu, sum_h, m), x = __shfl_up_sync(0xFFFFFFFFu, sum_l, m);
+                        if (lane >= m) sum_h += a, sum_l += x;
                     }
-                    *reinterpret_cast<uint4*>(st.kq[piece / 8] + r * 128 + ((piece % 8) ^ (r % 8)) * 16) =
-                        uint4{o[0], o[1], o[2], o[3]};
+                    *reinterpret_cast<float2*>(in.g_hi + 2 * lane) = float2{sum_h - hi[1], sum_h};
+                    *reinterpret_cast<float2*>(in.g_lo + 2 * lane) = float2{sum_l - lo[1], sum_l};
+                    *reinterpret_cast<float2*>(in.beta + 2 * lane) = float2{beta[0], beta[1]};
+                    if (c + 1 < chunks) gates(c + 1, g, beta);
                 }
-                if (c4 == 0) {
-                    const float y = (p.normalize ? rsqrtf(sq + kGdnNormEps) : 1.0f) * f.y;
-                    if (r < 64) sh.tok[r].z = y;
-                    else sh.row_q[r - 64] = y * p.scale;
-                }
-            }
-            fence_proxy_async_smem();
-            named_bar_sync(5, 128);
-            if (t == 0) {
-                const uint32_t kq = smem_u32(st.kq);
-                tc_fence_after();
+                wait(&sh.kq_in[slot_k], (c / kKqSlots) & 1, kStatusTimeoutFull);
+                // k and q rows -> fp16 in their places, four lanes a row, scaled to a 2-norm in [2^13, 2^14) (a norm below
+                // 2^-60, whose square may underflow, counts as 2^-60); rows past the end, which the box takes from what
+                // follows, -> 0
+                const int left = rows - c * kChunk;
+                // (two groups of 8 rows at a time, whose latencies overlap; the last one may be done twice)
+#pragma unroll 1
+                for (int u0 = w; u0 < 16; u0 += 6) {
+                    uint4 raw[2][kPieces / 4];
+                    uint64_t sum[2] = {};
+                    float sq[2], f[2], back[2];
 #pragma unroll
-                for (int ks = 0; ks < DK / 16; ++ks) {
-                    const uint64_t d = sw128_kmajor_desc(kq + (ks / 4) * 16384 + (ks % 4) * 32);
-                    umma_f16(tm + kTmPrep, d, d, idesc_f16_f32(128, 64, false), ks > 0);
-                }
-                umma_commit(&sh.kk_done);
-            }
-            if (c + 1 < chunks) load_kq(c + 1);
-            const float4 me = sh.tok[i];
-            const float mine = is_q ? sh.row_q[i] : me.z * me.w;
-            wait(&sh.kk_done, par, kStatusTimeoutAccFull);
-            tc_fence_after();
-            // this row of A (k) or P (q), in two halves of 32 columns
-            uint64_t z1[16], z2[16];
-            {
-                uint32_t x[32];
-                float y[32];
-                tmem_ld_x32_sync(lanes + kTmPrep, x);
+                    for (int g2 = 0; g2 < 2; ++g2) {
+                        const uint8_t* row = in.kq[0] + (g2 && u0 + 3 < 16 ? u0 + 3 : u0) * 1024;
 #pragma unroll
-                for (int j = 0; j < 32; ++j) {
-                    const float4 o = sh.tok[j];
-                    const float d = ex2((me.x - o.x) + (me.y - o.y)) * (o.z * mine) * __uint_as_float(x[j]);
-                    y[j] = j < i || (is_q && j == i) ? d : 0.0f;
-                }
+                        for (int x = 0; x < kPieces / 4; ++x) raw[g2][x] = *reinterpret_cast<const uint4*>(row + at[x]);
+                    }
 #pragma unroll
-                for (int j = 0; j < 16; ++j) z1[j] = f2(y[2 * j], y[2 * j + 1]);
-                if (!is_q) {
-                    if (!upper) {
+                    for (int x = 0; x < kPieces / 4; ++x)
 #pragma unroll
-                        for (int j = 0; j < 8; ++j)
-                            *reinterpret_cast<float4*>(sh.a11 + i * 32 + (j ^ (i & 7)) * 4) =
-                                float4{y[4 * j], y[4 * j + 1], y[4 * j + 2], y[4 * j + 3]};
-                    } else {
-                        float m = 0.0f;
+                        for (int g2 = 0; g2 < 2; ++g2) {
+                            const uint32_t y[4] = {raw[g2][x].x, raw[g2][x].y, raw[g2][x].z, raw[g2][x].w};
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) m = fmaxf(m, fabsf(y[j]));
-                        const float2 f = scale_of(m);
-                        sh.a21_inv[i - 32] = f.y;
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            uint32_t hi[4], lo[4];
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) split2(y[8 * j + 2 * e] * f.x, y[8 * j + 2 * e + 1] * f.x, hi[e], lo[e]);
-                            const int at = (i - 32) * 128 + ((j ^ (i & 7)) * 16);
-                            *reinterpret_cast<uint4*>(sh.a21[0] + at) = uint4{hi[0], hi[1], hi[2], hi[3]};
-                            *reinterpret_cast<uint4*>(sh.a21[1] + at) = uint4{lo[0], lo[1], lo[2], lo[3]};
+                            for (int j = 0; j < 4; ++j) sum[g2] = fma2_rn(bf16x2_to_f2(y[j]), bf16x2_to_f2(y[j]), sum[g2]);
                         }
+#pragma unroll
+                    for (int g2 = 0; g2 < 2; ++g2) sq[g2] = f2_lo(sum[g2]) + f2_hi(sum[g2]);
+#pragma unroll
+                    for (int m = 1; m < 4; m <<= 1)
+#pragma unroll
+                        for (int g2 = 0; g2 < 2; ++g2) sq[g2] += __shfl_xor_sync(0xFFFFFFFFu, sq[g2], m);
+#pragma unroll
+                    for (int g2 = 0; g2 < 2; ++g2) {
+                        const int u = g2 && u0 + 3 < 16 ? u0 + 3 : u0, r = u * 8 + lane / 4;
+                        // 2^(k - 1) <= norm < 2^k
+                        const int k = static_cast<int>((max(__float_as_uint(sq[g2]) >> 23, 7u) + 1) >> 1) - 63;
+                        f[g2] = __uint_as_float(static_cast<uint32_t>(127 + 14 - k) << 23);
+                        back[g2] = __uint_as_float(static_cast<uint32_t>(127 - 14 + k) << 23);
+                        if (p.normalize) back[g2] *= rsqrtf(sq[g2] + kGdnNormEps);
+                        const bool real = r % 64 < left;
+                        if (!real) back[g2] = 0.0f;
+                        uint8_t* row = in.kq[0] + u * 1024;
+#pragma unroll
+                        for (int x = 0; x < kPieces / 4; ++x) {
+                            const uint32_t y[4] = {raw[g2][x].x, raw[g2][x].y, raw[g2][x].z, raw[g2][x].w};
+                            uint32_t o[4];
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) o[j] = real ? half2_of(mul2_rn(bf16x2_to_f2(y[j]), f2(f[g2], f[g2]))) : 0u;
+                            *reinterpret_cast<uint4*>(row + at[x]) = uint4{o[0], o[1], o[2], o[3]};
+                        }
+                        if (lane % 4 == 0) (r < 64 ? in.row_k : in.row_q - 64)[r] = r < 64 ? back[g2] : back[g2] * p.scale;
                     }
                 }
-                if (upper) {
-                    tmem_ld_x32_sync(lanes + kTmPrep + 32, x);
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) {
-                        const float4 o = sh.tok[32 + j];
-                        const float d = ex2((me.x - o.x) + (me.y - o.y)) * (o.z * mine) * __uint_as_float(x[j]);
-                        y[j] = 32 + j < i || (is_q && 32 + j == i) ? d : 0.0f;
-                    }
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) z2[j] = f2(y[2 * j], y[2 * j + 1]);
-                    if (!is_q)
-#pragma unroll
-                        for (int j = 0; j < 8; ++j)
-                            *reinterpret_cast<float4*>(sh.a22 + (i - 32) * 32 + (j ^ (i & 7)) * 4) =
-                                float4{y[4 * j], y[4 * j + 1], y[4 * j + 2], y[4 * j + 3]};
+                fence_proxy_async_smem();
+                arrive(&sh.rows_full[slot_k]);
+                if (t == 32) {
+                    if (c > 1) wait(&sh.v_free[par], ((c >> 1) - 1) & 1, kStatusTimeoutEmpty);
+                    fence_proxy_async_smem();
+                    mbar_arrive_expect_tx(&sh.v_in[par], kChunk * 2 * DV);
+                    tma_load_2d(sh.v[par], &maps.v, &sh.v_in[par], hv * DV, r0 + c * kChunk, policy);
+                }
+                __syncwarp();
+                if (c + 2 < chunks) {
+                    const int next = slot_k == 0 ? kKqSlots - 1 : slot_k - 1;          // (c + 2) % 3, chunk c - 1's
+                    if (w == 0 && c > 0) wait(&sh.rows_free[next], ((c - 1) / kKqSlots) & 1, kStatusTimeoutEmpty);
+                    load_kq(c + 2, next);
                 }
             }
-            if (!is_q) {                       // T starts from the identity
-#pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    z1[j] = f2(2 * j == i ? 1.0f : 0.0f, 2 * j + 1 == i ? 1.0f : 0.0f);
-                    z2[j] = f2(32 + 2 * j == i ? 1.0f : 0.0f, 33 + 2 * j == i ? 1.0f : 0.0f);
-                }
-            } else if (!upper) {
-#pragma unroll
-                for (int j = 0; j < 16; ++j) z2[j] = 0;
-            }
-            fence_proxy_async_smem();
-            tc_fence_before();
-            named_bar_sync(5, 128);
-            float z_inv = 0.0f;
-            if (upper) {
-                // the columns 32.. first, then their product with A[32.., ..31] on the tensor cores
-                solve32(z2, sh.a22);
-                float y[32], m = 0.0f;
-#pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    y[2 * j] = f2_lo(z2[j]) * sh.a21_inv[2 * j];
-                    y[2 * j + 1] = f2_hi(z2[j]) * sh.a21_inv[2 * j + 1];
-                    m = fmaxf(m, fmaxf(fabsf(y[2 * j]), fabsf(y[2 * j + 1])));
-                }
-                const float2 f = scale_of(m);
-                z_inv = f.y;
-                uint32_t hi[16], lo[16];
-#pragma unroll
-                for (int j = 0; j < 16; ++j) split2(y[2 * j] * f.x, y[2 * j + 1] * f.x, hi[j], lo[j]);
-                tmem_st_x16(lanes + kTmPrep, hi);
-                tmem_st_x16(lanes + kTmPrep + 16, lo);
-                tmem_wait_st();
-                tc_fence_before();
-            }
-            named_bar_sync(5, 128);
             if (t == 0) {
-                tc_fence_after();
-#pragma unroll
-                for (int e = 0; e < 6; ++e) {
-                    const int ks = e % 2, term = e / 2;
-                    umma_f16_ts(tm + kTmPrep + 32, tm + kTmPrep + (term == 1 ? 16 : 0) + ks * 8,
-                                sw128_mn_desc(smem_u32(sh.a21[term == 2]) + ks * 2048, 4096), idesc_f16_f32(128, 32, true), e > 0);
+                // no copy may be in flight when the block ends, also after a wait that expired
+                for (int c = max(chunks - 2, 0); c < chunks; ++c) {
+                    mbar_wait_bounded(&sh.kq_in[c % kKqSlots], (c / kKqSlots) & 1, limit_ns, nullptr);
+                    mbar_wait_bounded(&sh.v_in[c & 1], (c >> 1) & 1, limit_ns, nullptr);
                 }
-                umma_commit(&sh.z_done);
             }
-            if (upper) {
-                wait(&sh.z_done, par, kStatusTimeoutAccFull);
-                tc_fence_after();
-                uint32_t x[32];
-                tmem_ld_x32_sync(lanes + kTmPrep + 32, x);
-                tc_fence_before();
-#pragma unroll
-                for (int j = 0; j < 16; ++j)
-                    z1[j] = fma2_rn(f2(-z_inv, -z_inv), f2(__uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1])), z1[j]);
-            }
-            solve32(z1, sh.a11);
-            // columns times beta; a row of T in two terms, of W in one
-            float m = 0.0f;
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                z1[j] = mul2_rn(z1[j], f2(sh.tok[2 * j].w, sh.tok[2 * j + 1].w));
-                z2[j] = mul2_rn(z2[j], f2(sh.tok[32 + 2 * j].w, sh.tok[33 + 2 * j].w));
-                m = fmaxf(m, fmaxf(fmaxf(fabsf(f2_lo(z1[j])), fabsf(f2_hi(z1[j]))), fmaxf(fabsf(f2_lo(z2[j])), fabsf(f2_hi(z2[j])))));
-            }
-            const float2 f = scale_of(m);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                uint32_t hi[4], lo[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const uint64_t z = j < 4 ? z1[j * 4 + e] : z2[j * 4 + e - 16];
-                    split2(f2_lo(z) * f.x, f2_hi(z) * f.x, hi[e], lo[e]);
-                }
-                const int at = i * 128 + ((j ^ (i & 7)) * 16);
-                *reinterpret_cast<uint4*>((is_q ? st.w : st.t_hi) + at) = uint4{hi[0], hi[1], hi[2], hi[3]};
-                if (!is_q) *reinterpret_cast<uint4*>(st.t_lo + at) = uint4{lo[0], lo[1], lo[2], lo[3]};
-            }
-            const float4 last = sh.tok[kChunk - 1];
-            if (is_q) {
-                st.c[i].z = mine * ex2(me.x + me.y);
-                st.c[i].w = f.y;
-            } else {
-                st.c[i].x = me.z * ex2(me.x + me.y);
-                st.c[i].y = me.z * ex2((last.x - me.x) + (last.y - me.y)) * f.y;
-            }
-            fence_proxy_async_smem();
-            mbar_arrive(&sh.full[c & 1]);
-            // every lane has read tok, a11 and a22 before the next chunk's are written
-            named_bar_sync(5, 128);
         }
-        if (t == 0) mbar_wait_bounded(&sh.z_done, (chunks - 1) & 1, limit_ns, nullptr);
     }
     tc_fence_before();
     __syncthreads();
+    if (tid == 0 && sh.abort) atomicOr(&g_mixer_status, sh.abort);
     if (warp == 12) {
         tmem_relinquish();
         tmem_dealloc(tm, 512);
@@ -629,5 +838,6 @@ __global__ void __launch_bounds__(kChunkThreads, 1) gdn_chunk_kernel(const GdnPa
 }
 
 constexpr size_t gdn_chunk_smem() { return sizeof(GdnShared) + 1024; }
+static_assert(gdn_chunk_smem() <= 227 * 1024, "shared memory of one block");
 
 }  // namespace reax

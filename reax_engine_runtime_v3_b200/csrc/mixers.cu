@@ -66,13 +66,22 @@ int allow_smem(const void* kernel, std::atomic<bool> (&done)[kMaxDevices], size_
     return REAX_OK;
 }
 
+// The bound of device-side waits for kernels that keep it in 32 bits (at most 4 s).
+uint32_t wait_ns() { return static_cast<uint32_t>(std::min(reax_abi::wait_timeout_ns(), 4000000000ull)); }
+
 template <int DK, int DV>
 int gdn_chunks(const char* who, const reax::GdnParams& p, void* stream) {
     static std::atomic<bool> done[kMaxDevices];
-    const int rc = allow_smem(reinterpret_cast<const void*>(reax::gdn_chunk_kernel<DK, DV>), done, reax::gdn_chunk_smem());
+    int rc = allow_smem(reinterpret_cast<const void*>(reax::gdn_chunk_kernel<DK, DV>), done, reax::gdn_chunk_smem());
+    reax::GdnMaps maps;
+    if (rc == REAX_OK) rc = reax_abi::encode_rows(&maps.q, p.q, p.k_heads * DK, p.rows, p.ldq, 64, reax::kChunk, true);
+    if (rc == REAX_OK) rc = reax_abi::encode_rows(&maps.k, p.k, p.k_heads * DK, p.rows, p.ldk, 64, reax::kChunk, true);
+    if (rc == REAX_OK) rc = reax_abi::encode_rows(&maps.v, p.v, p.v_heads * DV, p.rows, p.ldv, DV, reax::kChunk, false);
+    if (rc == REAX_OK)
+        rc = reax_abi::encode_rows(&maps.out, p.out, p.v_heads * DV, p.rows, static_cast<long long>(p.v_heads) * DV, 32, 32, false);
     if (rc != REAX_OK) return rc;
     return launch(who, reax::gdn_chunk_kernel<DK, DV>, dim3(p.v_heads, p.batch), reax::kChunkThreads, reax::gdn_chunk_smem(),
-                  stream, p, reax_abi::wait_timeout_ns());
+                  stream, p, maps, wait_ns());
 }
 
 int gdn_rows(const char* who, const reax::GdnParams& p, int Dk, int Dv, void* stream) {
