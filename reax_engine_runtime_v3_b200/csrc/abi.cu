@@ -837,6 +837,22 @@ int encode_rows(CUtensorMap* map, const void* base, int cols, int rows, long lon
     return REAX_OK;
 }
 
+int encode_codes(CUtensorMap* map, const void* base, int dim, long long rows, int box_rows) {
+    PFN_cuTensorMapEncodeTiled_v12000 enc;
+    int rc = get_encoder(&enc);
+    if (rc != REAX_OK) return rc;
+    cuuint64_t dims[2] = {static_cast<cuuint64_t>(dim), static_cast<cuuint64_t>(rows)};
+    cuuint64_t strides[1] = {static_cast<cuuint64_t>(dim)};
+    cuuint32_t box[2] = {static_cast<cuuint32_t>(std::min(dim, 128)), static_cast<cuuint32_t>(box_rows)};
+    cuuint32_t estr[2] = {1, 1};
+    CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+                     CU_TENSOR_MAP_INTERLEAVE_NONE, dim == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                     CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS)
+        return fail(REAX_ERR_INVALID, "cuTensorMapEncodeTiled failed (%d) for %lld rows of %d codes", static_cast<int>(r), rows, dim);
+    return REAX_OK;
+}
+
 unsigned long long wait_timeout_ns() { return g_timeout_ns; }
 
 }  // namespace reax_abi

@@ -19,6 +19,9 @@ int device_sms(int device);
 // swizzle: the 128-byte one (box_cols 64).
 int encode_rows(CUtensorMap* map, const void* base, int cols, int rows, long long ld, int box_cols, int box_rows,
                 bool swizzle);
+// Tensor map of contiguous rows of `dim` (64, 128 or 256) 8-bit codes; boxes of min(dim, 128) codes by box_rows rows, 128-byte
+// swizzle (64-byte where dim is 64).
+int encode_codes(CUtensorMap* map, const void* base, int dim, long long rows, int box_rows);
 // Bound of device-side waits (reax_set_wait_timeout_ns).
 unsigned long long wait_timeout_ns();
 

@@ -222,48 +222,4 @@ struct Kv8Attend {
     float scale;
 };
 
-// One warp a row and query head, one cached row at a time; lane l holds elements l * D/32 .. of the row.
-template <int D>
-__global__ void __launch_bounds__(128) kv8_attend_rows_kernel(const Kv8Attend a) {
-    constexpr int kPer = D / 32;
-    const int lane = threadIdx.x % 32, hq = blockIdx.y, h = hq / a.group;
-    const int r = blockIdx.x * 4 + threadIdx.x / 32;
-    if (r >= a.rows) return;
-    int b = 0;
-    if (a.cu) {
-        int hi = a.batch;
-        while (hi - b > 1) {
-            const int mid = (b + hi) / 2;
-            if (a.cu[mid] <= r) b = mid; else hi = mid;
-        }
-    } else b = r;
-    int lo, hi;
-    kv8_span(a.cu, b, a.rows, &lo, &hi);
-    const int heads_q = a.c.heads * a.group;
-    const int seen = r < hi ? min(a.lengths[b] - (hi - lo) + (r - lo) + 1, a.table_ld * a.c.page) : 0;
-    float q[kPer], o[kPer] = {}, m = -INFINITY, l = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) q[i] = __bfloat162float(a.q[r * a.ldq + hq * D + lane * kPer + i]) * a.scale;
-    for (int t = 0; t < seen; ++t) {
-        const int id = a.tables[static_cast<long long>(b) * a.table_ld + t / a.c.page];
-        if (id < 0 || id >= a.c.pages) continue;
-        const long long at = static_cast<long long>(id) * a.c.heads + h;
-        const long long e = (at * a.c.page + t % a.c.page) * D + lane * kPer;
-        float s = 0.0f;
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) s += q[i] * static_cast<float>(a.c.k[e + i]);
-        s = warp_sum(s) * a.c.k_scale[at];
-        const float top = fmaxf(m, s), keep = __expf(m - top), w = __expf(s - top), ws = w * a.c.v_scale[at];
-        l = l * keep + w;
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) o[i] = o[i] * keep + ws * static_cast<float>(a.c.v[e + i]);
-        m = top;
-    }
-    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-    const long long at = static_cast<long long>(r) * heads_q + hq;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) a.out[at * D + lane * kPer + i] = __float2bfloat16_rn(o[i] * inv);
-    if (lane == 0 && a.lse) a.lse[at] = l > 0.0f ? m + logf(l) : -INFINITY;
-}
-
 }  // namespace reax

@@ -8,6 +8,7 @@
 #include "gdn.cuh"
 #include "gdn_chunk.cuh"
 #include "kv8.cuh"
+#include "kv8_step.cuh"
 #include "reax_b200.h"
 
 namespace {
@@ -111,6 +112,32 @@ int check_rows(const char* who, const int32_t* tables, const int32_t* lengths, c
     return REAX_OK;
 }
 
+// Workspace of the attention: counters (zero between calls), then the parts of items that blocks share.
+struct StepWorkspace {
+    reax::StepWork work;
+    size_t bytes;
+    StepWorkspace(void* base, int sms) {
+        const size_t blocks = static_cast<size_t>(sms) * reax::kStepBlocksPerSm;
+        const size_t counters = (blocks * sizeof(int) + 255) / 256 * 256;
+        const size_t stats = blocks * 2 * 2 * reax::kStepRows * sizeof(float);
+        char* p = static_cast<char*>(base);
+        work.counters = reinterpret_cast<int*>(p);
+        work.stats = reinterpret_cast<float*>(p + counters);
+        work.parts = reinterpret_cast<float*>(p + counters + stats);
+        bytes = counters + stats + blocks * 2 * reax::kStepRows * 256 * sizeof(float);
+    }
+};
+
+template <int D>
+int attend_step(const char* who, const reax::Kv8Attend& a, const reax::Kv8Maps& maps, void* workspace, int sms, void* stream) {
+    static std::atomic<bool> done[kMaxDevices];
+    constexpr size_t smem = sizeof(reax::StepShared<D>) + 1024;
+    const int rc = allow_smem(reinterpret_cast<const void*>(reax::kv8_step_kernel<D>), done, smem);
+    if (rc != REAX_OK) return rc;
+    return launch(who, reax::kv8_step_kernel<D>, dim3(sms * reax::kStepBlocksPerSm), reax::kAttendStepThreads, smem, stream, a, maps,
+                  StepWorkspace(workspace, sms).work, wait_ns());
+}
+
 }  // namespace
 
 extern "C" {
@@ -203,7 +230,7 @@ int reax_kv8_read(const int8_t* k_codes, const int8_t* v_codes, const float* k_s
 
 size_t reax_kv8_workspace_bytes(int device) {
     const int sms = reax_abi::device_sms(device);
-    return sms < 0 ? 0 : 256;
+    return sms < 0 ? 0 : StepWorkspace(nullptr, sms).bytes;
 }
 
 int reax_kv8_attend(const void* q, const int8_t* k_codes, const int8_t* v_codes, const float* k_scales,
@@ -225,10 +252,18 @@ int reax_kv8_attend(const void* q, const int8_t* k_codes, const int8_t* v_codes,
     if (!aligned(q, 16) || !aligned(out, 16) || ldq % 8)
         return fail(REAX_ERR_ALIGN, "%s: q and out must be 16-byte aligned, the row stride a multiple of 8", who);
     if ((rc = reax_abi::current_sms(&sms)) != REAX_OK) return rc;
-    const dim3 grid((rows + 3) / 4, heads * group);
-    if (dim == 64) return launch(who, reax::kv8_attend_rows_kernel<64>, grid, 128, 0, stream, a);
-    if (dim == 128) return launch(who, reax::kv8_attend_rows_kernel<128>, grid, 128, 0, stream, a);
-    return launch(who, reax::kv8_attend_rows_kernel<256>, grid, 128, 0, stream, a);
+    if (!workspace || workspace_bytes < StepWorkspace(nullptr, sms).bytes)
+        return fail(REAX_ERR_WORKSPACE, "%s: workspace of %zu bytes, needs reax_kv8_workspace_bytes() = %zu", who, workspace_bytes,
+                    StepWorkspace(nullptr, sms).bytes);
+    if (!aligned(workspace, 256)) return fail(REAX_ERR_ALIGN, "%s: the workspace must be 256-byte aligned", who);
+    const long long pool = static_cast<long long>(pages) * heads * page;
+    if (pool > 0x7FFFFFFF) return fail(REAX_ERR_INVALID, "%s: the pool has 2^31 rows or more", who);
+    reax::Kv8Maps maps;
+    if ((rc = reax_abi::encode_codes(&maps.k, k_codes, dim, std::max(pool, 16ll), 16)) != REAX_OK) return rc;
+    if ((rc = reax_abi::encode_codes(&maps.v, v_codes, dim, std::max(pool, 16ll), 16)) != REAX_OK) return rc;
+    if (dim == 64) return attend_step<64>(who, a, maps, workspace, sms, stream);
+    if (dim == 128) return attend_step<128>(who, a, maps, workspace, sms, stream);
+    return attend_step<256>(who, a, maps, workspace, sms, stream);
 }
 
 }  // extern "C"
