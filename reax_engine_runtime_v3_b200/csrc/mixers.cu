@@ -9,6 +9,7 @@
 #include "gdn_chunk.cuh"
 #include "kv8.cuh"
 #include "kv8_step.cuh"
+#include "kv8_tile.cuh"
 #include "reax_b200.h"
 
 namespace {
@@ -127,6 +128,22 @@ struct StepWorkspace {
         bytes = counters + stats + blocks * 2 * reax::kStepRows * 256 * sizeof(float);
     }
 };
+
+// Rows x heads of a sequence up to which the step form is used: it reads the cache once for each 16 of them.
+constexpr int kStepMostRows = 32;
+
+template <int D>
+int attend_tiles(const char* who, const reax::Kv8Attend& a, const reax::Kv8Maps& maps, void* stream) {
+    static std::atomic<bool> done[kMaxDevices];
+    constexpr size_t smem = std::min<size_t>(sizeof(reax::TileShared<D>) + 1024, 227 * 1024);
+    static_assert(sizeof(reax::TileShared<D>) <= smem, "shared memory of one block");
+    const int rc = allow_smem(reinterpret_cast<const void*>(reax::kv8_tile_kernel<D>), done, smem);
+    if (rc != REAX_OK) return rc;
+    // the most items that any split of the rows over the batch gives
+    const long long items = static_cast<long long>(a.rows) * a.group / reax::kTileRows + std::min(a.rows, a.batch);
+    return launch(who, reax::kv8_tile_kernel<D>, dim3(static_cast<unsigned>(items), a.c.heads), reax::kAttendTileThreads, smem, stream, a,
+                  maps, wait_ns());
+}
 
 template <int D>
 int attend_step(const char* who, const reax::Kv8Attend& a, const reax::Kv8Maps& maps, void* workspace, int sms, void* stream) {
@@ -261,6 +278,11 @@ int reax_kv8_attend(const void* q, const int8_t* k_codes, const int8_t* v_codes,
     reax::Kv8Maps maps;
     if ((rc = reax_abi::encode_codes(&maps.k, k_codes, dim, std::max(pool, 16ll), 16)) != REAX_OK) return rc;
     if ((rc = reax_abi::encode_codes(&maps.v, v_codes, dim, std::max(pool, 16ll), 16)) != REAX_OK) return rc;
+    if (static_cast<long long>(max_rows) * group > kStepMostRows) {
+        if (dim == 64) return attend_tiles<64>(who, a, maps, stream);
+        if (dim == 128) return attend_tiles<128>(who, a, maps, stream);
+        return attend_tiles<256>(who, a, maps, stream);
+    }
     if (dim == 64) return attend_step<64>(who, a, maps, workspace, sms, stream);
     if (dim == 128) return attend_step<128>(who, a, maps, workspace, sms, stream);
     return attend_step<256>(who, a, maps, workspace, sms, stream);
