@@ -1,20 +1,23 @@
 // Attention of many query rows over the paged INT8 cache (a prompt's chunk), on tcgen05 tensor cores.
 //
 // A block takes 128 query rows (rows x heads that share a cached head) and goes through the cache in tiles of 64 rows with a
-// running maximum and denominator.  Codes come through TMA, are turned into bf16 (exact) by warps of their own into
-// swizzled tiles, and serve as the B operands: K-major for the scores S = Q K^T, MN-major for O += P V.  S and P alternate
-// between two places in TMEM, where O stays in float32.
+// running maximum and denominator.  Codes come through TMA, are turned into fp16 (k) or bf16 (v), both exact, by warps of
+// their own into swizzled tiles, and serve as the B operands: K-major for the scores S = Q K^T, MN-major for O += P V.  q and P are the A
+// operands, in TMEM, where O stays in float32.
 //
-// Precision.  q is bf16 as it comes.  A weight is split into two bf16 numbers, hi + lo (2^-17), whose exponents reach as far as
+// Precision.  q becomes fp16 times a power of two for each row (its 8 bits fit); with it k can be fp16, which takes half the
+// instructions of bf16 to make from codes.  A weight is split into two bf16 numbers, hi + lo (cut, not rounded: 2^-15), whose exponents reach as far as
 // float32's: a single bf16 would lose half the output's bits again, and fp16 the weights below 2^-28 of the largest.
 //
-// What bounds it: 64 x 128 scores cost 1024 tensor cycles at 256 values a head (N = 64 runs at half rate), O 1024 with
-// both terms, and the softmax, the split and the codes' conversion about as much on the other pipes; the roles overlap.
+// What bounds it: 128 x 64 scores cost about 1000 tensor cycles at 256 values a head (an MMA of N = 64 takes 60 cycles with
+// its A operand in TMEM, and twice that with q read from shared memory beside the conversion's traffic: q lives in TMEM), O
+// another 1000 with both terms; the softmax, the split and the codes' conversion take the other pipes about as long.  The
+// roles overlap.
 //
 // Scaling O (in TMEM) costs as much as a tile, so the reference that the exponents are taken from moves only when a maximum
 // exceeds it by 8 (in log2): weights stay below 2^8, which bf16 holds as well as any.
 //
-// Roles (16 warps): 0-7 softmax (thread = row and half of the columns), 8-11 and 14-15 codes to bf16, 12 MMAs, 13 loads.
+// Roles (16 warps): 0-7 softmax (thread = row and half of the columns), 8-11 and 14-15 codes to 16 bits, 12 MMAs, 13 loads.
 #pragma once
 
 #include "common.cuh"
@@ -27,15 +30,14 @@ namespace reax {
 constexpr int kTileRows = 128, kTileCols = 64;
 constexpr int kAttendTileThreads = 16 * 32;
 constexpr int kConverters = 6;                // warps
-constexpr uint32_t kTmO = 0, kTmScore = 256, kTmWeight = 384;
+constexpr uint32_t kTmO = 0, kTmQ = 256, kTmScore = 384, kTmWeight = 448;
 
 template <int D>
 struct TileShared {
-    uint8_t q[kTileRows * D * 2];             // [D / 64][128 rows][64 values], 128-byte swizzle
-    uint8_t k[2][kTileCols * D * 2], v[2][kTileCols * D * 2];
-    uint8_t codes[2][kTileCols * D];          // of k and v as they come: 16 rows after 16 rows
+    uint8_t k[2][kTileCols * D * 2], v[2][kTileCols * D * 2];   // [D / 64][64 rows][64 values], 128-byte swizzle
+    uint8_t codes[2][2][kTileCols * D];       // of k and v as they come, two tiles: 16 rows after 16 rows
     float xch[2][8][32];
-    uint64_t in[2], in_free[2], k_full[2], v_full[2], s_full[2], s_free[2], p_full[2], pv_done[2];
+    uint64_t in[2][2], in_free[2][2], k_full[2], v_full[2], k_free[2], v_free[2], s_full, s_free, p_full, pv_done;
     uint32_t tmem;
     uint32_t abort;
 };
@@ -57,15 +59,10 @@ REAX_DEVI uint32_t codes_bf162(uint32_t x) {
 template <int D>
 __global__ void __launch_bounds__(kAttendTileThreads, 1)
     kv8_tile_kernel(const __grid_constant__ Kv8Attend a, const __grid_constant__ Kv8Maps maps, uint32_t limit_ns) {
-    // The array starts on a swizzle atom (256 columns leave no room to round its address up); checked all the same.
-    extern __shared__ __align__(1024) uint8_t tile_smem[];
-    TileShared<D>& sh = *reinterpret_cast<TileShared<D>*>(tile_smem);
-    if (smem_u32(tile_smem) & 1023u) {
-        if (threadIdx.x == 0) atomicOr(&g_mixer_status, static_cast<unsigned>(kStatusPlanLimit));
-        return;
-    }
+    extern __shared__ uint8_t tile_smem[];
+    TileShared<D>& sh = *reinterpret_cast<TileShared<D>*>(tile_smem + (-smem_u32(tile_smem) & 1023u));
     const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32, quarter = warp % 4;
-    const int heads = a.c.heads, page = a.c.page, h = blockIdx.y;
+    const int heads = a.c.heads, page = a.c.page, shift = __ffs(page) - 1, h = blockIdx.y;
     // the sequence and the 128 rows of block x: items of the sequences one after the other
     int b = -1, item = 0;
     for (int b0 = 0, before = 0; b0 < a.batch; b0 += 32) {
@@ -110,22 +107,14 @@ __global__ void __launch_bounds__(kAttendTileThreads, 1)
     if (warp == 12) tmem_alloc(&sh.tmem, 512);
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&sh.in[i], 1), mbar_init(&sh.in_free[i], kConverters);
+            for (int e = 0; e < 2; ++e) mbar_init(&sh.in[i][e], 1), mbar_init(&sh.in_free[i][e], kConverters);
             mbar_init(&sh.k_full[i], kConverters), mbar_init(&sh.v_full[i], kConverters);
-            mbar_init(&sh.s_full[i], 1), mbar_init(&sh.s_free[i], 8), mbar_init(&sh.p_full[i], 8), mbar_init(&sh.pv_done[i], 1);
+            mbar_init(&sh.k_free[i], 1), mbar_init(&sh.v_free[i], 1);
         }
+        mbar_init(&sh.s_full, 1), mbar_init(&sh.s_free, 8), mbar_init(&sh.p_full, 8), mbar_init(&sh.pv_done, 1);
         sh.abort = 0;
         fence_mbar_init();
     }
-    // q
-    for (int e = tid; e < kTileRows * (D / 8); e += kAttendTileThreads) {
-        const int r = e / (D / 8), x = e % (D / 8), i = first + r;
-        uint4 w = {};
-        if (r < live) w = *reinterpret_cast<const uint4*>(a.q + (static_cast<long long>(seq.lo) + i / a.group) * a.ldq +
-                                                        (h * a.group + i % a.group) * D + x * 8);
-        *reinterpret_cast<uint4*>(sh.q + (x / 8) * (kTileRows * 128) + r * 128 + ((x % 8) ^ (r % 8)) * 16) = w;
-    }
-    fence_proxy_async_smem();
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -140,10 +129,7 @@ __global__ void __launch_bounds__(kAttendTileThreads, 1)
     if (warp < 8) {
         // ------------------------------------------------------------------------------------------------- softmax
         const int half = warp / 4, r = quarter * 32 + lane;
-        const int seen = r < live ? min(seq.len, a.lengths[b] - seq.rows + (first + r) / a.group + 1) : 0;
-        const int least = min(seq.len, a.lengths[b] - seq.rows + first / a.group + 1);     // what the first row sees
-        const float scale = a.scale * 1.44269504f;
-        float ref = -INFINITY, den = 0.0f;
+        float scale = a.scale * 1.44269504f;
         int turn = 0;
         auto row_max = [&](float m) {
             float* x = &sh.xch[turn][quarter * 2][lane];
@@ -152,6 +138,36 @@ __global__ void __launch_bounds__(kAttendTileThreads, 1)
             turn ^= 1;
             return fmaxf(x[0], x[32]);
         };
+        {
+            // q's row, half of it, into TMEM: two values a column, scaled to a largest in [2^13, 2^14)
+            const int i = first + min(r, live - 1);
+            const __nv_bfloat16* src = a.q + (static_cast<long long>(seq.lo) + i / a.group) * a.ldq + (h * a.group + i % a.group) * D + half * (D / 2);
+            uint32_t top = 0;
+#pragma unroll 4
+            for (int e = 0; e < D / 2; e += 8) {
+                const uint4 y = *reinterpret_cast<const uint4*>(src + e);
+                top = __vmaxu2(__vmaxu2(top, y.x & 0x7FFF7FFFu), __vmaxu2(y.y & 0x7FFF7FFFu, __vmaxu2(y.z & 0x7FFF7FFFu, y.w & 0x7FFF7FFFu)));
+            }
+            const float2 f = scale_of(row_max(__uint_as_float(max(top & 0xFFFFu, top >> 16) << 16)));
+            scale *= f.y;
+#pragma unroll 1
+            for (int e = 0; e < D / 2; e += 32) {
+                uint32_t w[16];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint4 y = *reinterpret_cast<const uint4*>(src + e + j * 8);
+                    w[4 * j] = half2_of(mul2_rn(bf16x2_to_f2(y.x), f2(f.x, f.x))), w[4 * j + 1] = half2_of(mul2_rn(bf16x2_to_f2(y.y), f2(f.x, f.x)));
+                    w[4 * j + 2] = half2_of(mul2_rn(bf16x2_to_f2(y.z), f2(f.x, f.x))), w[4 * j + 3] = half2_of(mul2_rn(bf16x2_to_f2(y.w), f2(f.x, f.x)));
+                }
+                tmem_st_x16(lanes + kTmQ + half * (D / 4) + e / 2, w);
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            arrive(&sh.s_free);
+        }
+        const int seen = r < live ? min(seq.len, a.lengths[b] - seq.rows + (first + r) / a.group + 1) : 0;
+        const int least = min(seq.len, a.lengths[b] - seq.rows + first / a.group + 1);     // what the first row sees
+        float ref = -INFINITY, den = 0.0f;
         // scales of this half's two runs of 16 rows: pages looked up two tiles ahead, scales fetched one ahead
         int id[2];
         float ks[2], vs[2];
@@ -160,7 +176,7 @@ __global__ void __launch_bounds__(kAttendTileThreads, 1)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int row = x * kTileCols + half * 32 + e * 16;
-                id[e] = x < tiles && row < seq.len ? table[row / page] : -1;
+                id[e] = x < tiles && row < seq.len ? table[row >> shift] : -1;
             }
         };
         auto fetch = [&]() {
@@ -177,19 +193,17 @@ __global__ void __launch_bounds__(kAttendTileThreads, 1)
         look_up(1);
 #pragma unroll 1
         for (int x = 0; x < tiles; ++x) {
-            const int buf = x & 1;
-            const uint32_t par = (x >> 1) & 1;
-            const float f[2] = {ks[0] * scale, ks[1] * scale}, inv[2] = {1.0f / vs[0], 1.0f / vs[1]}, add[2] = {lg2f(vs[0]), lg2f(vs[1])};
+            const float f[2] = {ks[0] * scale, ks[1] * scale}, inv[2] = {__fdividef(1.0f, vs[0]), __fdividef(1.0f, vs[1])}, add[2] = {lg2f(vs[0]), lg2f(vs[1])};
             const bool plain = in[0] && in[1] && x * kTileCols + half * 32 + 32 <= least;
             const bool have[2] = {in[0], in[1]};
             fetch();
             look_up(x + 2);
-            wait(&sh.s_full[buf], par, kStatusTimeoutAccFull);
+            wait(&sh.s_full, x & 1, kStatusTimeoutAccFull);
             tc_fence_after();
             uint32_t c[32];
-            tmem_ld_x32_sync(lanes + kTmScore + buf * kTileCols + half * 32, c);
+            tmem_ld_x32_sync(lanes + kTmScore + half * 32, c);
             tc_fence_before();
-            arrive(&sh.s_free[buf]);
+            arrive(&sh.s_free);
             float t[32], m = -INFINITY;
 #pragma unroll
             for (int i = 0; i < 32; ++i) t[i] = fmaf(__uint_as_float(c[i]), f[i / 16], add[i / 16]);
@@ -206,7 +220,7 @@ __global__ void __launch_bounds__(kAttendTileThreads, 1)
             if (__any_sync(0xFFFFFFFFu, move)) {
                 const float to = move ? m : ref, g = ref == -INFINITY ? 0.0f : ex2(ref - to);
                 if (x > 0) {
-                    wait(&sh.pv_done[buf ^ 1], ((x - 1) >> 1) & 1, kStatusTimeoutAccFull);
+                    wait(&sh.pv_done, (x - 1) & 1, kStatusTimeoutAccFull);
                     tc_fence_after();
 #pragma unroll 1
                     for (int e = half * (D / 2); e < (half + 1) * (D / 2); e += 16) {
@@ -229,30 +243,32 @@ __global__ void __launch_bounds__(kAttendTileThreads, 1)
                 sum[i / 16] += t[i];
             }
             den += sum[0] * inv[0] + sum[1] * inv[1];
-            // P's place is free once O has taken the tile before last
-            if (x > 1) wait(&sh.pv_done[buf], ((x >> 1) - 1) & 1, kStatusTimeoutAccFull);
+            // P's place is free once O has taken the tile before
+            if (x > 0) wait(&sh.pv_done, (x - 1) & 1, kStatusTimeoutAccFull);
             tc_fence_after();
 #pragma unroll
             for (int e = 0; e < 32; e += 16) {
                 uint32_t hi[8], lo[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const uint64_t y = f2(t[e + 2 * i], t[e + 2 * i + 1]);
-                    hi[i] = bf16x2_rn(y);
-                    lo[i] = bf16x2_rn(sub2_rn(y, bf16x2_to_f2(hi[i])));
+                    // upper halves, and upper halves of what they leave
+                    const uint32_t y0 = __float_as_uint(t[e + 2 * i]), y1 = __float_as_uint(t[e + 2 * i + 1]);
+                    hi[i] = __byte_perm(y0, y1, 0x7632);
+                    const uint64_t rest = sub2_rn(u2(y0, y1), u2(y0 & 0xFFFF0000u, y1 & 0xFFFF0000u));
+                    lo[i] = __byte_perm(static_cast<uint32_t>(rest), static_cast<uint32_t>(rest >> 32), 0x7632);
                 }
-                tmem_st_x8(lanes + kTmWeight + buf * 64 + half * 16 + e / 2, hi);
-                tmem_st_x8(lanes + kTmWeight + buf * 64 + 32 + half * 16 + e / 2, lo);
+                tmem_st_x8(lanes + kTmWeight + half * 16 + e / 2, hi);
+                tmem_st_x8(lanes + kTmWeight + 32 + half * 16 + e / 2, lo);
             }
             tmem_wait_st();
             tc_fence_before();
-            arrive(&sh.p_full[buf]);
+            arrive(&sh.p_full);
         }
         // out
         sh.xch[turn][quarter * 2 + half][lane] = den;
         named_bar_sync(1 + quarter, 64);
         den = sh.xch[turn][quarter * 2][lane] + sh.xch[turn][quarter * 2 + 1][lane];
-        wait(&sh.pv_done[(tiles - 1) & 1], ((tiles - 1) >> 1) & 1, kStatusTimeoutAccFull);
+        wait(&sh.pv_done, (tiles - 1) & 1, kStatusTimeoutAccFull);
         tc_fence_after();
         const float scale_out = den > 0.0f ? 1.0f / den : 0.0f;
         const int i = first + r;
@@ -273,37 +289,36 @@ __global__ void __launch_bounds__(kAttendTileThreads, 1)
     } else if (warp == 12) {
         // ---------------------------------------------------------------------------------------------------- MMAs
         if (lane == 0) {
-            constexpr uint32_t id_s = idesc_bf16_ts(128, kTileCols, false), id_o = idesc_bf16_ts(128, D, true);
-            const uint64_t qd = sw128_kmajor_desc(smem_u32(sh.q));
+            constexpr uint32_t id_s = idesc_f16_f32(128, kTileCols, false), id_o = idesc_bf16_ts(128, D, true);
 #pragma unroll 1
             for (int x = 0; x <= tiles; ++x) {
                 if (x < tiles) {
                     const int buf = x & 1;
                     const uint64_t kd = sw128_kmajor_desc(smem_u32(sh.k[buf]));
                     wait(&sh.k_full[buf], (x >> 1) & 1, kStatusTimeoutFull);
-                    if (x > 1) wait(&sh.s_free[buf], ((x >> 1) - 1) & 1, kStatusTimeoutAccEmpty);
+                    wait(&sh.s_free, x & 1, kStatusTimeoutAccEmpty);       // (first: q is there)
                     tc_fence_after();
 #pragma unroll 1
                     for (int ks = 0; ks < D / 16; ++ks)
-                        umma_f16(tm + kTmScore + buf * kTileCols, qd + (ks / 4) * (kTileRows * 8) + (ks % 4) * 2,
-                                 kd + (ks / 4) * (kTileCols * 8) + (ks % 4) * 2, id_s, ks > 0);
-                    umma_commit(&sh.s_full[buf]);
+                        umma_f16_ts(tm + kTmScore, tm + kTmQ + ks * 8, kd + (ks / 4) * (kTileCols * 8) + (ks % 4) * 2, id_s, ks > 0);
+                    umma_commit(&sh.s_full);
+                    umma_commit(&sh.k_free[buf]);
                 }
                 if (x > 0) {
                     const int y = x - 1, buf = y & 1;
                     const uint64_t vd = sw128_mn_desc(smem_u32(sh.v[buf]), kTileCols * 128);
                     wait(&sh.v_full[buf], (y >> 1) & 1, kStatusTimeoutFull);
-                    wait(&sh.p_full[buf], (y >> 1) & 1, kStatusTimeoutEmpty);
+                    wait(&sh.p_full, y & 1, kStatusTimeoutEmpty);
                     tc_fence_after();
 #pragma unroll 1
                     for (int e = 0; e < 8; ++e)
-                        umma_f16_ts(tm + kTmO, tm + kTmWeight + buf * 64 + (e / 4) * 32 + (e % 4) * 8, vd + (e % 4) * 128, id_o,
-                                    y > 0 || e > 0);
-                    umma_commit(&sh.pv_done[buf]);
+                        umma_f16_ts(tm + kTmO, tm + kTmWeight + (e / 4) * 32 + (e % 4) * 8, vd + (e % 4) * 128, id_o, y > 0 || e > 0);
+                    umma_commit(&sh.pv_done);
+                    umma_commit(&sh.v_free[buf]);
                 }
             }
             // TMEM may be freed once the MMAs are done, also after a wait that expired
-            mbar_wait_bounded(&sh.pv_done[(tiles - 1) & 1], ((tiles - 1) >> 1) & 1, limit_ns, nullptr);
+            mbar_wait_bounded(&sh.pv_done, (tiles - 1) & 1, limit_ns, nullptr);
         }
         __syncwarp();
     } else if (warp == 13) {
@@ -312,63 +327,76 @@ __global__ void __launch_bounds__(kAttendTileThreads, 1)
         int id = -1;
         auto look_up = [&](int x) {           // lane l < 4: rows 16 l .. of the tile
             const int row = x * kTileCols + lane * 16;
-            id = x < tiles && lane < 4 && row < seq.len ? table[row / page] : -1;
+            id = x < tiles && lane < 4 && row < seq.len ? table[row >> shift] : -1;
         };
         look_up(0);
 #pragma unroll 1
         for (int x = 0; x < tiles; ++x) {
             const bool in = id >= 0 && id < a.c.pages;
-            const int at = (id * heads + h) * page + (x * kTileCols + lane * 16) % page;
+            const int at = (id * heads + h) * page + ((x * kTileCols + lane * 16) & (page - 1)), buf = x & 1;
             const uint32_t have = __popc(__ballot_sync(0xFFFFFFFFu, in));
 #pragma unroll 1
             for (int e = 0; e < 2; ++e) {     // k, then v
-                if (x > 0) wait(&sh.in_free[e], (x - 1) & 1, kStatusTimeoutEmpty);
+                if (x > 1) wait(&sh.in_free[buf][e], ((x >> 1) - 1) & 1, kStatusTimeoutEmpty);
                 if (lane == 0) {
                     fence_proxy_async_smem();
-                    mbar_arrive_expect_tx(&sh.in[e], have * 16 * D);
+                    mbar_arrive_expect_tx(&sh.in[buf][e], have * 16 * D);
                 }
                 __syncwarp();
                 if (in)
 #pragma unroll
                     for (int d = 0; d < D; d += 128)
-                        tma_load_2d(sh.codes[e] + lane * 16 * D + d * 16, e ? &maps.v : &maps.k, &sh.in[e], d, at, policy);
+                        tma_load_2d(sh.codes[buf][e] + lane * 16 * D + d * 16, e ? &maps.v : &maps.k, &sh.in[buf][e], d, at, policy);
                 __syncwarp();
             }
             look_up(x + 1);
         }
         if (lane == 0) {
-            mbar_wait_bounded(&sh.in[0], (tiles - 1) & 1, limit_ns, nullptr);
-            mbar_wait_bounded(&sh.in[1], (tiles - 1) & 1, limit_ns, nullptr);
+            for (int x = max(tiles - 2, 0); x < tiles; ++x)
+                for (int e = 0; e < 2; ++e) mbar_wait_bounded(&sh.in[x & 1][e], (x >> 1) & 1, limit_ns, nullptr);
         }
         __syncwarp();
     } else {
         // ------------------------------------------------------------------------------------------- codes to bf16
-        const int w = warp < 12 ? warp - 8 : warp - 10;
+        // each scheduler gets a quarter of the work: warps 8 and 9 that of one, 10 and 14, 11 and 15 share that of one
+        const int begin = warp - 8, step = warp < 10 ? 4 : 8;
+        // this lane's place in 8 rows of 64 codes as they come, and in the tile
+        const int from = D == 64 ? step_at<64>(lane % 8, lane / 8 * 16) : (lane % 8) * 128 + ((lane / 8) ^ (lane % 8)) * 16;
+        const int into = (lane % 8) * 128 + ((lane / 8 * 2) ^ (lane % 8)) * 16;
 #pragma unroll 1
         for (int x = 0; x < tiles; ++x) {
             const int buf = x & 1;
 #pragma unroll 1
             for (int e = 0; e < 2; ++e) {
-                wait(&sh.in[e], x & 1, kStatusTimeoutFull);
+                wait(&sh.in[buf][e], (x >> 1) & 1, kStatusTimeoutFull);
                 // K's place is free once the scores of the tile before last are there, V's once O has taken it
-                if (x > 1) wait(e ? &sh.pv_done[buf] : &sh.s_full[buf], ((x >> 1) - 1) & 1, kStatusTimeoutEmpty);
+                if (x > 1) wait(e ? &sh.v_free[buf] : &sh.k_free[buf], ((x >> 1) - 1) & 1, kStatusTimeoutEmpty);
                 uint8_t* to = e ? sh.v[buf] : sh.k[buf];
                 // 8 rows by 4 pieces of 16 codes a warp and turn
-#pragma unroll 2
-                for (int u = w; u < (kTileCols / 8) * (D / 64); u += kConverters) {
-                    const int r = u / (D / 64) * 8 + lane % 8, p = u % (D / 64) * 4 + lane / 8;
-                    const uint4 y = *reinterpret_cast<const uint4*>(sh.codes[e] + (r / 16) * 16 * D + step_at<D>(r % 16, p * 16));
-                    uint8_t* row = to + (p / 4) * (kTileCols * 128) + r * 128;
-                    const int at = (p % 4) * 2;
-                    *reinterpret_cast<uint4*>(row + ((at ^ (r % 8)) * 16)) =
-                        uint4{codes_bf162<0x4140>(y.x), codes_bf162<0x4342>(y.x), codes_bf162<0x4140>(y.y), codes_bf162<0x4342>(y.y)};
-                    *reinterpret_cast<uint4*>(row + (((at + 1) ^ (r % 8)) * 16)) =
-                        uint4{codes_bf162<0x4140>(y.z), codes_bf162<0x4342>(y.z), codes_bf162<0x4140>(y.w), codes_bf162<0x4342>(y.w)};
-                }
+                auto convert = [&](auto pair) {
+#pragma unroll 4
+                    for (int u = begin; u < (kTileCols / 8) * (D / 64); u += step) {
+                        const int rb = u / (D / 64), pb = u % (D / 64);
+                        const uint8_t* src = D == 64 ? sh.codes[buf][e] + rb * 512 + from
+                                                     : sh.codes[buf][e] + (rb / 2) * (16 * D) + (rb % 2) * 1024 + (pb / 2) * 2048 + (from ^ (pb % 2 * 64));
+                        const uint4 y = *reinterpret_cast<const uint4*>(src);
+                        uint8_t* row = to + pb * (kTileCols * 128) + rb * 1024;
+                        uint32_t w[8];
+                        pair(y.x, w[0], w[1]), pair(y.y, w[2], w[3]), pair(y.z, w[4], w[5]), pair(y.w, w[6], w[7]);
+                        *reinterpret_cast<uint4*>(row + into) = uint4{w[0], w[1], w[2], w[3]};
+                        *reinterpret_cast<uint4*>(row + (into ^ 16)) = uint4{w[4], w[5], w[6], w[7]};
+                    }
+                };
+                if (e)
+                    convert([](uint32_t x, uint32_t& lo, uint32_t& hi) { lo = codes_bf162<0x4140>(x), hi = codes_bf162<0x4342>(x); });
+                else
+                    convert([](uint32_t x, uint32_t& lo, uint32_t& hi) {
+                        lo = codes_half2<0x4140>(x ^ 0x80808080u), hi = codes_half2<0x4342>(x ^ 0x80808080u);
+                    });
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) {
-                    mbar_arrive(&sh.in_free[e]);
+                    mbar_arrive(&sh.in_free[buf][e]);
                     mbar_arrive(e ? &sh.v_full[buf] : &sh.k_full[buf]);
                 }
             }

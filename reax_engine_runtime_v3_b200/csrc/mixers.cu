@@ -135,8 +135,8 @@ constexpr int kStepMostRows = 32;
 template <int D>
 int attend_tiles(const char* who, const reax::Kv8Attend& a, const reax::Kv8Maps& maps, void* stream) {
     static std::atomic<bool> done[kMaxDevices];
-    constexpr size_t smem = std::min<size_t>(sizeof(reax::TileShared<D>) + 1024, 227 * 1024);
-    static_assert(sizeof(reax::TileShared<D>) <= smem, "shared memory of one block");
+    constexpr size_t smem = sizeof(reax::TileShared<D>) + 1024;
+    static_assert(smem <= 227 * 1024, "shared memory of one block");
     const int rc = allow_smem(reinterpret_cast<const void*>(reax::kv8_tile_kernel<D>), done, smem);
     if (rc != REAX_OK) return rc;
     // the most items that any split of the rows over the batch gives
