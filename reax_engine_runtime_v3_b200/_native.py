@@ -99,8 +99,13 @@ def ptr(t: torch.Tensor | None) -> int | None:
     return t.data_ptr()
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def stream_handle(device: torch.device | None = None) -> int:
     """The current torch stream, as the reference passes it to cuLaunchKernel (reaxv2/gate_up.py:25-26)."""
+    if _raw_stream is not None and device is not None and device.index is not None:
+        return _raw_stream(device.index)      # the handle alone: a Stream object takes longer to make than a small launch
     return torch.cuda.current_stream(device).cuda_stream
 
 
@@ -120,6 +125,15 @@ def require_cuda(*tensors: torch.Tensor) -> None:
     for t in tensors:
         if t is not None and not t.is_cuda:
             raise RuntimeError("REAX B200 kernels take CUDA tensors only (no CPU path)")
+
+
+def require_one_device(*tensors: torch.Tensor) -> None:
+    """All tensors (None aside) on one GPU."""
+    index = tensors[0].get_device()
+    for t in tensors:
+        if t is not None and (t.get_device() != index or index < 0):
+            require_cuda(*tensors)
+            raise RuntimeError("REAX B200 kernels take tensors of one device")
 
 
 # ------------------------------------------------------------------------------------------------------ workspace

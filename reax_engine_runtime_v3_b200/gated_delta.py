@@ -19,40 +19,42 @@ from . import _native
 _WIDTHS = (64, 128)
 
 
+def _rows(x, name):
+    """Checks packed rows [rows, heads, width] of bf16, a row's heads one after the other, and returns their stride."""
+    assert x.dtype is torch.bfloat16, f"{name} is bf16"
+    n, heads, width = x.shape
+    s0, s1, s2 = x.stride()
+    assert s2 == 1 and (s1 == width or heads == 1), f"the heads of a row of {name} must lie one after the other"
+    return s0 if n > 1 else heads * width     # (torch leaves the stride of a dimension of one row undefined)
+
+
 def _check(q, k, v, g, beta, state, slots, out, batch):
-    """The checks that both forms share: shapes, types and layouts the kernels take; returns the output."""
-    assert q.dtype == k.dtype == v.dtype == torch.bfloat16, "q, k and v are bf16"
+    """The checks that both forms share: shapes, types and layouts the kernels take.  Returns the output, the row strides
+    of q, k and v and the sizes."""
     n, k_heads, dk = q.shape
     n_v, v_heads, dv = v.shape
     assert k.shape == q.shape and n_v == n, "q, k [rows, k_heads, Dk] and v [rows, v_heads, Dv] disagree"
     assert v_heads % k_heads == 0, "the value heads are a multiple of the key heads"
     assert dk in _WIDTHS and dv in _WIDTHS, "head widths are 64 or 128"
-    for t in (q, k, v):
-        _, heads, width = t.shape
-        _, s1, s2 = t.stride()
-        assert s2 == 1 and (s1 == width or heads == 1), "a row's heads must lie one after the other"
-    assert g.dtype == beta.dtype == torch.float32 and g.shape == beta.shape == (n, v_heads), \
+    strides = _rows(q, "q"), _rows(k, "k"), _rows(v, "v")
+    assert g.dtype is torch.float32 and beta.dtype is torch.float32 and g.shape == (n, v_heads) and beta.shape == (n, v_heads), \
         "g and beta are float32 [rows, v_heads]"
     assert g.is_contiguous() and beta.is_contiguous(), "g and beta must be contiguous"
-    assert state.dtype == torch.float32 and state.is_contiguous() and state.shape[1:] == (v_heads, dk, dv), \
+    n_slots, *rest = state.shape
+    assert state.dtype is torch.float32 and state.is_contiguous() and rest == [v_heads, dk, dv], \
         "state is contiguous float32 [slots, v_heads, Dk, Dv]"
     if slots is None:
-        assert len(state) >= batch, "fewer states than sequences"
+        assert n_slots >= batch, "fewer states than sequences"
     else:
-        assert slots.dtype == torch.int32 and slots.shape == (batch,) and slots.is_contiguous(), \
+        assert slots.dtype is torch.int32 and slots.shape == (batch,) and slots.is_contiguous(), \
             "slots is int32, one for each sequence"
     if out is None:
-        out = torch.empty((n, v_heads, dv), dtype=torch.bfloat16, device=q.device)
+        out = torch.empty_like(v)             # (contiguous: v's heads are)
     else:
-        assert out.dtype == torch.bfloat16 and out.shape == v.shape and out.is_contiguous(), \
+        assert out.dtype is torch.bfloat16 and out.shape == v.shape and out.is_contiguous(), \
             "out is contiguous bf16 [rows, v_heads, Dv]"
-    _native.require_cuda(q, k, v, g, beta, state, slots, out)
-    return out
-
-
-def _ld(t):
-    """Row stride of packed rows (torch leaves the stride of a dimension of one row undefined)."""
-    return t.stride(0) if len(t) > 1 else t.shape[1] * t.shape[2]
+    _native.require_one_device(q, k, v, g, beta, state, slots, out)
+    return out, strides, (k_heads, v_heads, dk, dv, n_slots)
 
 
 def prefill(q, k, v, g, beta, state, *, cu_seqlens=None, slots=None, carry=True, scale=None, normalize=True, out=None):
@@ -61,27 +63,26 @@ def prefill(q, k, v, g, beta, state, *, cu_seqlens=None, slots=None, carry=True,
     device; without it all rows are one sequence).  ``carry``: start from the states kept, else from zeros.
     ``normalize``: divide q and k by the root of their sum of squares first; ``scale`` is Dk ** -0.5 if not given.
     Returns out bf16 [rows, v_heads, Dv]; the states are updated in place."""
-    batch = 1 if cu_seqlens is None else len(cu_seqlens) - 1
-    out = _check(q, k, v, g, beta, state, slots, out, batch)
+    batch = 1 if cu_seqlens is None else cu_seqlens.shape[0] - 1
+    out, strides, sizes = _check(q, k, v, g, beta, state, slots, out, batch)
     if cu_seqlens is not None:
-        assert cu_seqlens.dtype == torch.int32 and cu_seqlens.dim() == 1 and cu_seqlens.is_contiguous(), \
+        assert cu_seqlens.dtype is torch.int32 and cu_seqlens.dim() == 1 and cu_seqlens.is_contiguous(), \
             "cu_seqlens is contiguous int32"
-        _native.require_cuda(cu_seqlens)
-    n, k_heads, dk = q.shape
+        _native.require_one_device(q, cu_seqlens)
     _native.check(_native.load().reax_gdn_prefill(
-        _native.ptr(q), _native.ptr(k), _native.ptr(v), _native.ptr(g), _native.ptr(beta), _native.ptr(state),
-        _native.ptr(cu_seqlens), _native.ptr(slots), _native.ptr(out), n, batch, k_heads, v.shape[1], dk, v.shape[2],
-        len(state), _ld(q), _ld(k), _ld(v), dk ** -0.5 if scale is None else scale, bool(normalize), bool(carry),
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), state.data_ptr(),
+        None if cu_seqlens is None else cu_seqlens.data_ptr(), None if slots is None else slots.data_ptr(), out.data_ptr(),
+        q.shape[0], batch, *sizes, *strides, sizes[2] ** -0.5 if scale is None else scale, normalize, carry,
         _native.stream_handle(q.device)))
     return out
 
 
 def decode(q, k, v, g, beta, state, *, slots=None, scale=None, normalize=True, out=None):
     """One row of each sequence, from the states kept: arguments and result as ``prefill``, row b is sequence b's."""
-    n, k_heads, dk = q.shape
-    out = _check(q, k, v, g, beta, state, slots, out, n)
+    n = q.shape[0]
+    out, strides, sizes = _check(q, k, v, g, beta, state, slots, out, n)
     _native.check(_native.load().reax_gdn_decode(
-        _native.ptr(q), _native.ptr(k), _native.ptr(v), _native.ptr(g), _native.ptr(beta), _native.ptr(state),
-        _native.ptr(slots), _native.ptr(out), n, k_heads, v.shape[1], dk, v.shape[2], len(state), _ld(q), _ld(k), _ld(v),
-        dk ** -0.5 if scale is None else scale, bool(normalize), _native.stream_handle(q.device)))
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), state.data_ptr(),
+        None if slots is None else slots.data_ptr(), out.data_ptr(), n, *sizes, *strides,
+        sizes[2] ** -0.5 if scale is None else scale, normalize, _native.stream_handle(q.device)))
     return out

@@ -16,16 +16,16 @@ DIMS = (64, 128, 256)
 
 
 def _ints(t, shape, name):
-    assert t.dtype == torch.int32 and t.shape == shape and t.is_contiguous(), f"{name} is contiguous int32 {shape}"
+    assert t.dtype is torch.int32 and t.shape == shape and t.is_contiguous(), f"{name} is contiguous int32 {shape}"
 
 
 def _rows(x, heads, dim, name):
     """Checks packed rows [rows, heads, dim] of bf16 and returns their row stride."""
-    assert x.dtype == torch.bfloat16 and x.dim() == 3 and x.shape[1:] == (heads, dim), \
-        f"{name} is bf16 [rows, {heads}, {dim}]"
-    _, s1, s2 = x.stride()
+    n, *rest = x.shape
+    assert x.dtype is torch.bfloat16 and rest == [heads, dim], f"{name} is bf16 [rows, {heads}, {dim}]"
+    s0, s1, s2 = x.stride()
     assert s2 == 1 and (s1 == dim or heads == 1), f"the heads of a row of {name} must lie one after the other"
-    return x.stride(0) if len(x) > 1 else heads * dim
+    return s0 if n > 1 else heads * dim       # (torch leaves the stride of a dimension of one row undefined)
 
 
 class Int8Cache:
@@ -36,12 +36,14 @@ class Int8Cache:
     def __init__(self, k, v, k_scale, v_scale):
         self.pages, self.heads, self.page, self.dim = k.shape
         assert self.page in PAGES and self.dim in DIMS, f"pages have {PAGES} rows, heads {DIMS} values"
-        assert k.dtype == v.dtype == torch.int8 and v.shape == k.shape, "codes are int8 [pages, heads, page, dim]"
-        assert k_scale.dtype == v_scale.dtype == torch.float32 and k_scale.shape == v_scale.shape == k.shape[:2], \
-            "scales are float32 [pages, heads]"
+        assert k.dtype is torch.int8 and v.dtype is torch.int8 and v.shape == k.shape, \
+            "codes are int8 [pages, heads, page, dim]"
+        two = (self.pages, self.heads)
+        assert k_scale.dtype is torch.float32 and v_scale.dtype is torch.float32 and k_scale.shape == two and \
+            v_scale.shape == two, "scales are float32 [pages, heads]"
         assert k.is_contiguous() and v.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous(), \
             "the cache must be contiguous"
-        _native.require_cuda(k, v, k_scale, v_scale)
+        _native.require_one_device(k, v, k_scale, v_scale)
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
 
     @classmethod
@@ -51,8 +53,7 @@ class Int8Cache:
         return cls(*codes, *[torch.zeros((pages, heads), dtype=torch.float32, device=device) for _ in "kv"])
 
     def _cache(self):
-        p = _native.ptr
-        return p(self.k), p(self.v), p(self.k_scale), p(self.v_scale)
+        return self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr()
 
     def _sequences(self, tables, counts, cu_seqlens, rows, name):
         batch, width = tables.shape
@@ -68,25 +69,26 @@ class Int8Cache:
         """Rows ``cu_seqlens[b]`` up to ``cu_seqlens[b + 1]`` of k and v (bf16 [rows, heads, dim]; without
         ``cu_seqlens`` row b alone) become sequence b's rows ``lengths[b]`` on.  ``lengths`` is not changed."""
         ldk, ldv = _rows(k, self.heads, self.dim, "k"), _rows(v, self.heads, self.dim, "v")
-        assert len(k) == len(v), "k and v have the same rows"
-        batch, width = self._sequences(tables, lengths, cu_seqlens, len(k), "lengths")
-        _native.require_cuda(k, v, tables, lengths, cu_seqlens)
-        p = _native.ptr
+        n = k.shape[0]
+        assert n == v.shape[0], "k and v have the same rows"
+        batch, width = self._sequences(tables, lengths, cu_seqlens, n, "lengths")
+        _native.require_one_device(self.k, k, v, tables, lengths, cu_seqlens)
         _native.check(_native.load().reax_kv8_append(
-            p(k), p(v), *self._cache(), p(tables), p(lengths), p(cu_seqlens), len(k), batch, width, self.pages, self.heads,
-            self.page, self.dim, ldk, ldv, _native.stream_handle(k.device)))
+            k.data_ptr(), v.data_ptr(), *self._cache(), tables.data_ptr(), lengths.data_ptr(),
+            None if cu_seqlens is None else cu_seqlens.data_ptr(), n, batch, width, self.pages, self.heads, self.page, self.dim,
+            ldk, ldv, _native.stream_handle(k.device)))
 
     def read(self, tables, starts, cu_seqlens, rows):
         """Sequence b's rows ``starts[b]`` on, ``cu_seqlens[b + 1] - cu_seqlens[b]`` of them and ``rows`` in all, as bf16
         k and v [rows, heads, dim]."""
         batch, width = self._sequences(tables, starts, cu_seqlens, rows, "starts")
         assert cu_seqlens is not None, "read needs cu_seqlens"
-        _native.require_cuda(tables, starts, cu_seqlens)
-        k, v = (torch.empty((rows, self.heads, self.dim), dtype=torch.bfloat16, device=self.k.device) for _ in "kv")
-        p = _native.ptr
+        _native.require_one_device(self.k, tables, starts, cu_seqlens)
+        k = torch.empty((rows, self.heads, self.dim), dtype=torch.bfloat16, device=self.k.device)
+        v = torch.empty_like(k)
         _native.check(_native.load().reax_kv8_read(
-            *self._cache(), p(tables), p(starts), p(cu_seqlens), p(k), p(v), rows, batch, width, self.pages, self.heads,
-            self.page, self.dim, _native.stream_handle(self.k.device)))
+            *self._cache(), tables.data_ptr(), starts.data_ptr(), cu_seqlens.data_ptr(), k.data_ptr(), v.data_ptr(), rows, batch,
+            width, self.pages, self.heads, self.page, self.dim, _native.stream_handle(self.k.device)))
         return k, v
 
     def attend(self, q, tables, lengths, *, cu_seqlens=None, max_rows=None, scale=None, return_lse=False, out=None):
@@ -101,18 +103,18 @@ class Int8Cache:
         ldq = _rows(q, heads_q, self.dim, "q")
         batch, width = self._sequences(tables, lengths, cu_seqlens, n, "lengths")
         if out is None:
-            out = torch.empty((n, heads_q, self.dim), dtype=torch.bfloat16, device=q.device)
+            out = torch.empty_like(q)         # (contiguous: q's heads are)
         else:
-            assert out.dtype == torch.bfloat16 and out.shape == q.shape and out.is_contiguous(), \
+            assert out.dtype is torch.bfloat16 and out.shape == q.shape and out.is_contiguous(), \
                 "out is contiguous bf16 like q"
-        _native.require_cuda(q, tables, lengths, cu_seqlens, out)
+        _native.require_one_device(self.k, q, tables, lengths, cu_seqlens, out)
         lse = torch.empty((n, heads_q), dtype=torch.float32, device=q.device) if return_lse else None
         if max_rows is None:
             max_rows = 1 if cu_seqlens is None else n
         ws = _native.kv8_workspace(q.device)
-        p = _native.ptr
         _native.check(_native.load().reax_kv8_attend(
-            p(q), *self._cache(), p(tables), p(lengths), p(cu_seqlens), p(out), p(lse), n, max_rows, batch, width,
-            self.pages, self.heads, heads_q // self.heads, self.page, self.dim, ldq,
+            q.data_ptr(), *self._cache(), tables.data_ptr(), lengths.data_ptr(),
+            None if cu_seqlens is None else cu_seqlens.data_ptr(), out.data_ptr(), None if lse is None else lse.data_ptr(), n,
+            max_rows, batch, width, self.pages, self.heads, heads_q // self.heads, self.page, self.dim, ldq,
             self.dim ** -0.5 if scale is None else scale, ws.data_ptr(), ws.numel(), _native.stream_handle(q.device)))
         return (out, lse) if return_lse else out
