@@ -54,6 +54,25 @@ REAX_DEVI int kv8_code(float x, float scale) {
     return q != q ? 0 : static_cast<int>(fminf(fmaxf(q, -127.0f), 127.0f));
 }
 
+// The codes of 4 values.  x times the scale's inverse is within 127 * 2^-22 of x / scale, so that it rounds to the same whole
+// number unless it lies that near to a half; those few, and what is not finite, take the division.
+REAX_DEVI uint32_t kv8_codes(float x0, float x1, float x2, float x3, float scale, float inv) {
+    constexpr float kRound = 12582912.0f;     // 1.5 * 2^23: a sum with it is rounded to a whole number, in its low bits
+    const float x[4] = {x0, x1, x2, x3};
+    uint32_t c[4];
+    bool sure = true;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float t = __fmaf_rn(x[i], inv, kRound);
+        sure = sure && fabsf(__fmaf_rn(x[i], inv, kRound - t)) <= 0.4999f;
+        c[i] = __float_as_uint(t);
+    }
+    if (!sure)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c[i] = static_cast<uint32_t>(kv8_code(x[i], scale));
+    return __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
+}
+
 // One block writes the new rows of one page, one head, of k (blockIdx.z = 0) or v (1).  Block x is the x-th
 // page touched, counted over the sequences in order: a warp's prefix sum over the batch finds whose it is,
 // so the host need not know the lengths.
@@ -109,7 +128,7 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const Kv8App
     const long long at = static_cast<long long>(id) * a.c.heads + h;
     int8_t* dst = (is_v ? a.c.v : a.c.k) + at * a.c.page * dim;
     float* scale = (is_v ? a.c.v_scale : a.c.k_scale) + at;
-    const int per_row = dim / 8, total = (to - from) * per_row;       // pieces of 8 values
+    const int per_row = dim / 8, row_shift = __ffs(per_row) - 1, total = (to - from) * per_row;       // pieces of 8 values
     constexpr int kHeld = 64 * 256 / 8 / kAppendThreads;              // a whole page of the largest size
     uint4 x[kHeld];
     float m = 0.0f;
@@ -117,7 +136,7 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const Kv8App
     for (int i = 0; i < kHeld; ++i) {
         const int e = tid + i * kAppendThreads;
         if (e < total) {
-            x[i] = *reinterpret_cast<const uint4*>(src + (e / per_row) * ld + (e % per_row) * 8);
+            x[i] = *reinterpret_cast<const uint4*>(src + (e >> row_shift) * ld + (e & (per_row - 1)) * 8);
             m = absmax_finite(absmax_finite(absmax_finite(absmax_finite(m, x[i].x), x[i].y), x[i].z), x[i].w);
         }
     }
@@ -130,18 +149,16 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const Kv8App
     for (int i = 1; i < kAppendThreads / 32; ++i) m = fmaxf(m, s_max[i]);
     const float now = fmaxf(was, __fdiv_rn(fmaxf(m, 1e-12f), 127.0f));
     if (tid == 0) *scale = now;
+    const float inv = __frcp_rn(now);
 #pragma unroll
     for (int i = 0; i < kHeld; ++i) {
         const int e = tid + i * kAppendThreads;
         if (e < total) {
-            const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-            uint32_t o[2] = {};
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float f = __uint_as_float(j % 2 ? w[j / 2] & 0xFFFF0000u : w[j / 2] << 16);
-                o[j / 4] |= (static_cast<uint32_t>(kv8_code(f, now)) & 0xFFu) << (8 * (j % 4));
-            }
-            *reinterpret_cast<uint2*>(dst + (from + e / per_row) * dim + (e % per_row) * 8) = uint2{o[0], o[1]};
+            auto lo = [](uint32_t w) { return __uint_as_float(w << 16); };
+            auto hi = [](uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); };
+            *reinterpret_cast<uint2*>(dst + (from + (e >> row_shift)) * dim + (e & (per_row - 1)) * 8) =
+                uint2{kv8_codes(lo(x[i].x), hi(x[i].x), lo(x[i].y), hi(x[i].y), now, inv),
+                      kv8_codes(lo(x[i].z), hi(x[i].z), lo(x[i].w), hi(x[i].w), now, inv)};
         }
     }
     if (now > was && from > 0) {
@@ -171,40 +188,51 @@ struct Kv8Read {
     int rows, batch, table_ld;
 };
 
-// 8 codes a thread; row r of the output belongs to the last sequence that starts at or before it.
+// A warp a row, 16 codes a lane and turn; row r of the output belongs to the last sequence that starts at or before it.
 __global__ void __launch_bounds__(256) kv8_read_kernel(const Kv8Read a) {
-    const int per_row = a.c.heads * a.c.dim / 8;
-    const long long total = static_cast<long long>(a.rows) * per_row;
+    const int lane = threadIdx.x % 32, shift = __ffs(a.c.page) - 1, dim_shift = __ffs(a.c.dim) - 1;
     const bool is_v = blockIdx.y != 0;
     const int8_t* codes = is_v ? a.c.v : a.c.k;
     const float* scales = is_v ? a.c.v_scale : a.c.k_scale;
     __nv_bfloat16* out = is_v ? a.v : a.k;
-    for (long long e = blockIdx.x * 256ll + threadIdx.x; e < total; e += gridDim.x * 256ll) {
-        const int r = static_cast<int>(e / per_row), x = static_cast<int>(e % per_row) * 8;
-        const int h = x / a.c.dim, d = x % a.c.dim;
+    const int width = a.c.heads << dim_shift;
+    for (int r = blockIdx.x * 8 + threadIdx.x / 32; r < a.rows; r += gridDim.x * 8) {
         int lo = 0, hi = a.batch;                                     // cu[lo] <= r < cu[hi]
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) / 2;
-            if (a.cu[mid] <= r) lo = mid; else hi = mid;
-        }
-        const int place = a.starts[lo] + r - a.cu[lo];
-        uint4 o = {};
-        if (place >= 0 && r < a.cu[a.batch] && place / a.c.page < a.table_ld) {
-            const int id = a.tables[static_cast<long long>(lo) * a.table_ld + place / a.c.page];
-            if (id >= 0 && id < a.c.pages) {
-                const long long at = static_cast<long long>(id) * a.c.heads + h;
-                const uint2 w = *reinterpret_cast<const uint2*>(codes + (at * a.c.page + place % a.c.page) * a.c.dim + d);
-                const float s = scales[at];
-                uint32_t y[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const uint32_t b = j < 2 ? w.x : w.y;
-                    y[j] = bf16x2_rn(f2(static_cast<int8_t>(b >> (16 * (j % 2))) * s, static_cast<int8_t>(b >> (16 * (j % 2) + 8)) * s));
-                }
-                o = uint4{y[0], y[1], y[2], y[3]};
+        if (a.batch > 1) {
+            // 32 places at a time: the lanes' comparisons narrow the range to a 32nd
+            while (hi - lo > 1) {
+                const int step = (hi - lo + 31) / 32, at = lo + lane * step;
+                const unsigned below = __ballot_sync(0xFFFFFFFFu, at < hi && (lane == 0 || a.cu[at] <= r));
+                const int last = 31 - __clz(below);
+                hi = min(hi, lo + (last + 1) * step);
+                lo += last * step;
             }
         }
-        *reinterpret_cast<uint4*>(out + r * static_cast<long long>(a.c.heads) * a.c.dim + x) = o;
+        const int place = a.starts[lo] + r - a.cu[lo];
+        int id = -1;
+        if (place >= 0 && r < a.cu[a.batch] && (place >> shift) < a.table_ld)
+            id = a.tables[static_cast<long long>(lo) * a.table_ld + (place >> shift)];
+        const bool in = id >= 0 && id < a.c.pages;
+        const long long first = static_cast<long long>(in ? id : 0) * a.c.heads;
+        for (int x = lane * 16; x < width; x += 512) {
+            const int h = x >> dim_shift;
+            uint4 o[2] = {};
+            if (in) {
+                const uint4 w = *reinterpret_cast<const uint4*>(codes + (((first + h) << shift) + (place & (a.c.page - 1))) * a.c.dim +
+                                                                (x & (a.c.dim - 1)));
+                const float s = scales[first + h];
+                const uint32_t c[4] = {w.x, w.y, w.z, w.w};
+                uint32_t y[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const uint32_t b = c[j / 2] >> (16 * (j % 2));
+                    y[j] = bf16x2_rn(f2(static_cast<int8_t>(b) * s, static_cast<int8_t>(b >> 8) * s));
+                }
+                o[0] = uint4{y[0], y[1], y[2], y[3]}, o[1] = uint4{y[4], y[5], y[6], y[7]};
+            }
+            uint4* to = reinterpret_cast<uint4*>(out + static_cast<long long>(r) * width + x);
+            to[0] = o[0], to[1] = o[1];
+        }
     }
 }
 

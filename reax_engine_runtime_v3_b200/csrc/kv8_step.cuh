@@ -507,18 +507,37 @@ __global__ void __launch_bounds__(kAttendStepThreads, kStepBlocksPerSm)
 #pragma unroll 1
                 for (int r = warp; r < live; r += 4) {
                     float m = -INFINITY, d = 0.0f, y[D / 32] = {};
-                    for (int w = w0; w <= w1; ++w) m = fmaxf(m, __ldcg(&work.stats[((2 * w + (w == w0)) * 2) * kStepRows + r]));
-#pragma unroll 4
-                    for (int w = w0; w <= w1; ++w) {
-                        const int slot = 2 * w + (w == w0);
-                        const float mw = __ldcg(&work.stats[slot * 2 * kStepRows + r]);
-                        const float fw = mw == -INFINITY ? 0.0f : ex2f(mw - m);
-                        d += fw * __ldcg(&work.stats[(slot * 2 + 1) * kStepRows + r]);
+                    for (int w = w0 + lane; w <= w1; w += 32) m = fmaxf(m, __ldcg(&work.stats[(2 * w + (w == w0)) * 2 * kStepRows + r]));
+                    m = warp_max(m);
+                    // 32 parts at a time: a lane has the factor of one
+#pragma unroll 1
+                    for (int first = w0; first <= w1; first += 32) {
+                        float f_lane = 0.0f, d_lane = 0.0f;
+                        if (first + lane <= w1) {
+                            const int slot = 2 * (first + lane) + (first + lane == w0);
+                            const float mw = __ldcg(&work.stats[slot * 2 * kStepRows + r]);
+                            f_lane = mw == -INFINITY ? 0.0f : ex2f(mw - m);
+                            d_lane = f_lane * __ldcg(&work.stats[(slot * 2 + 1) * kStepRows + r]);
+                        }
+                        d += warp_sum(d_lane);
+                        const int n_parts = min(32, w1 - first + 1);
+#pragma unroll 1
+                        for (int i0 = 0; i0 < n_parts; i0 += 8) {
+                            float2 z[8][D / 64];
 #pragma unroll
-                        for (int e = 0; e < D / 64; ++e) {
-                            const float2 z = __ldcg(reinterpret_cast<const float2*>(
-                                work.parts + (static_cast<long long>(slot) * kStepRows + r) * D + e * 64 + lane * 2));
-                            y[2 * e] += fw * z.x, y[2 * e + 1] += fw * z.y;
+                            for (int i = 0; i < 8; ++i)
+#pragma unroll
+                                for (int e = 0; e < D / 64; ++e) {
+                                    const int w = min(first + i0 + i, w1), slot = 2 * w + (w == w0);     // (past the end: factor 0)
+                                    z[i][e] = __ldcg(reinterpret_cast<const float2*>(
+                                        work.parts + (static_cast<long long>(slot) * kStepRows + r) * D + e * 64 + lane * 2));
+                                }
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) {
+                                const float fw = __shfl_sync(0xFFFFFFFFu, f_lane, i0 + i);
+#pragma unroll
+                                for (int e = 0; e < D / 64; ++e) y[2 * e] += fw * z[i][e].x, y[2 * e + 1] += fw * z[i][e].y;
+                            }
                         }
                     }
                     write_row(r, m, d, y);

@@ -240,8 +240,7 @@ int reax_kv8_read(const int8_t* k_codes, const int8_t* v_codes, const float* k_s
     if (!cu_seqlens || !k || !v) return fail(REAX_ERR_INVALID, "%s: NULL pointer", who);
     if (!aligned(k, 16) || !aligned(v, 16)) return fail(REAX_ERR_ALIGN, "%s: k and v must be 16-byte aligned", who);
     if ((rc = reax_abi::current_sms(&sms)) != REAX_OK) return rc;
-    const long long work = (static_cast<long long>(rows) * heads * dim / 8 + 255) / 256;
-    return launch(who, reax::kv8_read_kernel, dim3(static_cast<unsigned>(std::min<long long>(work, sms * 8ll)), 2), 256, 0,
+    return launch(who, reax::kv8_read_kernel, dim3(std::min((rows + 7) / 8, sms * 8), 2), 256, 0,
                   stream, a);
 }
 
