@@ -23,8 +23,8 @@
 // have 8 bits and are exact in one.  X_k, V' and D, which the state depends on, take all terms down to 2^-22; X_q and Y
 // only reach the bf16 output and take the hi terms.  Sums are float32.
 //
-// Roles (16 warps): 0-7 carry the state; 8-11 find T and P of the chunks ahead; 12 issues the chain's MMAs; 13-15 load
-// rows and turn k and q into fp16 tiles.  No role may spill: beside this much shared memory little is left of the L1
+// Roles (16 warps): 0-7 carry the state; 8-11 find T and P of the chunks ahead; 13 issues the chain's MMAs; 12, 14 and
+// 15 load rows and turn k and q into fp16 tiles (13 shares its scheduler with 9, which has the most to solve).  No role may spill: beside this much shared memory little is left of the L1
 // cache, and a spilled value comes back from L2.
 #pragma once
 
@@ -39,6 +39,7 @@ constexpr int kChunk = 64;
 constexpr int kChunkThreads = 16 * 32;
 constexpr int kKqSlots = 3;                   // chunks of k and q tiles in flight
 constexpr int kLoaders = 3 * 32;
+constexpr int kGdnSorted = 256;               // sequences up to which blocks take them in the order of their lengths
 constexpr float kGdnDown = 0x1p-20f, kGdnUp = 0x1p20f;
 
 // TMEM columns.  S hi and lo (64 each) share the columns of D, and the decayed V' hi and lo those of X_k, V' hi those of R:
@@ -81,6 +82,7 @@ struct GdnShared {
     float xch[2][8][32];
     uint64_t kq_in[kKqSlots], rows_full[kKqSlots], rows_free[kKqSlots], v_in[2], v_free[2], tiles_full[2], tiles_free[2];
     uint64_t s_ready, r_ready, v_ready, x_done, v_done, d_done, y_done, kk_done, kk_free, z_done;
+    int length[kGdnSorted], sequence;
     uint32_t tmem;
     uint32_t abort;
 };
@@ -226,8 +228,24 @@ __global__ void __launch_bounds__(kChunkThreads, 1) gdn_chunk_kernel(const __gri
     // (an offset into the array, not an integer made a pointer: the accesses stay known as shared-memory ones)
     GdnShared& sh = *reinterpret_cast<GdnShared*>(smem_raw + (-smem_u32(smem_raw) & 1023u));
     const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
-    const int hv = blockIdx.x, b = blockIdx.y, hk = hv / (p.v_heads / p.k_heads);
-    int r0, r1;
+    const int hv = blockIdx.x, hk = hv / (p.v_heads / p.k_heads);
+    int r0, r1, b = blockIdx.y;
+    if (gridDim.y > 1 && gridDim.y <= kGdnSorted) {
+        // blocks start in their order: the longest sequences first, so that no long one is left for the end
+        if (tid < p.batch) {
+            gdn_rows(p, tid, &r0, &r1);
+            sh.length[tid] = r1 - r0;
+        }
+        __syncthreads();
+        if (tid < p.batch) {
+            const int mine = sh.length[tid];
+            int rank = 0;
+            for (int i = 0; i < p.batch; ++i) rank += sh.length[i] > mine || (sh.length[i] == mine && i < tid);
+            if (rank == static_cast<int>(blockIdx.y)) sh.sequence = tid;
+        }
+        __syncthreads();
+        b = sh.sequence;
+    }
     gdn_rows(p, b, &r0, &r1);
     const int slot = gdn_slot(p, b), rows = r1 - r0, chunks = (rows + kChunk - 1) / kChunk;
     if (slot < 0) {
@@ -583,12 +601,12 @@ __global__ void __launch_bounds__(kChunkThreads, 1) gdn_chunk_kernel(const __gri
                     asm volatile("bar.sync 6, 64;" ::: "memory");
                     if (lane == 0) {
                         tc_fence_after();
-#pragma unroll 1
+                        const uint64_t hi_desc = sw128_mn_desc(smem_u32(sh.a21[0]), 4096), lo_desc = sw128_mn_desc(smem_u32(sh.a21[1]), 4096);
+#pragma unroll 2
                         for (int e = 0; e < 6; ++e) {
                             const int ks = e % 2, term = e / 2;
-                            umma_f16_ts(tm + kTmPrep + 32, tm + kTmPrep + (term == 1 ? 16 : 0) + ks * 8,
-                                        sw128_mn_desc(smem_u32(sh.a21[term == 2]) + ks * 2048, 4096), idesc_f16_f32(128, 32, true),
-                                        e > 0);
+                            umma_f16_ts(tm + kTmPrep + 32, tm + kTmPrep + (term == 1 ? 16 : 0) + ks * 8, (term == 2 ? lo_desc : hi_desc) + ks * 128,
+                                        idesc_f16_f32(128, 32, true), e > 0);
                         }
                         umma_commit(&sh.z_done);
                     }
@@ -635,7 +653,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) gdn_chunk_kernel(const __gri
         if (warp == 9 && lane == 0) mbar_wait_bounded(&sh.z_done, (chunks - 1) & 1, limit_ns, nullptr);
         if (warp == 8 && lane == 0) mbar_wait_bounded(&sh.kk_done, (chunks - 1) & 1, limit_ns, nullptr);
     } else {
-        if (warp == 12) {
+        if (warp == 13) {
             // --------------------------------------------------------------------------- issuer of the chain's MMAs
             if (lane == 0) {
                 constexpr uint32_t id64 = idesc_f16_f32(128, 64, false);
@@ -652,7 +670,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) gdn_chunk_kernel(const __gri
                     wait(&sh.s_ready, par, kStatusTimeoutEmpty);
                     tc_fence_after();
                     // descriptor addresses count in units of 16 bytes
-#pragma unroll 1
+#pragma unroll 4
                     for (int e = 0; e < 2 * (DK / 16); ++e) {
                         const int ks = e % (DK / 16);
                         umma_f16_ts(tm + kTmXk, tm + kTmS + (e / (DK / 16)) * 64 + ks * 8, kq + (ks / 4) * 1024 + (ks % 4) * 2, id64, e > 0);
@@ -661,13 +679,13 @@ __global__ void __launch_bounds__(kChunkThreads, 1) gdn_chunk_kernel(const __gri
                     // the chunk before's X_q has been read
                     if (c > 0) wait(&sh.tiles_free[par ^ 1], ((c - 1) >> 1) & 1, kStatusTimeoutEmpty);
                     tc_fence_after();
-#pragma unroll 1
+#pragma unroll 4
                     for (int ks = 0; ks < DK / 16; ++ks)
                         umma_f16_ts(tm + kTmXq, tm + kTmS + ks * 8, kq + 512 + (ks / 4) * 1024 + (ks % 4) * 2, id64, ks > 0);
                     wait(&sh.tiles_full[par], (c >> 1) & 1, kStatusTimeoutFull);
                     wait(&sh.r_ready, par, kStatusTimeoutEmpty);
                     tc_fence_after();
-#pragma unroll 1
+#pragma unroll 4
                     for (int e = 0; e < 12; ++e) {
                         const int ks = e % 4, term = e / 4;      // hi hi, lo hi, hi lo
                         umma_f16_ts(tm + kTmV, tm + kTmR + (term == 1 ? 32 : 0) + ks * 8, (term == 2 ? tlo : thi) + ks * 2, id64, e > 0);
@@ -675,12 +693,12 @@ __global__ void __launch_bounds__(kChunkThreads, 1) gdn_chunk_kernel(const __gri
                     umma_commit(&sh.v_done);
                     wait(&sh.v_ready, par, kStatusTimeoutEmpty);
                     tc_fence_after();
-#pragma unroll 1
+#pragma unroll 4
                     for (int e = 0; e < 8; ++e)
                         umma_f16_ts(tm + kTmS, tm + kTmXk + (e / 4) * 32 + (e % 4) * 8, kmn + (e % 4) * 128, id_d, e > 0);
                     umma_commit(&sh.d_done);
                     umma_commit(&sh.rows_free[slot_k]);
-#pragma unroll 1
+#pragma unroll 4
                     for (int ks = 0; ks < 4; ++ks) umma_f16_ts(tm + kTmY, tm + kTmR + ks * 8, pd + ks * 2, id64, ks > 0);
                     umma_commit(&sh.y_done);
                 }
@@ -690,7 +708,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) gdn_chunk_kernel(const __gri
             __syncwarp();
         } else {
             // ----------------------------------------------------------------------------------------- rows in
-            const int t = tid - 13 * 32, w = warp - 13;
+            const int w = warp == 12 ? 0 : warp - 13, t = w * 32 + lane;
             constexpr int kPieces = DK / 8;                               // 16-byte pieces of a row
             const uint64_t policy = l2_policy_evict_normal();
             auto load_kq = [&](int c, int slot_k) {

@@ -1,7 +1,7 @@
 // Attention of few query rows over the paged INT8 cache: a step of the serving loop.
 //
-// What bounds it is the cache's bytes, read once: k and v codes of a page and head come through TMA into shared memory
-// (128-byte swizzle), are turned into fp16 in registers (exact: |code| <= 128) and multiplied with mma.sync m16n8k16,
+// What bounds it is the cache's bytes, read once: k and v codes of a page and head are copied into shared memory (16-byte
+// pieces xor-ed with their row's number, against bank conflicts), are turned into fp16 in registers (exact: |code| <= 128) and multiplied with mma.sync m16n8k16,
 // whose 16 rows hold the query rows and heads that share a cached head.  tcgen05 tiles would be 128 rows high, all but
 // a few of them empty; at 16 rows the tensor cores need a third of the time that the bytes take.
 //
@@ -13,9 +13,10 @@
 // differ by more than 19, it multiplies such weights in passes of their own, times 2^29 each, and the outputs so far with
 // them: every weight then counts with its 11 bits, down to 2^-115 of the largest.
 //
-// Loads.  Each warp fetches its own 16 rows of a tile into its own ring, so that warps never wait for one another but to
-// join their parts; all registers then go to eight warps on an SM (a fifth warp for loads took 168 of the 255 away, and the
-// outputs of 256 columns spilled).
+// Loads.  Each warp fetches its own 16 rows of a tile into its own ring with asynchronous 16-byte copies, so that warps never
+// wait for one another but to join their parts, and all registers go to eight warps on an SM.  (A fifth warp for the loads
+// left 168 of 255 registers and the outputs of 256 columns spilled; boxes of 16 rows by TMA cost about 1100 cycles a tile to
+// issue: 141 us for 64 sequences with 261000 rows, where the copies take 134.)
 //
 // Work.  Tiles of 64 cached rows of every (sequence, cached head, 16 query rows) lie on one line, of which each block takes
 // an equal part: lengths need not be known on the host and long ones are split by themselves.  A part of an item that
@@ -39,15 +40,13 @@ template <int D>
 struct StepShared {
     static constexpr int kStages = D == 256 ? 2 : 4;
     uint8_t kv[kStages][4][2][16 * D];        // a warp's 16 rows of codes of k and v
-    float o[kStepRows][D + 4];                // parts of the output added up
+    float o[kStepRows][D + 16];               // parts of the output added up (columns in the order of step_col)
     __half q[kStepRows][D + 8];
     float q_scale[kStepRows];
     float4 meta[kStages][4];                  // of each 16 rows: scale of k, log2 and inverse of that of v, 1 if in the cache
     float stat[2][4][kStepRows];
     long long sum[4];
-    uint64_t full[kStages][4];
     int last;
-    uint32_t abort;
 };
 
 struct StepWork {
@@ -98,6 +97,9 @@ REAX_DEVI int step_at(int r, int x) {
     return (x / 128) * (16 * 128) + r * 128 + ((((x / 16) & 7) ^ (r & 7)) * 16) + x % 16;
 }
 
+// Place of column `col` in a row of parts: pieces of 4 columns in an order that spreads a warp's pieces over the banks.
+REAX_DEVI int step_col(int col) { return ((col / 4) ^ ((col / 32) & 3)) * 4 + col % 4; }
+
 REAX_DEVI void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -123,25 +125,16 @@ REAX_DEVI float lg2f(float x) {
     return y;
 }
 
-struct Kv8Maps {
-    CUtensorMap k, v;                         // rows of D bytes, boxes of min(D, 128) bytes by 16 rows
-};
-
 template <int D>
 __global__ void __launch_bounds__(kAttendStepThreads, kStepBlocksPerSm)
-    kv8_step_kernel(const __grid_constant__ Kv8Attend a, const __grid_constant__ Kv8Maps maps, const StepWork work, uint32_t limit_ns) {
+    kv8_step_kernel(const __grid_constant__ Kv8Attend a, const StepWork work) {
     using Shared = StepShared<D>;
     constexpr int kStages = Shared::kStages;
     extern __shared__ uint8_t step_smem[];
     Shared& sh = *reinterpret_cast<Shared*>(step_smem + (-smem_u32(step_smem) & 1023u));
     const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
-    const int heads = a.c.heads, page = a.c.page;
+    const int heads = a.c.heads, page = a.c.page, shift = __ffs(page) - 1;
 
-    if (tid == 0) {
-        for (int i = 0; i < kStages * 4; ++i) mbar_init(&sh.full[i / 4][i % 4], 1);
-        sh.abort = 0;
-        fence_mbar_init();
-    }
     // this block's part [u0, u1) of the line of tiles
     long long sum = 0;
     for (int b = tid; b < a.batch; b += kAttendStepThreads) sum += StepSeq(a, b).units(heads);
@@ -179,21 +172,8 @@ __global__ void __launch_bounds__(kAttendStepThreads, kStepBlocksPerSm)
     at_u.x = static_cast<int>((u0 - start) % at_u.s.tiles);
     at_u.item = static_cast<int>((u0 - start) / at_u.s.tiles % at_u.s.items);
     at_u.h = static_cast<int>((u0 - start) / at_u.s.tiles / at_u.s.items);
-    volatile uint32_t* abort = &sh.abort;
-    auto wait = [&](uint64_t* bar, uint32_t parity, uint32_t bit) {
-        if (mbar_try_wait_suspend(bar, parity, 2000u)) return;
-        uint32_t t0;
-        asm volatile("mov.u32 %0, %%globaltimer_lo;" : "=r"(t0));
-        while (!mbar_try_wait_suspend(bar, parity, 2000u)) {
-            uint32_t t;
-            asm volatile("mov.u32 %0, %%globaltimer_lo;" : "=r"(t));
-            if (*abort) return;
-            if (t - t0 > limit_ns) *abort = bit;
-        }
-    };
     // Loads of this warp's rows, kStages tiles ahead.  `ahead` is the tile to be loaded next and `id` its page (looked up one
     // load earlier); the scales of the tile loaded last arrive in registers and are put down at the next load.
-    const uint64_t policy = l2_policy_evict_first();
     StepCursor ahead = at_u;
     long long left = u1 - u0;                 // tiles not loaded yet
     int id = -1, fill = 0, put = -1;
@@ -201,37 +181,34 @@ __global__ void __launch_bounds__(kAttendStepThreads, kStepBlocksPerSm)
     bool in = false;
     auto look_up = [&]() {
         const int row = ahead.x * kStepTile + warp * 16;
-        id = row < ahead.s.len ? a.tables[static_cast<long long>(ahead.b) * a.table_ld + row / page] : -1;
+        id = row < ahead.s.len ? a.tables[static_cast<long long>(ahead.b) * a.table_ld + (row >> shift)] : -1;
     };
     auto put_down = [&]() {
-        if (put >= 0 && lane == 0) sh.meta[put][warp] = float4{ks, lg2f(vs), 1.0f / vs, in ? 1.0f : 0.0f};
+        if (put >= 0 && lane == 0) sh.meta[put][warp] = float4{ks, lg2f(vs), __fdividef(1.0f, vs), in ? 1.0f : 0.0f};
         put = -1;
     };
     auto load = [&]() {
         put_down();
-        if (left <= 0) return;
-        in = id >= 0 && id < a.c.pages;
-        ks = 0.0f, vs = 1.0f;
-        if (in) {
-            ks = a.c.k_scale[static_cast<long long>(id) * heads + ahead.h];
-            vs = fmaxf(a.c.v_scale[static_cast<long long>(id) * heads + ahead.h], 1e-30f);
-        }
-        put = fill;
-        if (lane == 0) {
-            uint64_t* bar = &sh.full[fill][warp];
-            fence_proxy_async_smem();
-            mbar_arrive_expect_tx(bar, in ? 2 * 16 * D : 0);
+        if (left > 0) {
+            in = id >= 0 && id < a.c.pages;
+            ks = 0.0f, vs = 1.0f;
             if (in) {
-                const int at = (id * heads + ahead.h) * page + (ahead.x * kStepTile + warp * 16) % page;
+                const long long at = static_cast<long long>(id) * heads + ahead.h;
+                ks = a.c.k_scale[at];
+                vs = fmaxf(a.c.v_scale[at], 1e-30f);
+                const long long first = ((at << shift) + ((ahead.x * kStepTile + warp * 16) & (page - 1))) * D + lane * 16;
 #pragma unroll
-                for (int e = 0; e < D; e += 128) {
-                    tma_load_2d(sh.kv[fill][warp][0] + e * 16, &maps.k, bar, e, at, policy);
-                    tma_load_2d(sh.kv[fill][warp][1] + e * 16, &maps.v, bar, e, at, policy);
+                for (int e = 0; e < 16 * D; e += 512) {
+                    const int to = step_at<D>((e + lane * 16) / D, (e + lane * 16) % D);
+                    cp_async16_cg(sh.kv[fill][warp][0] + to, a.c.k + first + e);
+                    cp_async16_cg(sh.kv[fill][warp][1] + to, a.c.v + first + e);
                 }
             }
+            put = fill;
+            if (++fill == kStages) fill = 0;
+            if (--left > 0 && ahead.next(a)) look_up();
         }
-        if (++fill == kStages) fill = 0;
-        if (--left > 0 && ahead.next(a)) look_up();
+        asm volatile("cp.async.commit_group;" ::: "memory");
     };
     look_up();
 #pragma unroll 1
@@ -245,7 +222,6 @@ __global__ void __launch_bounds__(kAttendStepThreads, kStepBlocksPerSm)
         const int perm = g ^ ((g & 1) << 2);                          // cached row of score column g: no bank conflicts
         const int v0 = 2 * q, v1 = (2 * q + 1) ^ 4;                   // cached rows behind weights 2q and 2q + 1
         int stage = 0;
-        uint32_t turn = 0;
         while (u < u1) {
             const StepSeq& s = at_u.s;
             const int b = at_u.b, h = at_u.h, at = at_u.item * kStepRows, from = at_u.x;
@@ -286,7 +262,8 @@ __global__ void __launch_bounds__(kAttendStepThreads, kStepBlocksPerSm)
             for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
 #pragma unroll 1
             for (int x = from; x < to; ++x) {
-                wait(&sh.full[stage][warp], turn & 1, kStatusTimeoutFull);
+                asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+                __syncwarp();
                 const float4 meta = sh.meta[stage][warp];
                 const uint8_t* kt = sh.kv[stage][warp][0];
                 const uint8_t* vt = sh.kv[stage][warp][1];
@@ -406,7 +383,7 @@ __global__ void __launch_bounds__(kAttendStepThreads, kStepBlocksPerSm)
                 __syncwarp();
                 load();
                 __syncwarp();
-                if (++stage == kStages) stage = 0, ++turn;
+                if (++stage == kStages) stage = 0;
             }
             u += to - from;
             at_u.x = to - 1;
@@ -428,18 +405,27 @@ __global__ void __launch_bounds__(kAttendStepThreads, kStepBlocksPerSm)
                 for (int w = 1; w < 4; ++w) m = fmaxf(m, sh.stat[0][w][g + 8 * i]);
                 f[i] = top[i] == -INFINITY ? 0.0f : ex2f(top[i] - m);
             }
+            constexpr int W = D == 64 ? 8 : 16;
+            const int live = min(kStepRows, s.rows * a.group - at);
 #pragma unroll 1
             for (int w = 0; w < 4; ++w) {
                 if (warp == w) {
-                    constexpr int W = D == 64 ? 8 : 16;
 #pragma unroll
-                    for (int i = 0; i < D / 8; ++i)
+                    for (int r = 0; r < 2; ++r)
+                        if (g + 8 * r < live)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int col = (i / W) * 8 * W + (2 * q + e % 2) * W + i % W;
-                            float& y = sh.o[g + 8 * (e / 2)][col];
-                            y = w == 0 ? o[i][e] * f[e / 2] : y + o[i][e] * f[e / 2];
-                        }
+                            for (int blk = 0; blk < D / (8 * W); ++blk)
+#pragma unroll
+                                for (int e = 0; e < 2; ++e)
+#pragma unroll
+                                    for (int j = 0; j < W; j += 4) {
+                                        const float(*x)[4] = o + blk * W + j;
+                                        const int k = 2 * r + e;
+                                        float4& y = *reinterpret_cast<float4*>(&sh.o[g + 8 * r][step_col(blk * 8 * W + (2 * q + e) * W + j)]);
+                                        float4 z = w == 0 ? float4{} : y;
+                                        z.x += x[0][k] * f[r], z.y += x[1][k] * f[r], z.z += x[2][k] * f[r], z.w += x[3][k] * f[r];
+                                        y = z;
+                                    }
                 }
                 __syncthreads();
             }
@@ -462,7 +448,6 @@ __global__ void __launch_bounds__(kAttendStepThreads, kStepBlocksPerSm)
                     *reinterpret_cast<uint32_t*>(a.out + row * D + e * 64 + lane * 2) = bf16x2_rn(f2(y[2 * e] * inv, y[2 * e + 1] * inv));
                 if (lane == 0 && a.lse) a.lse[row] = d > 0.0f ? 0.69314718f * (m + log2f(d)) : -INFINITY;
             };
-            const int live = min(kStepRows, s.rows * a.group - at);
             if (whole) {
 #pragma unroll 1
                 for (int r = warp; r < live; r += 4) {
@@ -470,7 +455,7 @@ __global__ void __launch_bounds__(kAttendStepThreads, kStepBlocksPerSm)
                     row_stat(r, &m, &d);
 #pragma unroll
                     for (int e = 0; e < D / 64; ++e) {
-                        const float2 z = *reinterpret_cast<const float2*>(&sh.o[r][e * 64 + lane * 2]);
+                        const float2 z = *reinterpret_cast<const float2*>(&sh.o[r][step_col(e * 64 + lane * 2)]);
                         y[2 * e] = z.x, y[2 * e + 1] = z.y;
                     }
                     write_row(r, m, d, y);
@@ -492,7 +477,7 @@ __global__ void __launch_bounds__(kAttendStepThreads, kStepBlocksPerSm)
 #pragma unroll
                 for (int e = 0; e < D / 64; ++e)
                     __stcg(reinterpret_cast<float2*>(work.parts + (static_cast<long long>(part) * kStepRows + r) * D + e * 64 + lane * 2),
-                           *reinterpret_cast<const float2*>(&sh.o[r][e * 64 + lane * 2]));
+                           *reinterpret_cast<const float2*>(&sh.o[r][step_col(e * 64 + lane * 2)]));
             }
             __threadfence();
             __syncthreads();
@@ -522,10 +507,10 @@ __global__ void __launch_bounds__(kAttendStepThreads, kStepBlocksPerSm)
                         d += warp_sum(d_lane);
                         const int n_parts = min(32, w1 - first + 1);
 #pragma unroll 1
-                        for (int i0 = 0; i0 < n_parts; i0 += 8) {
-                            float2 z[8][D / 64];
+                        for (int i0 = 0; i0 < n_parts; i0 += 16) {
+                            float2 z[16][D / 64];
 #pragma unroll
-                            for (int i = 0; i < 8; ++i)
+                            for (int i = 0; i < 16; ++i)
 #pragma unroll
                                 for (int e = 0; e < D / 64; ++e) {
                                     const int w = min(first + i0 + i, w1), slot = 2 * w + (w == w0);     // (past the end: factor 0)
@@ -533,7 +518,7 @@ __global__ void __launch_bounds__(kAttendStepThreads, kStepBlocksPerSm)
                                         work.parts + (static_cast<long long>(slot) * kStepRows + r) * D + e * 64 + lane * 2));
                                 }
 #pragma unroll
-                            for (int i = 0; i < 8; ++i) {
+                            for (int i = 0; i < 16; ++i) {
                                 const float fw = __shfl_sync(0xFFFFFFFFu, f_lane, i0 + i);
 #pragma unroll
                                 for (int e = 0; e < D / 64; ++e) y[2 * e] += fw * z[i][e].x, y[2 * e + 1] += fw * z[i][e].y;
@@ -546,11 +531,6 @@ __global__ void __launch_bounds__(kAttendStepThreads, kStepBlocksPerSm)
             if (u < u1) at_u.next(a);
         }
     }
-    // (no copy is in flight: each has been waited for, unless a wait expired)
-    if (sh.abort && lane == 0)
-        for (int i = 0; i < kStages; ++i) mbar_wait_bounded(&sh.full[i][warp], 0, limit_ns, nullptr), mbar_wait_bounded(&sh.full[i][warp], 1, limit_ns, nullptr);
-    __syncthreads();
-    if (tid == 0 && sh.abort) atomicOr(&g_mixer_status, sh.abort);
 }
 
 }  // namespace reax

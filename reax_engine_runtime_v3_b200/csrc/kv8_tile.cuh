@@ -32,6 +32,10 @@ constexpr int kAttendTileThreads = 16 * 32;
 constexpr int kConverters = 6;                // warps
 constexpr uint32_t kTmO = 0, kTmQ = 256, kTmScore = 384, kTmWeight = 448;
 
+struct Kv8Maps {
+    CUtensorMap k, v;                         // rows of D bytes, boxes of min(D, 128) bytes by 16 rows
+};
+
 template <int D>
 struct TileShared {
     uint8_t k[2][kTileCols * D * 2], v[2][kTileCols * D * 2];   // [D / 64][64 rows][64 values], 128-byte swizzle

@@ -146,13 +146,13 @@ int attend_tiles(const char* who, const reax::Kv8Attend& a, const reax::Kv8Maps&
 }
 
 template <int D>
-int attend_step(const char* who, const reax::Kv8Attend& a, const reax::Kv8Maps& maps, void* workspace, int sms, void* stream) {
+int attend_step(const char* who, const reax::Kv8Attend& a, void* workspace, int sms, void* stream) {
     static std::atomic<bool> done[kMaxDevices];
     constexpr size_t smem = sizeof(reax::StepShared<D>) + 1024;
     const int rc = allow_smem(reinterpret_cast<const void*>(reax::kv8_step_kernel<D>), done, smem);
     if (rc != REAX_OK) return rc;
-    return launch(who, reax::kv8_step_kernel<D>, dim3(sms * reax::kStepBlocksPerSm), reax::kAttendStepThreads, smem, stream, a, maps,
-                  StepWorkspace(workspace, sms).work, wait_ns());
+    return launch(who, reax::kv8_step_kernel<D>, dim3(sms * reax::kStepBlocksPerSm), reax::kAttendStepThreads, smem, stream, a,
+                  StepWorkspace(workspace, sms).work);
 }
 
 }  // namespace
@@ -272,19 +272,19 @@ int reax_kv8_attend(const void* q, const int8_t* k_codes, const int8_t* v_codes,
         return fail(REAX_ERR_WORKSPACE, "%s: workspace of %zu bytes, needs reax_kv8_workspace_bytes() = %zu", who, workspace_bytes,
                     StepWorkspace(nullptr, sms).bytes);
     if (!aligned(workspace, 256)) return fail(REAX_ERR_ALIGN, "%s: the workspace must be 256-byte aligned", who);
-    const long long pool = static_cast<long long>(pages) * heads * page;
-    if (pool > 0x7FFFFFFF) return fail(REAX_ERR_INVALID, "%s: the pool has 2^31 rows or more", who);
-    reax::Kv8Maps maps;
-    if ((rc = reax_abi::encode_codes(&maps.k, k_codes, dim, std::max(pool, 16ll), 16)) != REAX_OK) return rc;
-    if ((rc = reax_abi::encode_codes(&maps.v, v_codes, dim, std::max(pool, 16ll), 16)) != REAX_OK) return rc;
     if (static_cast<long long>(max_rows) * group > kStepMostRows) {
+        const long long pool = static_cast<long long>(pages) * heads * page;
+        if (pool > 0x7FFFFFFF) return fail(REAX_ERR_INVALID, "%s: the pool has 2^31 rows or more", who);
+        reax::Kv8Maps maps;
+        if ((rc = reax_abi::encode_codes(&maps.k, k_codes, dim, std::max(pool, 16ll), 16)) != REAX_OK) return rc;
+        if ((rc = reax_abi::encode_codes(&maps.v, v_codes, dim, std::max(pool, 16ll), 16)) != REAX_OK) return rc;
         if (dim == 64) return attend_tiles<64>(who, a, maps, stream);
         if (dim == 128) return attend_tiles<128>(who, a, maps, stream);
         return attend_tiles<256>(who, a, maps, stream);
     }
-    if (dim == 64) return attend_step<64>(who, a, maps, workspace, sms, stream);
-    if (dim == 128) return attend_step<128>(who, a, maps, workspace, sms, stream);
-    return attend_step<256>(who, a, maps, workspace, sms, stream);
+    if (dim == 64) return attend_step<64>(who, a, workspace, sms, stream);
+    if (dim == 128) return attend_step<128>(who, a, workspace, sms, stream);
+    return attend_step<256>(who, a, workspace, sms, stream);
 }
 
 }  // extern "C"
