@@ -48,69 +48,6 @@ REAX_DEVI void gdn_rows(const GdnParams& p, int b, int* begin, int* end) {
     *end = hi;
 }
 
-// ---------------------------------------------------------------------------------------------- row by row
-// One warp carries 4 columns of a head's state through the rows of a sequence: lane l holds rows
-// l * DK/32 .. of them in registers, so a row costs two warp sums a column and no shared memory.
-template <int DK, int DV>
-__global__ void __launch_bounds__(128) gdn_rows_kernel(const GdnParams p) {
-    constexpr int kPer = DK / 32;
-    const int lane = threadIdx.x % 32;
-    const int col = (blockIdx.x * 4 + threadIdx.x / 32) * 4;
-    const int hv = blockIdx.y, b = blockIdx.z, hk = hv / (p.v_heads / p.k_heads);
-    int r0, r1;
-    gdn_rows(p, b, &r0, &r1);
-    const int slot = gdn_slot(p, b);
-    if (slot < 0) {
-        if (lane == 0)
-            for (int r = r0; r < r1; ++r)
-                *reinterpret_cast<uint2*>(p.out + (static_cast<long long>(r) * p.v_heads + hv) * DV + col) = uint2{};
-        return;
-    }
-    float* st = p.state + (static_cast<long long>(slot) * p.v_heads + hv) * DK * DV;
-    float s[kPer][4] = {};
-    if (p.carry)
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            const float4 x = *reinterpret_cast<const float4*>(st + (lane * kPer + i) * DV + col);
-            s[i][0] = x.x, s[i][1] = x.y, s[i][2] = x.z, s[i][3] = x.w;
-        }
-    for (int r = r0; r < r1; ++r) {
-        float q[kPer], k[kPer], qq = 0, kk = 0, qk = 0;
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            q[i] = __bfloat162float(p.q[r * p.ldq + hk * DK + lane * kPer + i]);
-            k[i] = __bfloat162float(p.k[r * p.ldk + hk * DK + lane * kPer + i]);
-            qq += q[i] * q[i], kk += k[i] * k[i], qk += q[i] * k[i];
-        }
-        qk = warp_sum(qk);
-        float rq = p.scale, rk = 1.0f;
-        if (p.normalize) {
-            rq *= rsqrtf(warp_sum(qq) + kGdnNormEps);
-            rk = rsqrtf(warp_sum(kk) + kGdnNormEps);
-        }
-        const long long at = static_cast<long long>(r) * p.v_heads + hv;
-        const float decay = expf(p.g[at]), beta = p.beta[at];
-        float o[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            float ks = 0, qs = 0;
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) ks += k[i] * s[i][j], qs += q[i] * s[i][j];
-            ks = warp_sum(ks) * rk * decay;
-            qs = warp_sum(qs) * decay;
-            const float u = beta * (__bfloat162float(p.v[r * p.ldv + hv * DV + col + j]) - ks);
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) s[i][j] = decay * s[i][j] + k[i] * (rk * u);
-            o[j] = rq * (qs + qk * rk * u);
-        }
-        if (lane == 0)
-            *reinterpret_cast<uint2*>(p.out + at * DV + col) = uint2{bf16x2_rn(f2(o[0], o[1])), bf16x2_rn(f2(o[2], o[3]))};
-    }
-#pragma unroll
-    for (int i = 0; i < kPer; ++i)
-        *reinterpret_cast<float4*>(st + (lane * kPer + i) * DV + col) = float4{s[i][0], s[i][1], s[i][2], s[i][3]};
-}
-
 // ------------------------------------------------------------------------------------------ single-row step
 // One block a sequence and head: the block's threads hold the whole state, 4 columns of DV and DK / kGroups
 // rows each, so each value is read and written once and both sums over k (k^T S and q^T S) take one pass:

@@ -81,7 +81,7 @@ struct GdnShared {
     float a11[32 * 32], a22[32 * 32];         // -A's diagonal blocks; 16-byte pieces of a row xor-ed with row % 8
     float xch[2][8][32];
     uint64_t kq_in[kKqSlots], rows_full[kKqSlots], rows_free[kKqSlots], v_in[2], v_free[2], tiles_full[2], tiles_free[2];
-    uint64_t s_ready, r_ready, v_ready, x_done, v_done, d_done, y_done, kk_done, kk_free, z_done;
+    uint64_t s_ready, r_ready, v_ready, x_done, v_done, d_done, y_done, kk_done, kk_free, z_done, drained[3];
     int length[kGdnSorted], sequence;
     uint32_t tmem;
     uint32_t abort;
@@ -94,21 +94,31 @@ REAX_DEVI uint32_t timer_lo() {
     asm volatile("mov.u32 %0, %%globaltimer_lo;" : "=r"(t));
     return t;
 }
-// Wait for a phase, for at most limit_ns.  Once a wait of the block has expired all of them return at once, so that the
-// block runs on to its end; the flag then goes to the status word, which says that the results are invalid.  (Few
-// instructions: the roles' code has to fit the instruction cache.)
+// Wait for a phase, for at most limit_ns.  Once a wait of the block has expired all of them return at once, and a role that
+// knows of it (`dead`) neither arrives at barriers nor starts copies or MMAs any more, but goes through its loop, so that
+// the block ends; the flag then goes to the status word, which says that the results are invalid.
 struct GdnWait {
     volatile uint32_t* abort;
     uint32_t limit_ns;
-    REAX_DEVI void operator()(uint64_t* bar, uint32_t parity, uint32_t bit) const {
+    bool dead = false;
+    REAX_DEVI void operator()(uint64_t* bar, uint32_t parity, uint32_t bit) {
         if (mbar_try_wait_suspend(bar, parity, 2000u)) return;
         const uint32_t t0 = timer_lo();
         while (!mbar_try_wait_suspend(bar, parity, 2000u)) {
-            if (*abort) return;
+            if (*abort) {
+                dead = true;
+                return;
+            }
             if (timer_lo() - t0 > limit_ns) *abort = bit;
         }
     }
 };
+constexpr unsigned long long kDrainNs = 2000000000ull;   // bound of the waits for a block's own copies and MMAs at its end
+// Wait for the MMAs that this thread has issued (their TMEM and shared memory may be given back then).
+REAX_DEVI void drain_mmas(uint64_t* bar) {
+    umma_commit(bar);
+    mbar_wait_bounded(bar, 0, kDrainNs, nullptr);
+}
 
 REAX_DEVI float ex2(float x) {
     float y;
@@ -269,6 +279,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) gdn_chunk_kernel(const __gri
         mbar_init(&sh.s_ready, 8), mbar_init(&sh.r_ready, 8), mbar_init(&sh.v_ready, 8);
         mbar_init(&sh.x_done, 1), mbar_init(&sh.v_done, 1), mbar_init(&sh.d_done, 1), mbar_init(&sh.y_done, 1);
         mbar_init(&sh.kk_done, 1), mbar_init(&sh.kk_free, 4), mbar_init(&sh.z_done, 1);
+        for (int i = 0; i < 3; ++i) mbar_init(&sh.drained[i], 1);
         sh.abort = 0;
         fence_mbar_init();
     }
@@ -276,13 +287,13 @@ __global__ void __launch_bounds__(kChunkThreads, 1) gdn_chunk_kernel(const __gri
     __syncthreads();
     tc_fence_after();
     const uint32_t tm = sh.tmem;
-    const GdnWait wait{&sh.abort, limit_ns};
+    GdnWait wait{&sh.abort, limit_ns};
     const int quarter = warp % 4;
     const uint32_t lanes = tm + (static_cast<uint32_t>(quarter * 32) << 16);
     // One arrival for the warp, after what all its lanes have done.
     auto arrive = [&](uint64_t* bar) {
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar);
+        if (lane == 0 && !wait.dead) mbar_arrive(bar);
     };
 
     if (warp < 8) {
@@ -340,12 +351,15 @@ __global__ void __launch_bounds__(kChunkThreads, 1) gdn_chunk_kernel(const __gri
 #pragma unroll
                 for (int e = 0; e < 32; e += 16) {
                     uint32_t x[16], y[16];
+                    // (factors first: the compiler must not move a load over a store that it cannot tell apart)
+                    uint64_t cq[8], cp[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) cq[i] = pair_of(st.c_q + part * 32 + e + 2 * i), cp[i] = pair_of(st.c_p + part * 32 + e + 2 * i);
                     tmem_ld2_x16_sync(lanes + kTmXq + part * 32 + e, lanes + kTmY + part * 32 + e, x, y);
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
-                        const int at = part * 32 + e + 2 * i;
-                        const uint64_t z = mul2_rn(u2(x[2 * i], x[2 * i + 1]), mul2_rn(pair_of(st.c_q + at), f2(sq, sq)));
-                        const uint32_t w = bf16x2_rn(fma2_rn(u2(y[2 * i], y[2 * i + 1]), mul2_rn(pair_of(st.c_p + at), f2(sv, sv)), z));
+                        const uint64_t z = mul2_rn(u2(x[2 * i], x[2 * i + 1]), mul2_rn(cq[i], f2(sq, sq)));
+                        const uint32_t w = bf16x2_rn(fma2_rn(u2(y[2 * i], y[2 * i + 1]), mul2_rn(cp[i], f2(sv, sv)), z));
                         o[(e + 2 * i) * 32] = static_cast<uint16_t>(w);
                         o[(e + 2 * i + 1) * 32] = static_cast<uint16_t>(w >> 16);
                     }
@@ -480,6 +494,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) gdn_chunk_kernel(const __gri
                 GdnRows& in = sh.rows[c % kKqSlots];
                 wait(&sh.rows_full[c % kKqSlots], (c / kKqSlots) & 1, kStatusTimeoutFull);
                 if (c > 0) wait(&sh.kk_free, (c - 1) & 1, kStatusTimeoutAccEmpty);
+                if (wait.dead) return;
                 tc_fence_after();
                 const uint64_t d = sw128_kmajor_desc(smem_u32(in.kq));
 #pragma unroll 1
@@ -489,9 +504,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1) gdn_chunk_kernel(const __gri
                 }
                 umma_commit(&sh.kk_done);
             }
-            __syncwarp();
         };
         if (warp == 8) products(0);
+        __syncwarp();
 #pragma unroll 1
         for (int c = 0, slot_k = 0; c < chunks; ++c, slot_k = slot_k == kKqSlots - 1 ? 0 : slot_k + 1) {
             const uint32_t par = c & 1;
@@ -542,12 +557,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1) gdn_chunk_kernel(const __gri
                     const float f = -row_k * beta;
                     float* a = (upper ? sh.a22 : sh.a11) + l * 32;
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
+                    for (int e = 0; e < 8; ++e)
+                        y[e] = mul2_rn(y[e], mul2_rn(f2(f, f), *reinterpret_cast<const uint64_t*>(in.row_k + o + 2 * e)));
 #pragma unroll
-                        for (int e = 2 * q; e < 2 * q + 2; ++e)
-                            y[e] = mul2_rn(y[e], mul2_rn(f2(f, f), *reinterpret_cast<const uint64_t*>(in.row_k + o + 2 * e)));
+                    for (int q = 0; q < 4; ++q)
                         *reinterpret_cast<ulonglong2*>(a + piece((o & 31) / 4 + q) * 4) = ulonglong2{y[2 * q], y[2 * q + 1]};
-                    }
                 }
             }
             if (is_q) {
@@ -599,7 +613,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) gdn_chunk_kernel(const __gri
                     tmem_wait_st();
                     tc_fence_before();
                     asm volatile("bar.sync 6, 64;" ::: "memory");
-                    if (lane == 0) {
+                    if (lane == 0 && !wait.dead) {
                         tc_fence_after();
                         const uint64_t hi_desc = sw128_mn_desc(smem_u32(sh.a21[0]), 4096), lo_desc = sw128_mn_desc(smem_u32(sh.a21[1]), 4096);
 #pragma unroll 2
@@ -649,9 +663,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1) gdn_chunk_kernel(const __gri
             fence_proxy_async_smem();
             arrive(&sh.tiles_full[par]);
             if (warp == 8 && c + 1 < chunks) products(c + 1);
+            __syncwarp();
         }
-        if (warp == 9 && lane == 0) mbar_wait_bounded(&sh.z_done, (chunks - 1) & 1, limit_ns, nullptr);
-        if (warp == 8 && lane == 0) mbar_wait_bounded(&sh.kk_done, (chunks - 1) & 1, limit_ns, nullptr);
+        if (warp < 10 && lane == 0) drain_mmas(&sh.drained[warp - 8]);
     } else {
         if (warp == 13) {
             // --------------------------------------------------------------------------- issuer of the chain's MMAs
@@ -668,6 +682,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) gdn_chunk_kernel(const __gri
                     const uint64_t pd = sw128_kmajor_desc(smem_u32(st.p));
                     wait(&sh.rows_full[slot_k], (c / kKqSlots) & 1, kStatusTimeoutFull);
                     wait(&sh.s_ready, par, kStatusTimeoutEmpty);
+                    if (wait.dead) break;
                     tc_fence_after();
                     // descriptor addresses count in units of 16 bytes
 #pragma unroll 4
@@ -678,12 +693,14 @@ __global__ void __launch_bounds__(kChunkThreads, 1) gdn_chunk_kernel(const __gri
                     umma_commit(&sh.x_done);
                     // the chunk before's X_q has been read
                     if (c > 0) wait(&sh.tiles_free[par ^ 1], ((c - 1) >> 1) & 1, kStatusTimeoutEmpty);
+                    if (wait.dead) break;
                     tc_fence_after();
 #pragma unroll 4
                     for (int ks = 0; ks < DK / 16; ++ks)
                         umma_f16_ts(tm + kTmXq, tm + kTmS + ks * 8, kq + 512 + (ks / 4) * 1024 + (ks % 4) * 2, id64, ks > 0);
                     wait(&sh.tiles_full[par], (c >> 1) & 1, kStatusTimeoutFull);
                     wait(&sh.r_ready, par, kStatusTimeoutEmpty);
+                    if (wait.dead) break;
                     tc_fence_after();
 #pragma unroll 4
                     for (int e = 0; e < 12; ++e) {
@@ -692,6 +709,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) gdn_chunk_kernel(const __gri
                     }
                     umma_commit(&sh.v_done);
                     wait(&sh.v_ready, par, kStatusTimeoutEmpty);
+                    if (wait.dead) break;
                     tc_fence_after();
 #pragma unroll 4
                     for (int e = 0; e < 8; ++e)
@@ -702,8 +720,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) gdn_chunk_kernel(const __gri
                     for (int ks = 0; ks < 4; ++ks) umma_f16_ts(tm + kTmY, tm + kTmR + ks * 8, pd + ks * 2, id64, ks > 0);
                     umma_commit(&sh.y_done);
                 }
-                // TMEM may be freed once the MMAs are done, also after a wait that expired
-                mbar_wait_bounded(&sh.y_done, (chunks - 1) & 1, limit_ns, nullptr);
+                drain_mmas(&sh.drained[2]);
             }
             __syncwarp();
         } else {
@@ -711,8 +728,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1) gdn_chunk_kernel(const __gri
             const int w = warp == 12 ? 0 : warp - 13, t = w * 32 + lane;
             constexpr int kPieces = DK / 8;                               // 16-byte pieces of a row
             const uint64_t policy = l2_policy_evict_normal();
+            int kq_loads = 0, v_loads = 0;                                // copies started by this thread
             auto load_kq = [&](int c, int slot_k) {
-                if (t == 0) {
+                if (t == 0 && !wait.dead) {
+                    ++kq_loads;
                     uint64_t* bar = &sh.kq_in[slot_k];
                     fence_proxy_async_smem();
                     mbar_arrive_expect_tx(bar, kChunk * 4 * DK);
@@ -826,9 +845,12 @@ __global__ void __launch_bounds__(kChunkThreads, 1) gdn_chunk_kernel(const __gri
                 arrive(&sh.rows_full[slot_k]);
                 if (t == 32) {
                     if (c > 1) wait(&sh.v_free[par], ((c >> 1) - 1) & 1, kStatusTimeoutEmpty);
-                    fence_proxy_async_smem();
-                    mbar_arrive_expect_tx(&sh.v_in[par], kChunk * 2 * DV);
-                    tma_load_2d(sh.v[par], &maps.v, &sh.v_in[par], hv * DV, r0 + c * kChunk, policy);
+                    if (!wait.dead) {
+                        ++v_loads;
+                        fence_proxy_async_smem();
+                        mbar_arrive_expect_tx(&sh.v_in[par], kChunk * 2 * DV);
+                        tma_load_2d(sh.v[par], &maps.v, &sh.v_in[par], hv * DV, r0 + c * kChunk, policy);
+                    }
                 }
                 __syncwarp();
                 if (c + 2 < chunks) {
@@ -837,13 +859,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1) gdn_chunk_kernel(const __gri
                     load_kq(c + 2, next);
                 }
             }
-            if (t == 0) {
-                // no copy may be in flight when the block ends, also after a wait that expired
-                for (int c = max(chunks - 2, 0); c < chunks; ++c) {
-                    mbar_wait_bounded(&sh.kq_in[c % kKqSlots], (c / kKqSlots) & 1, limit_ns, nullptr);
-                    mbar_wait_bounded(&sh.v_in[c & 1], (c >> 1) & 1, limit_ns, nullptr);
-                }
-            }
+            // no copy may be in flight when the block ends
+            for (int c = max(kq_loads - kKqSlots, 0); c < kq_loads; ++c)
+                mbar_wait_bounded(&sh.kq_in[c % kKqSlots], (c / kKqSlots) & 1, kDrainNs, nullptr);
+            for (int c = max(v_loads - 2, 0); c < v_loads; ++c) mbar_wait_bounded(&sh.v_in[c & 1], (c >> 1) & 1, kDrainNs, nullptr);
         }
     }
     tc_fence_before();

@@ -54,6 +54,12 @@ REAX_DEVI int kv8_code(float x, float scale) {
     return q != q ? 0 : static_cast<int>(fminf(fmaxf(q, -127.0f), 127.0f));
 }
 
+// (Not inlined: it is rare, and the division is long.)
+__device__ __noinline__ uint32_t kv8_codes_divided(float x0, float x1, float x2, float x3, float scale) {
+    return (kv8_code(x0, scale) & 0xFF) | (kv8_code(x1, scale) & 0xFF) << 8 | (kv8_code(x2, scale) & 0xFF) << 16 |
+           static_cast<uint32_t>(kv8_code(x3, scale)) << 24;
+}
+
 // The codes of 4 values.  x times the scale's inverse is within 127 * 2^-22 of x / scale, so that it rounds to the same whole
 // number unless it lies that near to a half; those few, and what is not finite, take the division.
 REAX_DEVI uint32_t kv8_codes(float x0, float x1, float x2, float x3, float scale, float inv) {
@@ -67,9 +73,7 @@ REAX_DEVI uint32_t kv8_codes(float x0, float x1, float x2, float x3, float scale
         sure = sure && fabsf(__fmaf_rn(x[i], inv, kRound - t)) <= 0.4999f;
         c[i] = __float_as_uint(t);
     }
-    if (!sure)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) c[i] = static_cast<uint32_t>(kv8_code(x[i], scale));
+    if (!sure) return kv8_codes_divided(x0, x1, x2, x3, scale);
     return __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
 }
 

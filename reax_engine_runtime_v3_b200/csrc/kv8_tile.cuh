@@ -41,7 +41,7 @@ struct TileShared {
     uint8_t k[2][kTileCols * D * 2], v[2][kTileCols * D * 2];   // [D / 64][64 rows][64 values], 128-byte swizzle
     uint8_t codes[2][2][kTileCols * D];       // of k and v as they come, two tiles: 16 rows after 16 rows
     float xch[2][8][32];
-    uint64_t in[2][2], in_free[2][2], k_full[2], v_full[2], k_free[2], v_free[2], s_full, s_free, p_full, pv_done;
+    uint64_t in[2][2], in_free[2][2], k_full[2], v_full[2], k_free[2], v_free[2], s_full, s_free, p_full, pv_done, drained;
     uint32_t tmem;
     uint32_t abort;
 };
@@ -115,7 +115,7 @@ __global__ void __launch_bounds__(kAttendTileThreads, 1)
             mbar_init(&sh.k_full[i], kConverters), mbar_init(&sh.v_full[i], kConverters);
             mbar_init(&sh.k_free[i], 1), mbar_init(&sh.v_free[i], 1);
         }
-        mbar_init(&sh.s_full, 1), mbar_init(&sh.s_free, 8), mbar_init(&sh.p_full, 8), mbar_init(&sh.pv_done, 1);
+        mbar_init(&sh.s_full, 1), mbar_init(&sh.s_free, 8), mbar_init(&sh.p_full, 8), mbar_init(&sh.pv_done, 1), mbar_init(&sh.drained, 1);
         sh.abort = 0;
         fence_mbar_init();
     }
@@ -123,11 +123,11 @@ __global__ void __launch_bounds__(kAttendTileThreads, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tm = sh.tmem;
-    const GdnWait wait{&sh.abort, limit_ns};
+    GdnWait wait{&sh.abort, limit_ns};
     const uint32_t lanes = tm + (static_cast<uint32_t>(quarter * 32) << 16);
     auto arrive = [&](uint64_t* bar) {
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar);
+        if (lane == 0 && !wait.dead) mbar_arrive(bar);
     };
 
     if (warp < 8) {
@@ -301,6 +301,7 @@ __global__ void __launch_bounds__(kAttendTileThreads, 1)
                     const uint64_t kd = sw128_kmajor_desc(smem_u32(sh.k[buf]));
                     wait(&sh.k_full[buf], (x >> 1) & 1, kStatusTimeoutFull);
                     wait(&sh.s_free, x & 1, kStatusTimeoutAccEmpty);       // (first: q is there)
+                    if (wait.dead) break;
                     tc_fence_after();
 #pragma unroll 1
                     for (int ks = 0; ks < D / 16; ++ks)
@@ -313,6 +314,7 @@ __global__ void __launch_bounds__(kAttendTileThreads, 1)
                     const uint64_t vd = sw128_mn_desc(smem_u32(sh.v[buf]), kTileCols * 128);
                     wait(&sh.v_full[buf], (y >> 1) & 1, kStatusTimeoutFull);
                     wait(&sh.p_full, y & 1, kStatusTimeoutEmpty);
+                    if (wait.dead) break;
                     tc_fence_after();
 #pragma unroll 1
                     for (int e = 0; e < 8; ++e)
@@ -321,14 +323,13 @@ __global__ void __launch_bounds__(kAttendTileThreads, 1)
                     umma_commit(&sh.v_free[buf]);
                 }
             }
-            // TMEM may be freed once the MMAs are done, also after a wait that expired
-            mbar_wait_bounded(&sh.pv_done, (tiles - 1) & 1, limit_ns, nullptr);
+            drain_mmas(&sh.drained);
         }
         __syncwarp();
     } else if (warp == 13) {
         // --------------------------------------------------------------------------------------------------- loads
         const uint64_t policy = l2_policy_evict_normal();
-        int id = -1;
+        int id = -1, loads[2] = {};
         auto look_up = [&](int x) {           // lane l < 4: rows 16 l .. of the tile
             const int row = x * kTileCols + lane * 16;
             id = x < tiles && lane < 4 && row < seq.len ? table[row >> shift] : -1;
@@ -342,12 +343,14 @@ __global__ void __launch_bounds__(kAttendTileThreads, 1)
 #pragma unroll 1
             for (int e = 0; e < 2; ++e) {     // k, then v
                 if (x > 1) wait(&sh.in_free[buf][e], ((x >> 1) - 1) & 1, kStatusTimeoutEmpty);
-                if (lane == 0) {
+                wait.dead = __any_sync(0xFFFFFFFFu, wait.dead);
+                if (lane == 0 && !wait.dead) {
                     fence_proxy_async_smem();
                     mbar_arrive_expect_tx(&sh.in[buf][e], have * 16 * D);
                 }
                 __syncwarp();
-                if (in)
+                loads[e] += !wait.dead;
+                if (in && !wait.dead)
 #pragma unroll
                     for (int d = 0; d < D; d += 128)
                         tma_load_2d(sh.codes[buf][e] + lane * 16 * D + d * 16, e ? &maps.v : &maps.k, &sh.in[buf][e], d, at, policy);
@@ -355,10 +358,10 @@ __global__ void __launch_bounds__(kAttendTileThreads, 1)
             }
             look_up(x + 1);
         }
-        if (lane == 0) {
-            for (int x = max(tiles - 2, 0); x < tiles; ++x)
-                for (int e = 0; e < 2; ++e) mbar_wait_bounded(&sh.in[x & 1][e], (x >> 1) & 1, limit_ns, nullptr);
-        }
+        // no copy may be in flight when the block ends
+        if (lane == 0)
+            for (int e = 0; e < 2; ++e)
+                for (int x = max(loads[e] - 2, 0); x < loads[e]; ++x) mbar_wait_bounded(&sh.in[x & 1][e], (x >> 1) & 1, kDrainNs, nullptr);
         __syncwarp();
     } else {
         // ------------------------------------------------------------------------------------------- codes to bf16
@@ -378,17 +381,28 @@ __global__ void __launch_bounds__(kAttendTileThreads, 1)
                 uint8_t* to = e ? sh.v[buf] : sh.k[buf];
                 // 8 rows by 4 pieces of 16 codes a warp and turn
                 auto convert = [&](auto pair) {
-#pragma unroll 4
-                    for (int u = begin; u < (kTileCols / 8) * (D / 64); u += step) {
-                        const int rb = u / (D / 64), pb = u % (D / 64);
-                        const uint8_t* src = D == 64 ? sh.codes[buf][e] + rb * 512 + from
-                                                     : sh.codes[buf][e] + (rb / 2) * (16 * D) + (rb % 2) * 1024 + (pb / 2) * 2048 + (from ^ (pb % 2 * 64));
-                        const uint4 y = *reinterpret_cast<const uint4*>(src);
-                        uint8_t* row = to + pb * (kTileCols * 128) + rb * 1024;
-                        uint32_t w[8];
-                        pair(y.x, w[0], w[1]), pair(y.y, w[2], w[3]), pair(y.z, w[4], w[5]), pair(y.w, w[6], w[7]);
-                        *reinterpret_cast<uint4*>(row + into) = uint4{w[0], w[1], w[2], w[3]};
-                        *reinterpret_cast<uint4*>(row + (into ^ 16)) = uint4{w[4], w[5], w[6], w[7]};
+                    // (the loads first: the compiler must not move one over a store that it cannot tell apart)
+                    constexpr int kAll = (kTileCols / 8) * (D / 64);
+#pragma unroll 1
+                    for (int u0 = begin; u0 < kAll; u0 += 4 * step) {
+                        uint4 y[4];
+#pragma unroll
+                        for (int n = 0; n < 4; ++n) {
+                            const int u = min(u0 + n * step, kAll - 1), rb = u / (D / 64), pb = u % (D / 64);
+                            y[n] = *reinterpret_cast<const uint4*>(
+                                D == 64 ? sh.codes[buf][e] + rb * 512 + from
+                                        : sh.codes[buf][e] + (rb / 2) * (16 * D) + (rb % 2) * 1024 + (pb / 2) * 2048 + (from ^ (pb % 2 * 64)));
+                        }
+#pragma unroll
+                        for (int n = 0; n < 4; ++n) {
+                            const int u = u0 + n * step, rb = u / (D / 64), pb = u % (D / 64);
+                            if (u >= kAll) break;
+                            uint8_t* row = to + pb * (kTileCols * 128) + rb * 1024;
+                            uint32_t w[8];
+                            pair(y[n].x, w[0], w[1]), pair(y[n].y, w[2], w[3]), pair(y[n].z, w[4], w[5]), pair(y[n].w, w[6], w[7]);
+                            *reinterpret_cast<uint4*>(row + into) = uint4{w[0], w[1], w[2], w[3]};
+                            *reinterpret_cast<uint4*>(row + (into ^ 16)) = uint4{w[4], w[5], w[6], w[7]};
+                        }
                     }
                 };
                 if (e)
@@ -399,7 +413,7 @@ __global__ void __launch_bounds__(kAttendTileThreads, 1)
                     });
                 fence_proxy_async_smem();
                 __syncwarp();
-                if (lane == 0) {
+                if (lane == 0 && !wait.dead) {
                     mbar_arrive(&sh.in_free[buf][e]);
                     mbar_arrive(e ? &sh.v_full[buf] : &sh.k_full[buf]);
                 }

@@ -86,12 +86,6 @@ int gdn_chunks(const char* who, const reax::GdnParams& p, void* stream) {
                   stream, p, maps, wait_ns());
 }
 
-int gdn_rows(const char* who, const reax::GdnParams& p, int Dk, int Dv, void* stream) {
-#define X(K, V) reax::gdn_rows_kernel<K, V>
-    return launch(who, REAX_GDN_DISPATCH(Dk, Dv, X), dim3(Dv / 16, p.v_heads, p.batch), 128, 0, stream, p);
-#undef X
-}
-
 int check_cache(const char* who, const reax::Kv8Cache& c) {
     if (c.pages < 0 || c.heads <= 0 || c.heads > kGridYz)
         return fail(REAX_ERR_INVALID, "%s: %d pages of %d heads", who, c.pages, c.heads);
