@@ -570,7 +570,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1) gdn_chunk_kernel(const __gri
 #pragma unroll
                     for (int e = 4; e < 8; ++e) *reinterpret_cast<uint4*>(st.p + i * 128 + piece(e) * 16) = uint4{};
                 } else {
-                    asm volatile("bar.arrive 6, 64;" ::: "memory");     // columns 32.. may be written
+                    // columns 32.. may be written (both warps wait: one that arrived alone could, after a wait that expired,
+                    // arrive twice and leave the other without a partner)
+                    named_bar_sync(6, 64);
                 }
                 const float f = in.row_q[i];
                 st.c_q[i] = f * ex2(g_hi + g_lo);
@@ -612,7 +614,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) gdn_chunk_kernel(const __gri
                     tmem_st_x16(lanes + kTmPrep + 16, lo);
                     tmem_wait_st();
                     tc_fence_before();
-                    asm volatile("bar.sync 6, 64;" ::: "memory");
+                    named_bar_sync(6, 64);
                     if (lane == 0 && !wait.dead) {
                         tc_fence_after();
                         const uint64_t hi_desc = sw128_mn_desc(smem_u32(sh.a21[0]), 4096), lo_desc = sw128_mn_desc(smem_u32(sh.a21[1]), 4096);

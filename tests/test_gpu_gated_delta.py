@@ -228,3 +228,31 @@ def test_refusals():
     odd = torch.empty(4 * 256 + 4, dtype=torch.bfloat16, device="cuda")[4:].view(4, 2, 128)
     with pytest.raises(RuntimeError, match="status 2"):
         gated_delta.decode(odd, *x[1:])
+
+
+def test_expired_wait_is_reported_and_the_next_call_is_right():
+    """With waits bounded by a nanosecond a block gives up, ends and says so; with the default it works again."""
+    from reax_engine_runtime_v3_b200 import _native
+    x = inputs(18, 300, 2, 4, 128, 128, 1)
+    assert _native.mixer_status(clear=True) == 0
+    _native.load().reax_set_wait_timeout_ns(1)
+    try:
+        run_prefill(x, [300], [0])
+        assert _native.mixer_status(clear=True) != 0
+    finally:
+        _native.load().reax_set_wait_timeout_ns(0)
+    out, state, spans = run_prefill(x, [300], [0])
+    compare(out, state, *definition(*x, spans, [0]))
+    assert _native.mixer_status() == 0
+
+
+def test_example_runs():
+    """The example's prompt and steps through both mixers."""
+    import os
+    import runpy
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "token_mixers.py")
+    outs, state, cached = runpy.run_path(path)["main"]()
+    torch.cuda.synchronize()
+    assert cached.tolist() == [74, 5, 204] and torch.isfinite(state).all() and state.any()
+    for mixed, seen in outs:
+        assert torch.isfinite(mixed).all() and torch.isfinite(seen).all() and mixed.any() and seen.any()
