@@ -241,7 +241,13 @@ REAX_API int reax_sliced_i8_static(const int8_t* A, const int8_t* W, const void*
 REAX_API int reax_gdn_prefill(const void* q, const void* k, const void* v, const float* g, const float* beta,
                               float* state, const int32_t* cu_seqlens, const int32_t* slots, void* out, int rows,
                               int batch, int k_heads, int v_heads, int Dk, int Dv, int n_slots, long long ldq,
-                              long long ldk, long long ldv, float scale, int normalize, int carry, void* stream);
+                              long long ldk, long long ldv, float scale, int normalize, int carry, void* workspace,
+                              size_t workspace_bytes, void* stream);
+
+/* Bytes of scratch memory that reax_gdn_prefill needs for these sizes (0 for none or for sizes that it refuses): what it
+ * finds for each chunk of 64 rows before the states are carried along, at most about 1.5 GB (longer batches take several
+ * launches).  It need not be initialized; 128-byte aligned, and not shared by calls that can run at the same time. */
+REAX_API size_t reax_gdn_workspace_bytes(int rows, int batch, int k_heads, int v_heads, int Dk);
 
 /* One row for each of `batch` sequences, from the states kept. */
 REAX_API int reax_gdn_decode(const void* q, const void* k, const void* v, const float* g, const float* beta,

@@ -51,7 +51,8 @@ SIGNATURES = {
     "reax_bf16_partials": ([_P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _SZ, _P], _I),
     "reax_sliced_i8": ([_P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _SZ, _P], _I),
     "reax_sliced_i8_static": ([_P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _SZ, _P], _I),
-    "reax_gdn_prefill": ([_P] * 9 + [_I] * 7 + [_LL] * 3 + [_F, _I, _I, _P], _I),
+    "reax_gdn_prefill": ([_P] * 9 + [_I] * 7 + [_LL] * 3 + [_F, _I, _I, _P, _SZ, _P], _I),
+    "reax_gdn_workspace_bytes": ([_I] * 5, _SZ),
     "reax_gdn_decode": ([_P] * 8 + [_I] * 6 + [_LL] * 3 + [_F, _I, _P], _I),
     "reax_mixer_status": ([C.POINTER(C.c_uint), _I, _P], _I),
     "reax_kv8_append": ([_P] * 9 + [_I] * 7 + [_LL] * 2 + [_P], _I),

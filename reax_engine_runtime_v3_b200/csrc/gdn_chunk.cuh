@@ -23,9 +23,14 @@
 // have 8 bits and are exact in one.  X_k, V' and D, which the state depends on, take all terms down to 2^-22; X_q and Y
 // only reach the bf16 output and take the hi terms.  Sums are float32.
 //
-// Roles (16 warps): 0-7 carry the state; 8-11 find T and P of the chunks ahead; 13 issues the chain's MMAs; 12, 14 and
-// 15 load rows and turn k and q into fp16 tiles (13 shares its scheduler with 9, which has the most to solve).  No role may spill: beside this much shared memory little is left of the L1
-// cache, and a spilled value comes back from L2.
+// Two kernels.  What a chunk needs that does not depend on the state (k and q as fp16 tiles, T, P and the rows' factors) is
+// found by gdn_tiles_kernel for all chunks at once, a block of four warps for each chunk and key head, and kept in scratch
+// memory; gdn_chunk_kernel then carries the states along, a block for each sequence and value head, which reads those tiles
+// as they are.  Of one kernel with warps for each part, a chunk took 6.5 us of a block, most of it waiting for the solve of
+// the next one, where the second kernel takes 4.3: 8192 rows of one sequence and 32 value heads 860 -> 628 us, 32768 rows of
+// 16 sequences 836 -> 820 us, 4001 of 8 155 -> 141 us, 96 rows 22.5 -> 24.6 us.
+//
+// Roles of the second (10 warps): 0-7 carry the state; 8 issues the MMAs; 9 loads.
 #pragma once
 
 #include <cuda_fp16.h>
@@ -36,31 +41,24 @@
 namespace reax {
 
 constexpr int kChunk = 64;
-constexpr int kChunkThreads = 16 * 32;
+constexpr int kChunkThreads = 10 * 32;
+constexpr int kTilesThreads = 4 * 32;
 constexpr int kKqSlots = 3;                   // chunks of k and q tiles in flight
-constexpr int kLoaders = 3 * 32;
 constexpr int kGdnSorted = 256;               // sequences up to which blocks take them in the order of their lengths
 constexpr float kGdnDown = 0x1p-20f, kGdnUp = 0x1p20f;
 
 // TMEM columns.  S hi and lo (64 each) share the columns of D, and the decayed V' hi and lo those of X_k, V' hi those of R:
 // each is written after the other has been read.
-constexpr uint32_t kTmS = 0, kTmXk = 128, kTmXq = 192, kTmR = 256, kTmV = 320, kTmY = 384, kTmPrep = 448;
+constexpr uint32_t kTmS = 0, kTmXk = 128, kTmXq = 192, kTmR = 256, kTmV = 320, kTmY = 384;
+// ... and of the first kernel: [k; q] k^T, and the operand and result of a product within the solve.
+constexpr uint32_t kTmKk = 0, kTmZ = 64, kTmU = 96;
 
-// Tensor maps of q and k (boxes of 64 rows of 64 values, 128-byte swizzle), v (64 rows of one head) and the output (32 rows
-// of 32 columns).
+// Tensor maps of v (boxes of 64 rows of one head) and the output (32 rows of 32 columns).
 struct GdnMaps {
-    CUtensorMap q, k, v, out;
+    CUtensorMap v, out;
 };
 
-// What the loaders bring of a chunk.
-struct GdnRows {
-    uint8_t kq[2][128 * 128];                 // [half of dk][64 rows of k, then of q][64 fp16], 128-byte swizzle
-    float g_hi[kChunk], g_lo[kChunk];         // G in log2, as hi + lo
-    float row_k[kChunk], row_q[kChunk];       // scales of the rows of k and q
-    float beta[kChunk];
-    float pad[192];
-};
-// What the solvers find for it: tiles and the factors of each row.
+// What is found for a chunk and value head: swizzled tiles and the factors of each row.
 struct GdnTiles {
     uint8_t t_hi[64 * 128], t_lo[64 * 128];   // rows i, columns j of T
     uint8_t p[64 * 128];                      // of P
@@ -70,22 +68,42 @@ struct GdnTiles {
     float gamma;
     float pad[127];
 };
-static_assert(sizeof(GdnRows) % 1024 == 0 && sizeof(GdnTiles) % 1024 == 0, "tiles start on swizzle atoms");
+constexpr uint32_t kGdnTilesBytes = 3 * 64 * 128 + 6 * 4 * kChunk + 16;   // what of it is copied
+static_assert(sizeof(GdnTiles) % 1024 == 0, "tiles start on swizzle atoms");
 
-struct GdnShared {
-    GdnRows rows[kKqSlots];
-    GdnTiles tiles[2];
+// Scratch of one launch of both kernels, for `chunks` chunks from the x0-th on (chunks of the sequences one after the other).
+struct GdnScratch {
+    uint8_t* kq;                              // [chunks][k_heads][DK / 64][64 rows of k, then of q][64 fp16], 128-byte swizzle
+    GdnTiles* tiles;                          // [chunks][v_heads]
+    int x0, chunks;
+    int heads;                                // value heads of a key head that a block of the first kernel takes
+};
+
+struct GdnTilesShared {
+    uint8_t kq[2][128 * 128];                 // ... and, once k k^T and q k^T are there, a head's GdnTiles on their way out
     uint8_t a21[2][32 * 128];                 // A[32.., ..31] hi and lo: rows of 64 fp16, of which 32 are used
-    __nv_bfloat16 v[2][kChunk * 128];         // rows of DV values
-    __nv_bfloat16 out[8][32 * 32];            // a warp's 32 rows of 32 output columns
     float a11[32 * 32], a22[32 * 32];         // -A's diagonal blocks; 16-byte pieces of a row xor-ed with row % 8
-    float xch[2][8][32];
-    uint64_t kq_in[kKqSlots], rows_full[kKqSlots], rows_free[kKqSlots], v_in[2], v_free[2], tiles_full[2], tiles_free[2];
-    uint64_t s_ready, r_ready, v_ready, x_done, v_done, d_done, y_done, kk_done, kk_free, z_done, drained[3];
-    int length[kGdnSorted], sequence;
+    float g_hi[4][kChunk], g_lo[4][kChunk], beta[4][kChunk];   // of four value heads: G in log2, as hi + lo
+    float row_k[kChunk], row_q[kChunk];       // scales of the rows of k and q
+    uint64_t kk_done, z_done, drained[2];
     uint32_t tmem;
     uint32_t abort;
 };
+
+struct GdnShared {
+    uint8_t kq[kKqSlots][2][128 * 128];
+    GdnTiles tiles[2];
+    __nv_bfloat16 v[2][kChunk * 128];         // rows of DV values
+    __nv_bfloat16 out[8][32 * 32];            // a warp's 32 rows of 32 output columns
+    float xch[2][8][32];
+    uint64_t kq_in[kKqSlots], kq_free[kKqSlots], v_in[2], v_free[2], tiles_in[2], tiles_free[2];
+    uint64_t s_ready, r_ready, v_ready, x_done, v_done, d_done, y_done, drained;
+    int length[kGdnSorted], sequence, before;
+    uint32_t tmem;
+    uint32_t abort;
+};
+
+static_assert(sizeof(GdnTiles) <= sizeof(GdnTilesShared::kq), "tiles go out by way of k and q");
 
 static __device__ unsigned g_mixer_status;    // REAX_STATUS_* bits of waits that expired
 
@@ -231,11 +249,343 @@ REAX_DEVI void tmem_ld_x16_sync(uint32_t taddr, uint32_t (&r)[16]) {
         : "memory");
 }
 
+// Copy `bytes` (a multiple of 16) of this block's shared memory to global memory, in the thread's bulk group.
+REAX_DEVI void bulk_store(void* gdst, const void* smem_src, uint32_t bytes) {
+    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(gdst), "r"(smem_u32(smem_src)), "r"(bytes) : "memory");
+}
+
+// Chunks of sequence b.
+REAX_DEVI int gdn_chunks_of(const GdnParams& p, int b) {
+    int lo, hi;
+    gdn_rows(p, b, &lo, &hi);
+    return (hi - lo + kChunk - 1) / kChunk;
+}
+
+// k and q tiles, T, P and factors of chunk x0 + blockIdx.x for the value heads of key head blockIdx.y.  Four blocks share an
+// SM: what one waits for (its rows, its products, the solve's chain) the others fill.
+template <int DK>
+__global__ void __launch_bounds__(kTilesThreads, 4) gdn_tiles_kernel(const __grid_constant__ GdnParams p, const GdnScratch out, uint32_t limit_ns) {
+    extern __shared__ uint8_t tiles_smem[];
+    // (an offset into the array, not an integer made a pointer: the accesses stay known as shared-memory ones)
+    GdnTilesShared& sh = *reinterpret_cast<GdnTilesShared*>(tiles_smem + (-smem_u32(tiles_smem) & 1023u));
+    const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32, hk = blockIdx.y;
+    const int group = p.v_heads / p.k_heads, head0 = blockIdx.z * out.heads, heads = min(out.heads, group - head0);
+    asm volatile("griddepcontrol.launch_dependents;");                // (which wait for the end of this grid)
+    // the sequence and its chunk
+    int b = -1, c = 0;
+    for (int b0 = 0, before = 0; b0 < p.batch; b0 += 32) {
+        const int n = b0 + lane < p.batch ? gdn_chunks_of(p, b0 + lane) : 0;
+        int upto = n;
+#pragma unroll
+        for (int m = 1; m < 32; m <<= 1) {
+            const int t = __shfl_up_sync(0xFFFFFFFFu, upto, m);
+            if (lane >= m) upto += t;
+        }
+        const int x = out.x0 + static_cast<int>(blockIdx.x);
+        const unsigned who = __ballot_sync(0xFFFFFFFFu, before + upto > x);
+        if (who) {
+            const int l = __ffs(who) - 1;
+            b = b0 + l;
+            c = x - before - __shfl_sync(0xFFFFFFFFu, upto - n, l);
+            break;
+        }
+        before += __shfl_sync(0xFFFFFFFFu, upto, 31);
+    }
+    if (b < 0 || gdn_slot(p, b) < 0) return;
+    int r0, r1;
+    gdn_rows(p, b, &r0, &r1);
+    r0 += c * kChunk;
+    const int left = r1 - r0;                                         // rows of the chunk, if below 64
+
+    if (warp == 0) {
+        tmem_alloc(&sh.tmem, 128);
+        tmem_relinquish();                                            // the SM's next block may allocate before this one ends
+    }
+    if (tid == 0) {
+        mbar_init(&sh.kk_done, 1), mbar_init(&sh.z_done, 1), mbar_init(&sh.drained[0], 1), mbar_init(&sh.drained[1], 1);
+        sh.abort = 0;
+        fence_mbar_init();
+    }
+    {
+        // k and q rows -> fp16, four lanes a row, scaled to a 2-norm in [2^13, 2^14) (a norm below 2^-60, whose square may
+        // underflow, counts as 2^-60); rows past the end are zeros.  A lane's pieces of its row come in an order that the
+        // row's number turns, so that the eight lanes of a shared-memory pass meet all banks.
+        constexpr int kPieces = DK / 8, kTurns = kPieces / 4;
+        const int r8 = lane / 4;
+        uint4 raw[4][kTurns];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int r = warp * 32 + u * 8 + r8;
+            const bool real = r % 64 < left;
+            const __nv_bfloat16* row = r < 64 ? p.k + static_cast<long long>(r0 + (real ? r : 0)) * p.ldk + hk * DK
+                                              : p.q + static_cast<long long>(r0 + (real ? r - 64 : 0)) * p.ldq + hk * DK;
+#pragma unroll
+            for (int x = 0; x < kTurns; ++x)
+                raw[u][x] = real ? *reinterpret_cast<const uint4*>(row + (((x + r8) % kTurns) * 4 + lane % 4) * 8) : uint4{};
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int r = warp * 32 + u * 8 + r8;
+            uint64_t sum[2] = {};
+#pragma unroll
+            for (int x = 0; x < kTurns; ++x) {
+                const uint32_t y[4] = {raw[u][x].x, raw[u][x].y, raw[u][x].z, raw[u][x].w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) sum[j & 1] = fma2_rn(bf16x2_to_f2(y[j]), bf16x2_to_f2(y[j]), sum[j & 1]);
+            }
+            sum[0] = add2_rn(sum[0], sum[1]);
+            float sq = f2_lo(sum[0]) + f2_hi(sum[0]);
+            sq += __shfl_xor_sync(0xFFFFFFFFu, sq, 1);
+            sq += __shfl_xor_sync(0xFFFFFFFFu, sq, 2);
+            // 2^(k - 1) <= norm < 2^k
+            const int k = static_cast<int>((max(__float_as_uint(sq) >> 23, 7u) + 1) >> 1) - 63;
+            const float f = __uint_as_float(static_cast<uint32_t>(127 + 14 - k) << 23);
+            float back = __uint_as_float(static_cast<uint32_t>(127 - 14 + k) << 23);
+            if (p.normalize) back *= rsqrtf(sq + kGdnNormEps);
+#pragma unroll
+            for (int x = 0; x < kTurns; ++x) {
+                const int at = ((x + r8) % kTurns) * 4 + lane % 4;
+                const uint32_t y[4] = {raw[u][x].x, raw[u][x].y, raw[u][x].z, raw[u][x].w};
+                uint32_t o[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) o[j] = half2_of(mul2_rn(bf16x2_to_f2(y[j]), f2(f, f)));
+                *reinterpret_cast<uint4*>(sh.kq[at / 8] + r * 128 + ((at % 8) ^ r8) * 16) = uint4{o[0], o[1], o[2], o[3]};
+            }
+            if (lane % 4 == 0) (r < 64 ? sh.row_k : sh.row_q - 64)[r] = r % 64 >= left ? 0.0f : r < 64 ? back : back * p.scale;
+        }
+        fence_proxy_async_smem();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tm = sh.tmem;
+    GdnWait wait{&sh.abort, limit_ns};
+    if (tid == 0) {
+        const uint64_t d = sw128_kmajor_desc(smem_u32(sh.kq));
+#pragma unroll
+        for (int ks = 0; ks < DK / 16; ++ks) {
+            const uint64_t y = d + (ks / 4) * 1024 + (ks % 4) * 2;
+            umma_f16(tm + kTmKk, y, y, idesc_f16_f32(128, 64, false), ks > 0);
+        }
+        umma_commit(&sh.kk_done);
+        if (head0 == 0) {
+            bulk_store(out.kq + (static_cast<long long>(blockIdx.x) * p.k_heads + hk) * (DK / 64) * 16384, sh.kq, (DK / 64) * 16384);
+            bulk_commit_group();
+        }
+        bulk_wait_read_all();
+    }
+    __syncwarp();
+
+    const uint32_t lanes = tm + (static_cast<uint32_t>(warp * 32) << 16);
+    const int l = lane;
+    const bool is_q = warp >= 2, upper = (warp & 1) != 0;             // warps 0, 1: rows of k; 2, 3: of q; upper: rows 32..
+    const int i = upper ? 32 + l : l;                                 // this lane's row
+    auto piece = [&](int j) { return (j ^ (l & 7)); };
+    const float row_k = sh.row_k[i];
+    GdnTiles& st = *reinterpret_cast<GdnTiles*>(sh.kq);
+    uint32_t turn = 0;
+#pragma unroll 1
+    for (int head = 0; head < heads; ++head) {
+        if (head % 4 == 0) {
+            // running sums of g of four heads, one a warp, in log2 units: multiples of 2^-8 (exact in float32) and the rest,
+            // so that differences of far running sums keep their low bits; decays below 2^-128 count as 0
+            if (head > 0) __syncthreads();
+            if (head + warp < heads) {
+                float hi[2], lo[2], be[2];
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const bool real = lane * 2 + j < left;
+                    const long long at = (static_cast<long long>(r0) + (real ? lane * 2 + j : 0)) * p.v_heads + hk * group + head0 + head + warp;
+                    const float y = real ? p.g[at] * 1.44269504f : 0.0f, x = y < -128.0f ? -128.0f : y;
+                    be[j] = real ? p.beta[at] : 0.0f;
+                    hi[j] = rintf(x * 256.0f) * 0.00390625f;
+                    lo[j] = x - hi[j];
+                }
+                float sum_h = hi[0] + hi[1], sum_l = lo[0] + lo[1];
+#pragma unroll 1
+                for (int m = 1; m < 32; m <<= 1) {
+                    const float a = __shfl_up_sync(0xFFFFFFFFu, sum_h, m), x = __shfl_up_sync(0xFFFFFFFFu, sum_l, m);
+                    if (lane >= m) sum_h += a, sum_l += x;
+                }
+                *reinterpret_cast<float2*>(sh.g_hi[warp] + 2 * lane) = float2{sum_h - hi[1], sum_h};
+                *reinterpret_cast<float2*>(sh.g_lo[warp] + 2 * lane) = float2{sum_l - lo[1], sum_l};
+                *reinterpret_cast<float2*>(sh.beta[warp] + 2 * lane) = float2{be[0], be[1]};
+            }
+            __syncthreads();
+            if (head == 0) {
+                wait(&sh.kk_done, 0, kStatusTimeoutAccFull);
+                tc_fence_after();
+            }
+        }
+        const float *g_hi_s = sh.g_hi[head % 4], *g_lo_s = sh.g_lo[head % 4], *beta_s = sh.beta[head % 4];
+        GdnTiles* to = out.tiles + static_cast<long long>(blockIdx.x) * p.v_heads + hk * group + head0 + head;
+        {
+            const float g_hi = g_hi_s[i], g_lo = g_lo_s[i], beta = beta_s[i];
+            // the head before has left the tiles
+            if (tid % 64 == 0) bulk_wait_read_all();
+            if (is_q) named_bar_sync(6, 64);
+            // The row's products with the rows of k before it, with their decays, 8 at a time.  k and q have 2-norms below
+            // 2^14, so that products times kGdnDown fit fp16 (with room for a g above 0) and need no look at the row first:
+            // the scales of P's columns go with V', those of A[32.., ..31] with what it is multiplied by.
+#pragma unroll 1
+            for (int o = 0; o < (upper ? 64 : 32); o += 16) {
+                uint32_t x[16];
+                uint64_t y[8];
+                tmem_ld_x16_sync(lanes + kTmKk + o, x);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const uint64_t h = sub2_rn(f2(g_hi, g_hi), *reinterpret_cast<const uint64_t*>(g_hi_s + o + 2 * e));
+                    const uint64_t d = add2_rn(h, sub2_rn(f2(g_lo, g_lo), *reinterpret_cast<const uint64_t*>(g_lo_s + o + 2 * e)));
+                    y[e] = mul2_rn(f2(ex2(f2_lo(d)), ex2(f2_hi(d))), u2(x[2 * e], x[2 * e + 1]));
+                }
+                if (is_q) {
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        uint32_t hi[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int at = o + 8 * q + 2 * e;
+                            const uint64_t w = mul2_rn(y[4 * q + e], f2(kGdnDown, kGdnDown));
+                            hi[e] = half2_bits(at <= i ? f2_lo(w) : 0.0f, at + 1 <= i ? f2_hi(w) : 0.0f);
+                        }
+                        *reinterpret_cast<uint4*>(st.p + i * 128 + piece(o / 8 + q) * 16) = uint4{hi[0], hi[1], hi[2], hi[3]};
+                    }
+                } else if (o < 32 && upper) {
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        uint32_t hi[4], lo[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) split2(y[4 * q + e], f2(kGdnDown, kGdnDown), hi[e], lo[e]);
+                        *reinterpret_cast<uint4*>(sh.a21[0] + l * 128 + piece(o / 8 + q) * 16) = uint4{hi[0], hi[1], hi[2], hi[3]};
+                        *reinterpret_cast<uint4*>(sh.a21[1] + l * 128 + piece(o / 8 + q) * 16) = uint4{lo[0], lo[1], lo[2], lo[3]};
+                    }
+                } else {
+                    const float f = -row_k * beta;
+                    float* a = (upper ? sh.a22 : sh.a11) + l * 32;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        y[e] = mul2_rn(y[e], mul2_rn(f2(f, f), *reinterpret_cast<const uint64_t*>(sh.row_k + o + 2 * e)));
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        *reinterpret_cast<ulonglong2*>(a + piece((o & 31) / 4 + q) * 4) = ulonglong2{y[2 * q], y[2 * q + 1]};
+                }
+            }
+            if (is_q) {
+                if (!upper)
+#pragma unroll
+                    for (int e = 4; e < 8; ++e) *reinterpret_cast<uint4*>(st.p + i * 128 + piece(e) * 16) = uint4{};
+                const float f = sh.row_q[i];
+                st.c_q[i] = f * ex2(g_hi + g_lo);
+                st.c_p[i] = f * kGdnUp;
+                if (i == 0) st.gamma = ex2(g_hi_s[kChunk - 1] + g_lo_s[kChunk - 1]);
+                fence_proxy_async_smem();
+                named_bar_sync(6, 64);
+                if (tid == 64 && !wait.dead) {
+                    bulk_store(to->p, st.p, sizeof(st.p));
+                    bulk_store(to->c_q, st.c_q, kGdnTilesBytes - offsetof(GdnTiles, c_q));
+                    bulk_commit_group();
+                }
+                __syncwarp();
+                continue;
+            }
+            (upper ? sh.a22 : sh.a11)[l * 32 + piece(l / 4) * 4 + l % 4] = 0.0f;
+            fence_proxy_async_smem();
+            uint64_t z[16], z1[16];                   // T's row: columns ..31 and 32..
+#pragma unroll
+            for (int j = 0; j < 16; ++j) z[j] = f2(2 * j == l ? 1.0f : 0.0f, 2 * j + 1 == l ? 1.0f : 0.0f), z1[j] = 0;
+            named_bar_sync(5, 64);
+#pragma unroll 1
+            for (int pass = upper ? 0 : 1; pass < 2; ++pass) {
+                solve32(z, pass == 0 ? sh.a22 : sh.a11);
+                if (pass == 0) {
+                    // z (columns 32..) is done; its product with A[32.., ..31] on the tensor cores, then columns ..31
+                    uint64_t y[16];
+                    float m = 0.0f;
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        y[j] = mul2_rn(z[j], mul2_rn(*reinterpret_cast<const uint64_t*>(beta_s + 32 + 2 * j),
+                                                     *reinterpret_cast<const uint64_t*>(sh.row_k + 32 + 2 * j)));
+                        m = max3(m, y[j]);
+                    }
+                    const float2 f = scale_of(m);
+                    uint32_t hi[16], lo[16];
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) split2(y[j], f2(f.x, f.x), hi[j], lo[j]);
+                    tmem_st_x16(lanes + kTmZ, hi);
+                    tmem_st_x16(lanes + kTmZ + 16, lo);
+                    tmem_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0 && !wait.dead) {
+                        tc_fence_after();
+                        const uint64_t hi_desc = sw128_mn_desc(smem_u32(sh.a21[0]), 4096), lo_desc = sw128_mn_desc(smem_u32(sh.a21[1]), 4096);
+#pragma unroll 2
+                        for (int e = 0; e < 6; ++e) {
+                            const int ks = e % 2, term = e / 2;
+                            umma_f16_ts(tm + kTmU, tm + kTmZ + (term == 1 ? 16 : 0) + ks * 8, (term == 2 ? lo_desc : hi_desc) + ks * 128,
+                                        idesc_f16_f32(128, 32, true), e > 0);
+                        }
+                        umma_commit(&sh.z_done);
+                    }
+                    __syncwarp();
+                    wait(&sh.z_done, turn & 1, kStatusTimeoutAccFull);
+                    tc_fence_after();
+                    uint32_t x[32];
+                    tmem_ld_x32_sync(lanes + kTmU, x);
+                    tc_fence_before();
+                    const float g = -f.y * kGdnUp;
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        z1[j] = z[j];
+                        z[j] = mul2_rn(u2(x[2 * j], x[2 * j + 1]), mul2_rn(f2(g, g), *reinterpret_cast<const uint64_t*>(sh.row_k + 2 * j)));
+                    }
+                }
+            }
+            float m = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) m = max3(max3(m, z[j]), z1[j]);
+            const float2 f = scale_of(m);
+            st.c_x[i] = -row_k * beta * ex2(g_hi + g_lo);
+            st.c_b[i] = beta;
+            st.c_v[i] = row_k * ex2((g_hi_s[kChunk - 1] - g_hi) + (g_lo_s[kChunk - 1] - g_lo)) * f.y;
+            st.c_u[i] = row_k * f.y;
+#pragma unroll 1
+            for (int o = 0; o < 8; o += 4) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    uint32_t hi[4], lo[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) split2(z[4 * j + e], f2(f.x, f.x), hi[e], lo[e]);
+                    *reinterpret_cast<uint4*>(st.t_hi + i * 128 + piece(o + j) * 16) = uint4{hi[0], hi[1], hi[2], hi[3]};
+                    *reinterpret_cast<uint4*>(st.t_lo + i * 128 + piece(o + j) * 16) = uint4{lo[0], lo[1], lo[2], lo[3]};
+                }
+#pragma unroll
+                for (int j = 0; j < 16; ++j) z[j] = z1[j];
+            }
+            fence_proxy_async_smem();
+            named_bar_sync(5, 64);                    // (the next head may have a11, a22 and a21 as well)
+            if (tid == 0 && !wait.dead) {
+                bulk_store(to->t_hi, st.t_hi, sizeof(st.t_hi) + sizeof(st.t_lo));
+                bulk_store(to->c_x, st.c_x, 4 * sizeof(st.c_x));
+                bulk_commit_group();
+            }
+            __syncwarp();
+            ++turn;
+        }
+    }
+    if (warp < 2 && lane == 0) drain_mmas(&sh.drained[warp]);
+    if (tid % 64 == 0) bulk_wait_all();
+    tc_fence_before();
+    __syncthreads();
+    if (tid == 0 && sh.abort) atomicOr(&g_mixer_status, sh.abort);
+    if (warp == 0) tmem_dealloc(tm, 128);
+}
+
 template <int DK, int DV>
 __global__ void __launch_bounds__(kChunkThreads, 1) gdn_chunk_kernel(const __grid_constant__ GdnParams p,
-                                                                     const __grid_constant__ GdnMaps maps, uint32_t limit_ns) {
+                                                                     const __grid_constant__ GdnMaps maps, const GdnScratch in,
+                                                                     uint32_t limit_ns) {
     extern __shared__ uint8_t smem_raw[];
-    // (an offset into the array, not an integer made a pointer: the accesses stay known as shared-memory ones)
     GdnShared& sh = *reinterpret_cast<GdnShared*>(smem_raw + (-smem_u32(smem_raw) & 1023u));
     const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
     const int hv = blockIdx.x, hk = hv / (p.v_heads / p.k_heads);
@@ -256,30 +606,44 @@ __global__ void __launch_bounds__(kChunkThreads, 1) gdn_chunk_kernel(const __gri
         __syncthreads();
         b = sh.sequence;
     }
-    gdn_rows(p, b, &r0, &r1);
-    const int slot = gdn_slot(p, b), rows = r1 - r0, chunks = (rows + kChunk - 1) / kChunk;
-    if (slot < 0) {
-        __nv_bfloat16* out = p.out + (static_cast<long long>(r0) * p.v_heads + hv) * DV;
-        for (int e = tid; e < rows * (DV / 8); e += kChunkThreads)
-            *reinterpret_cast<uint4*>(out + static_cast<long long>(e / (DV / 8)) * p.v_heads * DV + e % (DV / 8) * 8) = uint4{};
-        return;
+    // chunks of the sequences before
+    if (tid == 0) sh.before = 0;
+    __syncthreads();
+    {
+        int n = 0;
+        for (int i = tid; i < b; i += kChunkThreads) n += gdn_chunks_of(p, i);
+        if (n) atomicAdd(&sh.before, n);
     }
-    float* state = p.state + (static_cast<long long>(slot) * p.v_heads + hv) * DK * DV;
-    if (chunks == 0) {
-        if (!p.carry)
+    __syncthreads();
+    gdn_rows(p, b, &r0, &r1);
+    const int slot = gdn_slot(p, b), all = gdn_chunks_of(p, b);
+    // this launch's part of the sequence
+    const int first = max(in.x0 - sh.before, 0), chunks = min(all, in.x0 + in.chunks - sh.before) - first;
+    const int x_first = sh.before + first - in.x0;                    // its place in the scratch memory
+    const bool from_state = p.carry || first > 0;
+    r0 += first * kChunk;
+    const int rows = min(r1 - r0, chunks * kChunk);
+    float* state = p.state + (static_cast<long long>(max(slot, 0)) * p.v_heads + hv) * DK * DV;
+    if (slot < 0 || chunks <= 0) {
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        if (slot < 0) {
+            __nv_bfloat16* o = p.out + (static_cast<long long>(r0) * p.v_heads + hv) * DV;
+            for (int e = tid; e < rows * (DV / 8); e += kChunkThreads)
+                *reinterpret_cast<uint4*>(o + static_cast<long long>(e / (DV / 8)) * p.v_heads * DV + e % (DV / 8) * 8) = uint4{};
+        } else if (all == 0 && !p.carry && in.x0 == 0) {
             for (int e = tid; e < DK * DV; e += kChunkThreads) state[e] = 0.0f;
+        }
         return;
     }
 
-    if (warp == 12) tmem_alloc(&sh.tmem, 512);
+    if (warp == 8) tmem_alloc(&sh.tmem, 512);
     if (tid == 0) {
-        for (int i = 0; i < kKqSlots; ++i) mbar_init(&sh.kq_in[i], 1), mbar_init(&sh.rows_full[i], 3), mbar_init(&sh.rows_free[i], 1);
+        for (int i = 0; i < kKqSlots; ++i) mbar_init(&sh.kq_in[i], 1), mbar_init(&sh.kq_free[i], 1);
         for (int i = 0; i < 2; ++i) mbar_init(&sh.v_in[i], 1), mbar_init(&sh.v_free[i], 8);
-        for (int i = 0; i < 2; ++i) mbar_init(&sh.tiles_full[i], 4), mbar_init(&sh.tiles_free[i], 8);
+        for (int i = 0; i < 2; ++i) mbar_init(&sh.tiles_in[i], 1), mbar_init(&sh.tiles_free[i], 8);
         mbar_init(&sh.s_ready, 8), mbar_init(&sh.r_ready, 8), mbar_init(&sh.v_ready, 8);
         mbar_init(&sh.x_done, 1), mbar_init(&sh.v_done, 1), mbar_init(&sh.d_done, 1), mbar_init(&sh.y_done, 1);
-        mbar_init(&sh.kk_done, 1), mbar_init(&sh.kk_free, 4), mbar_init(&sh.z_done, 1);
-        for (int i = 0; i < 3; ++i) mbar_init(&sh.drained[i], 1);
+        mbar_init(&sh.drained, 1);
         sh.abort = 0;
         fence_mbar_init();
     }
@@ -287,6 +651,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) gdn_chunk_kernel(const __gri
     __syncthreads();
     tc_fence_after();
     const uint32_t tm = sh.tmem;
+    asm volatile("griddepcontrol.wait;" ::: "memory");                // the tiles, and all that came before
     GdnWait wait{&sh.abort, limit_ns};
     const int quarter = warp % 4;
     const uint32_t lanes = tm + (static_cast<uint32_t>(quarter * 32) << 16);
@@ -304,7 +669,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) gdn_chunk_kernel(const __gri
 #pragma unroll
         for (int i = 0; i < kS / 2; ++i) {
             const float* at = state + (part * kS + 2 * i) * DV + n;
-            s[i] = p.carry && n < DV ? f2(at[0], at[DV]) : 0;
+            s[i] = from_state && n < DV ? f2(at[0], at[DV]) : 0;
         }
         int turn = 0;
         // Largest of both parts of this thread's row (the two warps of a quarter meet).
@@ -319,7 +684,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) gdn_chunk_kernel(const __gri
         const uint16_t* vcol = reinterpret_cast<const uint16_t*>(sh.v[0]) + part * 32 * DV + (n < DV ? n : 0);
         float sq = 0.0f, sv = 0.0f;          // scales of the S behind X_q and the V' behind Y
 #pragma unroll 1
-        for (int c = 0;; ++c) {
+        for (int c = 0;; ++c) {                // (c counts from the first chunk of this launch)
             const uint32_t par = c & 1;
             float2 ss = {};
             if (c < chunks) {
@@ -386,7 +751,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) gdn_chunk_kernel(const __gri
             const GdnTiles& st = sh.tiles[par];
             sq = ss.y;
             // X_k -> R
-            wait(&sh.tiles_full[par], (c >> 1) & 1, kStatusTimeoutFull);
+            wait(&sh.tiles_in[par], (c >> 1) & 1, kStatusTimeoutFull);
             wait(&sh.v_in[par], (c >> 1) & 1, kStatusTimeoutFull);
             wait(&sh.x_done, par, kStatusTimeoutAccFull);
             tc_fence_after();
@@ -482,401 +847,107 @@ __global__ void __launch_bounds__(kChunkThreads, 1) gdn_chunk_kernel(const __gri
                 at[0] = f2_lo(s[i]), at[DV] = f2_hi(s[i]);
             }
         if (lane == 0) bulk_wait_all();
-    } else if (warp < 12) {
-        // ---------------------------------------------------------------------------------- T and P of the chunks ahead
-        const int l = lane;
-        const bool is_q = quarter >= 2, upper = (quarter & 1) != 0;   // upper: rows 32.. of the chunk
-        const int i = upper ? 32 + l : l;                             // this lane's row, of k (warps 8, 9) or q (10, 11)
-        auto piece = [&](int j) { return (j ^ (l & 7)); };
-        // [k; q] k^T of a chunk, once its tiles are there
-        auto products = [&](int c) {
-            if (lane == 0) {
-                GdnRows& in = sh.rows[c % kKqSlots];
-                wait(&sh.rows_full[c % kKqSlots], (c / kKqSlots) & 1, kStatusTimeoutFull);
-                if (c > 0) wait(&sh.kk_free, (c - 1) & 1, kStatusTimeoutAccEmpty);
-                if (wait.dead) return;
-                tc_fence_after();
-                const uint64_t d = sw128_kmajor_desc(smem_u32(in.kq));
-#pragma unroll 1
-                for (int ks = 0; ks < DK / 16; ++ks) {
-                    const uint64_t y = d + (ks / 4) * 1024 + (ks % 4) * 2;
-                    umma_f16(tm + kTmPrep, y, y, idesc_f16_f32(128, 64, false), ks > 0);
-                }
-                umma_commit(&sh.kk_done);
-            }
-        };
-        if (warp == 8) products(0);
-        __syncwarp();
-#pragma unroll 1
-        for (int c = 0, slot_k = 0; c < chunks; ++c, slot_k = slot_k == kKqSlots - 1 ? 0 : slot_k + 1) {
-            const uint32_t par = c & 1;
-            const GdnRows& in = sh.rows[slot_k];
-            GdnTiles& st = sh.tiles[par];
-            wait(&sh.rows_full[slot_k], (c / kKqSlots) & 1, kStatusTimeoutFull);
-            wait(&sh.kk_done, par, kStatusTimeoutAccFull);
-            if (c > 1) wait(&sh.tiles_free[par], ((c >> 1) - 1) & 1, kStatusTimeoutEmpty);
-            tc_fence_after();
-            const float g_hi = in.g_hi[i], g_lo = in.g_lo[i], row_k = in.row_k[i], beta = in.beta[i];
-            if (!is_q) named_bar_sync(5, 64);      // the chunk before has been solved: a11, a22 and a21 are free
-            // The row's products with the rows of k before it, with their decays, 8 at a time.  k and q have 2-norms below
-            // 2^14, so that products times kGdnDown fit fp16 (with room for a g above 0) and need no look at the row first:
-            // the scales of P's columns go with V', those of A[32.., ..31] with what it is multiplied by.
-#pragma unroll 1
-            for (int o = 0; o < (upper ? 64 : 32); o += 16) {
-                uint32_t x[16];
-                uint64_t y[8];
-                tmem_ld_x16_sync(lanes + kTmPrep + o, x);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const uint64_t h = sub2_rn(f2(g_hi, g_hi), *reinterpret_cast<const uint64_t*>(in.g_hi + o + 2 * e));
-                    const uint64_t d = add2_rn(h, sub2_rn(f2(g_lo, g_lo), *reinterpret_cast<const uint64_t*>(in.g_lo + o + 2 * e)));
-                    y[e] = mul2_rn(f2(ex2(f2_lo(d)), ex2(f2_hi(d))), u2(x[2 * e], x[2 * e + 1]));
-                }
-                if (is_q) {
-#pragma unroll
-                    for (int q = 0; q < 2; ++q) {
-                        uint32_t hi[4];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int at = o + 8 * q + 2 * e;
-                            const uint64_t w = mul2_rn(y[4 * q + e], f2(kGdnDown, kGdnDown));
-                            hi[e] = half2_bits(at <= i ? f2_lo(w) : 0.0f, at + 1 <= i ? f2_hi(w) : 0.0f);
-                        }
-                        *reinterpret_cast<uint4*>(st.p + i * 128 + piece(o / 8 + q) * 16) = uint4{hi[0], hi[1], hi[2], hi[3]};
-                    }
-                } else if (o < 32 && upper) {
-#pragma unroll
-                    for (int q = 0; q < 2; ++q) {
-                        uint32_t hi[4], lo[4];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) split2(y[4 * q + e], f2(kGdnDown, kGdnDown), hi[e], lo[e]);
-                        *reinterpret_cast<uint4*>(sh.a21[0] + l * 128 + piece(o / 8 + q) * 16) = uint4{hi[0], hi[1], hi[2], hi[3]};
-                        *reinterpret_cast<uint4*>(sh.a21[1] + l * 128 + piece(o / 8 + q) * 16) = uint4{lo[0], lo[1], lo[2], lo[3]};
-                    }
-                } else {
-                    const float f = -row_k * beta;
-                    float* a = (upper ? sh.a22 : sh.a11) + l * 32;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        y[e] = mul2_rn(y[e], mul2_rn(f2(f, f), *reinterpret_cast<const uint64_t*>(in.row_k + o + 2 * e)));
-#pragma unroll
-                    for (int q = 0; q < 4; ++q)
-                        *reinterpret_cast<ulonglong2*>(a + piece((o & 31) / 4 + q) * 4) = ulonglong2{y[2 * q], y[2 * q + 1]};
-                }
-            }
-            if (is_q) {
-                tc_fence_before();
-                if (!upper) {
-#pragma unroll
-                    for (int e = 4; e < 8; ++e) *reinterpret_cast<uint4*>(st.p + i * 128 + piece(e) * 16) = uint4{};
-                } else {
-                    // columns 32.. may be written (both warps wait: one that arrived alone could, after a wait that expired,
-                    // arrive twice and leave the other without a partner)
-                    named_bar_sync(6, 64);
-                }
-                const float f = in.row_q[i];
-                st.c_q[i] = f * ex2(g_hi + g_lo);
-                st.c_p[i] = f * kGdnUp;
-                if (i == 0) st.gamma = ex2(in.g_hi[kChunk - 1] + in.g_lo[kChunk - 1]);
-                fence_proxy_async_smem();
-                arrive(&sh.kk_free);
-                arrive(&sh.tiles_full[par]);
-                continue;
-            }
-            (upper ? sh.a22 : sh.a11)[l * 32 + piece(l / 4) * 4 + l % 4] = 0.0f;
-            if (!upper) {
-                tc_fence_before();
-                arrive(&sh.kk_free);
-            }
-            fence_proxy_async_smem();
-            uint64_t z[16], z1[16];                   // T's row: columns ..31 and 32..
-#pragma unroll
-            for (int j = 0; j < 16; ++j) z[j] = f2(2 * j == l ? 1.0f : 0.0f, 2 * j + 1 == l ? 1.0f : 0.0f), z1[j] = 0;
-            named_bar_sync(5, 64);
-#pragma unroll 1
-            for (int pass = upper ? 0 : 1; pass < 2; ++pass) {
-                solve32(z, pass == 0 ? sh.a22 : sh.a11);
-                if (pass == 0) {
-                    // z (columns 32..) is done; its product with A[32.., ..31] on the tensor cores, then columns ..31
-                    uint64_t y[16];
-                    float m = 0.0f;
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        y[j] = mul2_rn(z[j], mul2_rn(*reinterpret_cast<const uint64_t*>(in.beta + 32 + 2 * j),
-                                                     *reinterpret_cast<const uint64_t*>(in.row_k + 32 + 2 * j)));
-                        m = max3(m, y[j]);
-                    }
-                    const float2 f = scale_of(m);
-                    uint32_t hi[16], lo[16];
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) split2(y[j], f2(f.x, f.x), hi[j], lo[j]);
-                    tmem_st_x16(lanes + kTmPrep, hi);
-                    tmem_st_x16(lanes + kTmPrep + 16, lo);
-                    tmem_wait_st();
-                    tc_fence_before();
-                    named_bar_sync(6, 64);
-                    if (lane == 0 && !wait.dead) {
-                        tc_fence_after();
-                        const uint64_t hi_desc = sw128_mn_desc(smem_u32(sh.a21[0]), 4096), lo_desc = sw128_mn_desc(smem_u32(sh.a21[1]), 4096);
-#pragma unroll 2
-                        for (int e = 0; e < 6; ++e) {
-                            const int ks = e % 2, term = e / 2;
-                            umma_f16_ts(tm + kTmPrep + 32, tm + kTmPrep + (term == 1 ? 16 : 0) + ks * 8, (term == 2 ? lo_desc : hi_desc) + ks * 128,
-                                        idesc_f16_f32(128, 32, true), e > 0);
-                        }
-                        umma_commit(&sh.z_done);
-                    }
-                    __syncwarp();
-                    wait(&sh.z_done, par, kStatusTimeoutAccFull);
-                    tc_fence_after();
-                    uint32_t x[32];
-                    tmem_ld_x32_sync(lanes + kTmPrep + 32, x);
-                    tc_fence_before();
-                    arrive(&sh.kk_free);
-                    const float g = -f.y * kGdnUp;
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        z1[j] = z[j];
-                        z[j] = mul2_rn(u2(x[2 * j], x[2 * j + 1]), mul2_rn(f2(g, g), *reinterpret_cast<const uint64_t*>(in.row_k + 2 * j)));
-                    }
-                }
-            }
-            float m = 0.0f;
-#pragma unroll
-            for (int j = 0; j < 16; ++j) m = max3(max3(m, z[j]), z1[j]);
-            const float2 f = scale_of(m);
-            st.c_x[i] = -row_k * beta * ex2(g_hi + g_lo);
-            st.c_b[i] = beta;
-            st.c_v[i] = row_k * ex2((in.g_hi[kChunk - 1] - g_hi) + (in.g_lo[kChunk - 1] - g_lo)) * f.y;
-            st.c_u[i] = row_k * f.y;
-#pragma unroll 1
-            for (int o = 0; o < 8; o += 4) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    uint32_t hi[4], lo[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) split2(z[4 * j + e], f2(f.x, f.x), hi[e], lo[e]);
-                    *reinterpret_cast<uint4*>(st.t_hi + i * 128 + piece(o + j) * 16) = uint4{hi[0], hi[1], hi[2], hi[3]};
-                    *reinterpret_cast<uint4*>(st.t_lo + i * 128 + piece(o + j) * 16) = uint4{lo[0], lo[1], lo[2], lo[3]};
-                }
-#pragma unroll
-                for (int j = 0; j < 16; ++j) z[j] = z1[j];
-            }
-            fence_proxy_async_smem();
-            arrive(&sh.tiles_full[par]);
-            if (warp == 8 && c + 1 < chunks) products(c + 1);
-            __syncwarp();
-        }
-        if (warp < 10 && lane == 0) drain_mmas(&sh.drained[warp - 8]);
-    } else {
-        if (warp == 13) {
-            // --------------------------------------------------------------------------- issuer of the chain's MMAs
-            if (lane == 0) {
-                constexpr uint32_t id64 = idesc_f16_f32(128, 64, false);
-                constexpr uint32_t id_d = idesc_f16_f32(128, DK, true);
-#pragma unroll 1
-                for (int c = 0, slot_k = 0; c < chunks; ++c, slot_k = slot_k == kKqSlots - 1 ? 0 : slot_k + 1) {
-                    const uint32_t par = c & 1;
-                    GdnTiles& st = sh.tiles[par];
-                    const uint32_t kq_at = smem_u32(sh.rows[slot_k].kq);
-                    const uint64_t kq = sw128_kmajor_desc(kq_at), kmn = sw128_mn_desc(kq_at, 16384);
-                    const uint64_t thi = sw128_kmajor_desc(smem_u32(st.t_hi)), tlo = sw128_kmajor_desc(smem_u32(st.t_lo));
-                    const uint64_t pd = sw128_kmajor_desc(smem_u32(st.p));
-                    wait(&sh.rows_full[slot_k], (c / kKqSlots) & 1, kStatusTimeoutFull);
-                    wait(&sh.s_ready, par, kStatusTimeoutEmpty);
-                    if (wait.dead) break;
-                    tc_fence_after();
-                    // descriptor addresses count in units of 16 bytes
-#pragma unroll 4
-                    for (int e = 0; e < 2 * (DK / 16); ++e) {
-                        const int ks = e % (DK / 16);
-                        umma_f16_ts(tm + kTmXk, tm + kTmS + (e / (DK / 16)) * 64 + ks * 8, kq + (ks / 4) * 1024 + (ks % 4) * 2, id64, e > 0);
-                    }
-                    umma_commit(&sh.x_done);
-                    // the chunk before's X_q has been read
-                    if (c > 0) wait(&sh.tiles_free[par ^ 1], ((c - 1) >> 1) & 1, kStatusTimeoutEmpty);
-                    if (wait.dead) break;
-                    tc_fence_after();
-#pragma unroll 4
-                    for (int ks = 0; ks < DK / 16; ++ks)
-                        umma_f16_ts(tm + kTmXq, tm + kTmS + ks * 8, kq + 512 + (ks / 4) * 1024 + (ks % 4) * 2, id64, ks > 0);
-                    wait(&sh.tiles_full[par], (c >> 1) & 1, kStatusTimeoutFull);
-                    wait(&sh.r_ready, par, kStatusTimeoutEmpty);
-                    if (wait.dead) break;
-                    tc_fence_after();
-#pragma unroll 4
-                    for (int e = 0; e < 12; ++e) {
-                        const int ks = e % 4, term = e / 4;      // hi hi, lo hi, hi lo
-                        umma_f16_ts(tm + kTmV, tm + kTmR + (term == 1 ? 32 : 0) + ks * 8, (term == 2 ? tlo : thi) + ks * 2, id64, e > 0);
-                    }
-                    umma_commit(&sh.v_done);
-                    wait(&sh.v_ready, par, kStatusTimeoutEmpty);
-                    if (wait.dead) break;
-                    tc_fence_after();
-#pragma unroll 4
-                    for (int e = 0; e < 8; ++e)
-                        umma_f16_ts(tm + kTmS, tm + kTmXk + (e / 4) * 32 + (e % 4) * 8, kmn + (e % 4) * 128, id_d, e > 0);
-                    umma_commit(&sh.d_done);
-                    umma_commit(&sh.rows_free[slot_k]);
-#pragma unroll 4
-                    for (int ks = 0; ks < 4; ++ks) umma_f16_ts(tm + kTmY, tm + kTmR + ks * 8, pd + ks * 2, id64, ks > 0);
-                    umma_commit(&sh.y_done);
-                }
-                drain_mmas(&sh.drained[2]);
-            }
-            __syncwarp();
-        } else {
-            // ----------------------------------------------------------------------------------------- rows in
-            const int w = warp == 12 ? 0 : warp - 13, t = w * 32 + lane;
-            constexpr int kPieces = DK / 8;                               // 16-byte pieces of a row
-            const uint64_t policy = l2_policy_evict_normal();
-            int kq_loads = 0, v_loads = 0;                                // copies started by this thread
-            auto load_kq = [&](int c, int slot_k) {
-                if (t == 0 && !wait.dead) {
-                    ++kq_loads;
-                    uint64_t* bar = &sh.kq_in[slot_k];
-                    fence_proxy_async_smem();
-                    mbar_arrive_expect_tx(bar, kChunk * 4 * DK);
-#pragma unroll 1
-                    for (int h = 0; h < DK / 64; ++h) {
-                        tma_load_2d(sh.rows[slot_k].kq[h], &maps.k, bar, hk * DK + h * 64, r0 + c * kChunk, policy);
-                        tma_load_2d(sh.rows[slot_k].kq[h] + kChunk * 128, &maps.q, bar, hk * DK + h * 64, r0 + c * kChunk, policy);
-                    }
-                }
-            };
-            auto gates = [&](int c, float (&g)[2], float (&beta)[2]) {
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const int row = c * kChunk + lane * 2 + j;
-                    const long long at = (static_cast<long long>(r0) + row) * p.v_heads + hv;
-                    g[j] = row < rows ? p.g[at] : 0.0f;
-                    beta[j] = row < rows ? p.beta[at] : 0.0f;
-                }
-            };
-            // Each lane's pieces of its row, in an order that the row's number turns, so that the eight lanes of a
-            // shared-memory pass meet all banks.
-            int at[kPieces / 4];
-#pragma unroll
-            for (int x = 0; x < kPieces / 4; ++x) {
-                const int r = lane / 4, y = ((x + r) % (kPieces / 4)) * 4 + lane % 4;
-                at[x] = (y / 8) * 16384 + r * 128 + ((y % 8) ^ r) * 16;
-            }
-            load_kq(0, 0);
-            if (chunks > 1) load_kq(1, 1);
-            float g[2] = {}, beta[2] = {};
-            if (w == 0) gates(0, g, beta);
+    } else if (warp == 8) {
+        // --------------------------------------------------------------------------- issuer of the chain's MMAs
+        if (lane == 0) {
+            constexpr uint32_t id64 = idesc_f16_f32(128, 64, false);
+            constexpr uint32_t id_d = idesc_f16_f32(128, DK, true);
 #pragma unroll 1
             for (int c = 0, slot_k = 0; c < chunks; ++c, slot_k = slot_k == kKqSlots - 1 ? 0 : slot_k + 1) {
                 const uint32_t par = c & 1;
-                GdnRows& in = sh.rows[slot_k];
-                // running sums of g in log2 units: multiples of 2^-8 (exact in float32) and the rest, so that differences
-                // of far running sums keep their low bits; decays below 2^-128 count as 0
-                if (w == 0) {
-                    float hi[2], lo[2];
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        const float y = g[j] * 1.44269504f, x = y < -128.0f ? -128.0f : y;
-                        hi[j] = rintf(x * 256.0f) * 0.00390625f;
-                        lo[j] = x - hi[j];
-                    }
-                    float sum_h = hi[0] + hi[1], sum_l = lo[0] + lo[1];
-#pragma unroll 1
-                    for (int m = 1; m < 32; m <<= 1) {
-                        const float a = __shfl_up_sync(0xFFFFFFFFu, sum_h, m), x = __shfl_up_sync(0xFFFFFFFFu, sum_l, m);
-                        if (lane >= m) sum_h += a, sum_l += x;
-                    }
-                    *reinterpret_cast<float2*>(in.g_hi + 2 * lane) = float2{sum_h - hi[1], sum_h};
-                    *reinterpret_cast<float2*>(in.g_lo + 2 * lane) = float2{sum_l - lo[1], sum_l};
-                    *reinterpret_cast<float2*>(in.beta + 2 * lane) = float2{beta[0], beta[1]};
-                    if (c + 1 < chunks) gates(c + 1, g, beta);
-                }
+                GdnTiles& st = sh.tiles[par];
+                const uint32_t kq_at = smem_u32(sh.kq[slot_k]);
+                const uint64_t kq = sw128_kmajor_desc(kq_at), kmn = sw128_mn_desc(kq_at, 16384);
+                const uint64_t thi = sw128_kmajor_desc(smem_u32(st.t_hi)), tlo = sw128_kmajor_desc(smem_u32(st.t_lo));
+                const uint64_t pd = sw128_kmajor_desc(smem_u32(st.p));
                 wait(&sh.kq_in[slot_k], (c / kKqSlots) & 1, kStatusTimeoutFull);
-                // k and q rows -> fp16 in their places, four lanes a row, scaled to a 2-norm in [2^13, 2^14) (a norm below
-                // 2^-60, whose square may underflow, counts as 2^-60); rows past the end, which the box takes from what
-                // follows, -> 0
-                const int left = rows - c * kChunk;
-                // (two groups of 8 rows at a time, whose latencies overlap; the last one may be done twice)
-#pragma unroll 1
-                for (int u0 = w; u0 < 16; u0 += 6) {
-                    uint4 raw[2][kPieces / 4];
-                    uint64_t sum[2] = {};
-                    float sq[2], f[2], back[2];
-#pragma unroll
-                    for (int g2 = 0; g2 < 2; ++g2) {
-                        const uint8_t* row = in.kq[0] + (g2 && u0 + 3 < 16 ? u0 + 3 : u0) * 1024;
-#pragma unroll
-                        for (int x = 0; x < kPieces / 4; ++x) raw[g2][x] = *reinterpret_cast<const uint4*>(row + at[x]);
-                    }
-#pragma unroll
-                    for (int x = 0; x < kPieces / 4; ++x)
-#pragma unroll
-                        for (int g2 = 0; g2 < 2; ++g2) {
-                            const uint32_t y[4] = {raw[g2][x].x, raw[g2][x].y, raw[g2][x].z, raw[g2][x].w};
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) sum[g2] = fma2_rn(bf16x2_to_f2(y[j]), bf16x2_to_f2(y[j]), sum[g2]);
-                        }
-#pragma unroll
-                    for (int g2 = 0; g2 < 2; ++g2) sq[g2] = f2_lo(sum[g2]) + f2_hi(sum[g2]);
-#pragma unroll
-                    for (int m = 1; m < 4; m <<= 1)
-#pragma unroll
-                        for (int g2 = 0; g2 < 2; ++g2) sq[g2] += __shfl_xor_sync(0xFFFFFFFFu, sq[g2], m);
-#pragma unroll
-                    for (int g2 = 0; g2 < 2; ++g2) {
-                        const int u = g2 && u0 + 3 < 16 ? u0 + 3 : u0, r = u * 8 + lane / 4;
-                        // 2^(k - 1) <= norm < 2^k
-                        const int k = static_cast<int>((max(__float_as_uint(sq[g2]) >> 23, 7u) + 1) >> 1) - 63;
-                        f[g2] = __uint_as_float(static_cast<uint32_t>(127 + 14 - k) << 23);
-                        back[g2] = __uint_as_float(static_cast<uint32_t>(127 - 14 + k) << 23);
-                        if (p.normalize) back[g2] *= rsqrtf(sq[g2] + kGdnNormEps);
-                        const bool real = r % 64 < left;
-                        if (!real) back[g2] = 0.0f;
-                        uint8_t* row = in.kq[0] + u * 1024;
-#pragma unroll
-                        for (int x = 0; x < kPieces / 4; ++x) {
-                            const uint32_t y[4] = {raw[g2][x].x, raw[g2][x].y, raw[g2][x].z, raw[g2][x].w};
-                            uint32_t o[4];
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) o[j] = real ? half2_of(mul2_rn(bf16x2_to_f2(y[j]), f2(f[g2], f[g2]))) : 0u;
-                            *reinterpret_cast<uint4*>(row + at[x]) = uint4{o[0], o[1], o[2], o[3]};
-                        }
-                        if (lane % 4 == 0) (r < 64 ? in.row_k : in.row_q - 64)[r] = r < 64 ? back[g2] : back[g2] * p.scale;
-                    }
+                wait(&sh.s_ready, par, kStatusTimeoutEmpty);
+                if (wait.dead) break;
+                tc_fence_after();
+                // descriptor addresses count in units of 16 bytes
+#pragma unroll 4
+                for (int e = 0; e < 2 * (DK / 16); ++e) {
+                    const int ks = e % (DK / 16);
+                    umma_f16_ts(tm + kTmXk, tm + kTmS + (e / (DK / 16)) * 64 + ks * 8, kq + (ks / 4) * 1024 + (ks % 4) * 2, id64, e > 0);
                 }
-                fence_proxy_async_smem();
-                arrive(&sh.rows_full[slot_k]);
-                if (t == 32) {
-                    if (c > 1) wait(&sh.v_free[par], ((c >> 1) - 1) & 1, kStatusTimeoutEmpty);
-                    if (!wait.dead) {
-                        ++v_loads;
-                        fence_proxy_async_smem();
-                        mbar_arrive_expect_tx(&sh.v_in[par], kChunk * 2 * DV);
-                        tma_load_2d(sh.v[par], &maps.v, &sh.v_in[par], hv * DV, r0 + c * kChunk, policy);
-                    }
+                umma_commit(&sh.x_done);
+                // the chunk before's X_q has been read
+                if (c > 0) wait(&sh.tiles_free[par ^ 1], ((c - 1) >> 1) & 1, kStatusTimeoutEmpty);
+                if (wait.dead) break;
+                tc_fence_after();
+#pragma unroll 4
+                for (int ks = 0; ks < DK / 16; ++ks)
+                    umma_f16_ts(tm + kTmXq, tm + kTmS + ks * 8, kq + 512 + (ks / 4) * 1024 + (ks % 4) * 2, id64, ks > 0);
+                wait(&sh.tiles_in[par], (c >> 1) & 1, kStatusTimeoutFull);
+                wait(&sh.r_ready, par, kStatusTimeoutEmpty);
+                if (wait.dead) break;
+                tc_fence_after();
+#pragma unroll 4
+                for (int e = 0; e < 12; ++e) {
+                    const int ks = e % 4, term = e / 4;      // hi hi, lo hi, hi lo
+                    umma_f16_ts(tm + kTmV, tm + kTmR + (term == 1 ? 32 : 0) + ks * 8, (term == 2 ? tlo : thi) + ks * 2, id64, e > 0);
                 }
-                __syncwarp();
-                if (c + 2 < chunks) {
-                    const int next = slot_k == 0 ? kKqSlots - 1 : slot_k - 1;          // (c + 2) % 3, chunk c - 1's
-                    if (w == 0 && c > 0) wait(&sh.rows_free[next], ((c - 1) / kKqSlots) & 1, kStatusTimeoutEmpty);
-                    load_kq(c + 2, next);
-                }
+                umma_commit(&sh.v_done);
+                wait(&sh.v_ready, par, kStatusTimeoutEmpty);
+                if (wait.dead) break;
+                tc_fence_after();
+#pragma unroll 4
+                for (int e = 0; e < 8; ++e)
+                    umma_f16_ts(tm + kTmS, tm + kTmXk + (e / 4) * 32 + (e % 4) * 8, kmn + (e % 4) * 128, id_d, e > 0);
+                umma_commit(&sh.d_done);
+                umma_commit(&sh.kq_free[slot_k]);
+#pragma unroll 4
+                for (int ks = 0; ks < 4; ++ks) umma_f16_ts(tm + kTmY, tm + kTmR + ks * 8, pd + ks * 2, id64, ks > 0);
+                umma_commit(&sh.y_done);
             }
-            // no copy may be in flight when the block ends
-            for (int c = max(kq_loads - kKqSlots, 0); c < kq_loads; ++c)
-                mbar_wait_bounded(&sh.kq_in[c % kKqSlots], (c / kKqSlots) & 1, kDrainNs, nullptr);
-            for (int c = max(v_loads - 2, 0); c < v_loads; ++c) mbar_wait_bounded(&sh.v_in[c & 1], (c >> 1) & 1, kDrainNs, nullptr);
+            drain_mmas(&sh.drained);
+        }
+        __syncwarp();
+    } else if (lane == 0) {
+        // ----------------------------------------------------------------------------------------------- loads
+        constexpr uint32_t kKqBytes = (DK / 64) * 16384;
+        const uint64_t policy = l2_policy_evict_normal();
+        int kq_loads = 0, pair_loads = 0;
+        auto load_kq = [&](int c) {
+            const int slot_k = c % kKqSlots;
+            if (c >= kKqSlots) wait(&sh.kq_free[slot_k], (c / kKqSlots - 1) & 1, kStatusTimeoutEmpty);
+            if (wait.dead) return;
+            ++kq_loads;
+            mbar_arrive_expect_tx(&sh.kq_in[slot_k], kKqBytes);
+            bulk_load(sh.kq[slot_k], in.kq + (static_cast<long long>(x_first + c) * p.k_heads + hk) * kKqBytes, kKqBytes, &sh.kq_in[slot_k]);
+        };
+        load_kq(0);
+#pragma unroll 1
+        for (int c = 0; c < chunks && !wait.dead; ++c) {
+            const int par = c & 1;
+            if (c + 1 < chunks) load_kq(c + 1);
+            if (c > 1) wait(&sh.v_free[par], ((c >> 1) - 1) & 1, kStatusTimeoutEmpty), wait(&sh.tiles_free[par], ((c >> 1) - 1) & 1, kStatusTimeoutEmpty);
+            if (wait.dead) break;
+            ++pair_loads;
+            mbar_arrive_expect_tx(&sh.v_in[par], kChunk * 2 * DV);
+            tma_load_2d(sh.v[par], &maps.v, &sh.v_in[par], hv * DV, r0 + c * kChunk, policy);
+            mbar_arrive_expect_tx(&sh.tiles_in[par], kGdnTilesBytes);
+            bulk_load(&sh.tiles[par], in.tiles + static_cast<long long>(x_first + c) * p.v_heads + hv, kGdnTilesBytes, &sh.tiles_in[par]);
+        }
+        // no copy may be in flight when the block ends
+        for (int c = max(kq_loads - kKqSlots, 0); c < kq_loads; ++c)
+            mbar_wait_bounded(&sh.kq_in[c % kKqSlots], (c / kKqSlots) & 1, kDrainNs, nullptr);
+        for (int c = max(pair_loads - 2, 0); c < pair_loads; ++c) {
+            mbar_wait_bounded(&sh.v_in[c & 1], (c >> 1) & 1, kDrainNs, nullptr);
+            mbar_wait_bounded(&sh.tiles_in[c & 1], (c >> 1) & 1, kDrainNs, nullptr);
         }
     }
     tc_fence_before();
     __syncthreads();
     if (tid == 0 && sh.abort) atomicOr(&g_mixer_status, sh.abort);
-    if (warp == 12) {
+    if (warp == 8) {
         tmem_relinquish();
         tmem_dealloc(tm, 512);
     }
 }
 
 constexpr size_t gdn_chunk_smem() { return sizeof(GdnShared) + 1024; }
-static_assert(gdn_chunk_smem() <= 227 * 1024, "shared memory of one block");
+constexpr size_t gdn_tiles_smem() { return sizeof(GdnTilesShared) + 1024; }
+static_assert(gdn_chunk_smem() <= 227 * 1024 && 4 * (gdn_tiles_smem() + 1024) <= 228 * 1024, "shared memory of one SM");
 
 }  // namespace reax

@@ -20,13 +20,19 @@ constexpr int kGridYz = 65535;
 
 bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
 
-template <typename... P>
+// (`dependent`: the kernel may start while the one before it on the stream still runs, and waits for its end itself)
+template <bool dependent = false, typename... P>
 int launch(const char* what, void (*kernel)(P...), dim3 grid, int threads, size_t smem, void* stream, const P&... p) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(threads, 1, 1);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = static_cast<cudaStream_t>(stream);
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = dependent ? 1 : 0;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p...);
     return e == cudaSuccess ? REAX_OK : reax_abi::cuda_fail(e, what);
 }
@@ -71,19 +77,45 @@ int allow_smem(const void* kernel, std::atomic<bool> (&done)[kMaxDevices], size_
 // The bound of device-side waits for kernels that keep it in 32 bits (at most 4 s).
 uint32_t wait_ns() { return static_cast<uint32_t>(std::min(reax_abi::wait_timeout_ns(), 4000000000ull)); }
 
+// Chunks that `rows` rows of `batch` sequences can have at most, and how many of them one launch takes (the scratch memory of
+// a launch is kept to about 1.5 GB; longer batches take several).
+long long gdn_most_chunks(int rows, int batch) { return static_cast<long long>(rows) / reax::kChunk + std::min(rows, batch); }
+size_t gdn_chunk_bytes(int k_heads, int v_heads, int Dk) {
+    return static_cast<size_t>(v_heads) * sizeof(reax::GdnTiles) + static_cast<size_t>(k_heads) * (Dk / 64) * 16384;
+}
+long long gdn_slab(int rows, int batch, int k_heads, int v_heads, int Dk) {
+    const long long cap = static_cast<long long>((1536ull << 20) / gdn_chunk_bytes(k_heads, v_heads, Dk));
+    return std::min(gdn_most_chunks(rows, batch), std::max(cap, 16ll));
+}
+
 template <int DK, int DV>
-int gdn_chunks(const char* who, const reax::GdnParams& p, void* stream) {
-    static std::atomic<bool> done[kMaxDevices];
+int gdn_chunks(const char* who, const reax::GdnParams& p, void* workspace, int sms, void* stream) {
+    static std::atomic<bool> done[kMaxDevices], tiles_done[kMaxDevices];
     int rc = allow_smem(reinterpret_cast<const void*>(reax::gdn_chunk_kernel<DK, DV>), done, reax::gdn_chunk_smem());
+    if (rc == REAX_OK) rc = allow_smem(reinterpret_cast<const void*>(reax::gdn_tiles_kernel<DK>), tiles_done, reax::gdn_tiles_smem());
     reax::GdnMaps maps;
-    if (rc == REAX_OK) rc = reax_abi::encode_rows(&maps.q, p.q, p.k_heads * DK, p.rows, p.ldq, 64, reax::kChunk, true);
-    if (rc == REAX_OK) rc = reax_abi::encode_rows(&maps.k, p.k, p.k_heads * DK, p.rows, p.ldk, 64, reax::kChunk, true);
     if (rc == REAX_OK) rc = reax_abi::encode_rows(&maps.v, p.v, p.v_heads * DV, p.rows, p.ldv, DV, reax::kChunk, false);
     if (rc == REAX_OK)
         rc = reax_abi::encode_rows(&maps.out, p.out, p.v_heads * DV, p.rows, static_cast<long long>(p.v_heads) * DV, 32, 32, false);
-    if (rc != REAX_OK) return rc;
-    return launch(who, reax::gdn_chunk_kernel<DK, DV>, dim3(p.v_heads, p.batch), reax::kChunkThreads, reax::gdn_chunk_smem(),
-                  stream, p, maps, wait_ns());
+    const long long most = gdn_most_chunks(p.rows, p.batch), slab = gdn_slab(p.rows, p.batch, p.k_heads, p.v_heads, DK);
+    reax::GdnScratch scratch;
+    scratch.tiles = static_cast<reax::GdnTiles*>(workspace);
+    scratch.kq = static_cast<uint8_t*>(workspace) + static_cast<size_t>(slab) * p.v_heads * sizeof(reax::GdnTiles);
+    for (long long x = 0; x < most && rc == REAX_OK; x += slab) {
+        scratch.x0 = static_cast<int>(x);
+        scratch.chunks = static_cast<int>(std::min(slab, most - x));
+        // A block takes the value heads of a key head one after the other, which saves their common products; where all blocks
+        // find room at once, four to an SM, more blocks of fewer heads are the shorter way.
+        const int group = p.v_heads / p.k_heads;
+        const int parts = static_cast<int>(std::clamp(4ll * sms / (static_cast<long long>(scratch.chunks) * p.k_heads), 1ll, static_cast<long long>(group)));
+        scratch.heads = (group + parts - 1) / parts;
+        rc = launch(who, reax::gdn_tiles_kernel<DK>, dim3(scratch.chunks, p.k_heads, (group + scratch.heads - 1) / scratch.heads), reax::kTilesThreads,
+                    reax::gdn_tiles_smem(), stream, p, scratch, wait_ns());
+        if (rc == REAX_OK)
+            rc = launch<true>(who, reax::gdn_chunk_kernel<DK, DV>, dim3(p.v_heads, p.batch), reax::kChunkThreads, reax::gdn_chunk_smem(), stream, p,
+                        maps, scratch, wait_ns());
+    }
+    return rc;
 }
 
 int check_cache(const char* who, const reax::Kv8Cache& c) {
@@ -153,10 +185,15 @@ int attend_step(const char* who, const reax::Kv8Attend& a, void* workspace, int 
 
 extern "C" {
 
+size_t reax_gdn_workspace_bytes(int rows, int batch, int k_heads, int v_heads, int Dk) {
+    if (rows <= 0 || batch <= 0 || k_heads <= 0 || v_heads <= 0 || (Dk != 64 && Dk != 128)) return 0;
+    return static_cast<size_t>(gdn_slab(rows, batch, k_heads, v_heads, Dk)) * gdn_chunk_bytes(k_heads, v_heads, Dk);
+}
+
 int reax_gdn_prefill(const void* q, const void* k, const void* v, const float* g, const float* beta, float* state,
                      const int32_t* cu_seqlens, const int32_t* slots, void* out, int rows, int batch, int k_heads,
                      int v_heads, int Dk, int Dv, int n_slots, long long ldq, long long ldk, long long ldv, float scale,
-                     int normalize, int carry, void* stream) {
+                     int normalize, int carry, void* workspace, size_t workspace_bytes, void* stream) {
     using bf16 = __nv_bfloat16;
     const reax::GdnParams p = {static_cast<const bf16*>(q), static_cast<const bf16*>(k), static_cast<const bf16*>(v), g,
                                beta, state, cu_seqlens, slots, static_cast<bf16*>(out), ldq, ldk, ldv, rows, batch, k_heads,
@@ -166,7 +203,11 @@ int reax_gdn_prefill(const void* q, const void* k, const void* v, const float* g
     if (!cu_seqlens && batch != 1)
         return fail(REAX_ERR_INVALID, "reax_gdn_prefill: %d sequences need cu_seqlens", batch);
     if ((rc = reax_abi::current_sms(&sms)) != REAX_OK) return rc;
-#define X(K, V) gdn_chunks<K, V>("reax_gdn_prefill", p, stream)
+    const size_t need = reax_gdn_workspace_bytes(rows, batch, k_heads, v_heads, Dk);
+    if (!workspace || workspace_bytes < need)
+        return fail(REAX_ERR_WORKSPACE, "reax_gdn_prefill: workspace of %zu bytes, needs reax_gdn_workspace_bytes() = %zu", workspace_bytes, need);
+    if (!aligned(workspace, 128)) return fail(REAX_ERR_ALIGN, "reax_gdn_prefill: the workspace must be 128-byte aligned");
+#define X(K, V) gdn_chunks<K, V>("reax_gdn_prefill", p, workspace, sms, stream)
     return REAX_GDN_DISPATCH(Dk, Dv, X);
 #undef X
 }

@@ -13,7 +13,7 @@ def prefill(**kw):
     a = dict(rows=0, batch=1, hk=2, hv=4, dk=128, dv=128, slots=1, ldq=256, ldk=256, ldv=512)
     a.update(kw)
     return lib().reax_gdn_prefill(*[None] * 9, a["rows"], a["batch"], a["hk"], a["hv"], a["dk"], a["dv"], a["slots"], a["ldq"],
-                                  a["ldk"], a["ldv"], 1.0, 1, 1, None)
+                                  a["ldk"], a["ldv"], 1.0, 1, 1, None, 0, None)
 
 
 def test_gated_delta_entry_refuses():
