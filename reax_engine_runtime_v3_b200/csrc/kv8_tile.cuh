@@ -32,6 +32,8 @@ constexpr int kAttendTileThreads = 16 * 32;
 constexpr int kConverters = 6;                // warps
 constexpr uint32_t kTmO = 0, kTmQ = 256, kTmScore = 384, kTmWeight = 448;
 
+constexpr int kTileSeqs = 256;                // sequences counted at a time
+
 struct Kv8Maps {
     CUtensorMap k, v;                         // rows of D bytes, boxes of min(D, 128) bytes by 16 rows
 };
@@ -41,6 +43,7 @@ struct TileShared {
     uint8_t k[2][kTileCols * D * 2], v[2][kTileCols * D * 2];   // [D / 64][64 rows][64 values], 128-byte swizzle
     uint8_t codes[2][2][kTileCols * D];       // of k and v as they come, two tiles: 16 rows after 16 rows
     float xch[2][8][32];
+    long long units[kTileSeqs];               // tiles of the sequences, for one cached head
     uint64_t in[2][2], in_free[2][2], k_full[2], v_full[2], k_free[2], v_free[2], s_full, s_free, p_full, pv_done, drained;
     uint32_t tmem;
     uint32_t abort;
@@ -60,52 +63,131 @@ REAX_DEVI uint32_t codes_bf162(uint32_t x) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// What the blocks leave for the join: the item that block i begins and others go on with, and the parts of both ends of each
+// block's stretch (0: of an item that it goes on with, 1: of one that it begins and does not end).
+struct TileRest {
+    int lo, first, live, h, parts;            // parts: blocks that have one (0: no such item)
+};
+struct TileWork {
+    TileRest* rest;                           // [blocks]
+    float* stats;                             // [blocks][2][2][kTileRows]: reference and denominator
+    float* sums;                              // [blocks][2][D][kTileRows]
+};
+
+struct TileSeq {
+    int lo, rows, len, before, items;         // `before`: rows that its first query row sees, less one
+    TileSeq() = default;
+    REAX_DEVI TileSeq(const Kv8Attend& a, int b) {
+        int hi;
+        kv8_span(a.cu, b, a.rows, &lo, &hi);
+        rows = hi - lo;
+        const int all = max(a.lengths[b], 0);
+        len = min(all, a.table_ld * a.c.page);
+        before = all - rows;
+        items = (rows * a.group + kTileRows - 1) / kTileRows;
+    }
+    // Rows that see nothing take one tile too (a masked one).
+    REAX_DEVI int tiles(const Kv8Attend& a, int item) const {
+        const int last = min((item + 1) * kTileRows, rows * a.group) - 1;
+        return max((min(len, before + last / a.group + 1) + kTileCols - 1) / kTileCols, 1);
+    }
+};
+
+// A place on the line of tiles: of the cached heads one after the other, in each of the items of the sequences.
+struct TileCursor {
+    long long u;
+    int h, b, item, x, tiles;
+    TileSeq s;
+    // Go on with the item at u (past `to - x` tiles), which is on the line.
+    REAX_DEVI void next(const Kv8Attend& a) {
+        x = 0;
+        if (++item >= s.items) {
+            item = 0;
+            do {
+                if (++b == a.batch) b = 0, ++h;
+                s = TileSeq(a, b);
+            } while (s.items == 0);
+        }
+        tiles = s.tiles(a, item);
+    }
+};
+
+REAX_DEVI long long warp_sum_ll(long long v) {
+#pragma unroll
+    for (int m = 16; m > 0; m >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, m);
+    return v;
+}
+// Takes from `rest` what lies before the first lane whose running sum of `n` exceeds it, and gives that lane, or -1.
+REAX_DEVI int warp_find(long long n, long long* rest, int lane) {
+    long long upto = n;
+#pragma unroll
+    for (int m = 1; m < 32; m <<= 1) {
+        const long long t = __shfl_up_sync(0xFFFFFFFFu, upto, m);
+        if (lane >= m) upto += t;
+    }
+    const unsigned who = __ballot_sync(0xFFFFFFFFu, upto > *rest);
+    const int l = who ? __ffs(who) - 1 : 31;
+    *rest -= __shfl_sync(0xFFFFFFFFu, who ? upto - n : upto, l);
+    return who ? l : -1;
+}
+
 template <int D>
 __global__ void __launch_bounds__(kAttendTileThreads, 1)
-    kv8_tile_kernel(const __grid_constant__ Kv8Attend a, const __grid_constant__ Kv8Maps maps, uint32_t limit_ns) {
+    kv8_tile_kernel(const __grid_constant__ Kv8Attend a, const __grid_constant__ Kv8Maps maps, const TileWork work, uint32_t limit_ns) {
     extern __shared__ uint8_t tile_smem[];
     TileShared<D>& sh = *reinterpret_cast<TileShared<D>*>(tile_smem + (-smem_u32(tile_smem) & 1023u));
     const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32, quarter = warp % 4;
-    const int heads = a.c.heads, page = a.c.page, shift = __ffs(page) - 1, h = blockIdx.y;
-    // the sequence and the 128 rows of block x: items of the sequences one after the other
-    int b = -1, item = 0;
-    for (int b0 = 0, before = 0; b0 < a.batch; b0 += 32) {
-        int n = 0;
-        if (b0 + lane < a.batch) {
-            int lo, hi;
-            kv8_span(a.cu, b0 + lane, a.rows, &lo, &hi);
-            n = ((hi - lo) * a.group + kTileRows - 1) / kTileRows;
+    const int heads = a.c.heads, page = a.c.page, shift = __ffs(page) - 1;
+    asm volatile("griddepcontrol.launch_dependents;");        // (the join, which waits for the end of this grid)
+    // this block's stretch [u0, u1) of the line, and where it begins
+    long long u0 = 0, u1 = 0, all = 0;
+    int blocks = 0;
+    TileCursor start;
+    {
+        auto count = [&](int b0) {
+            __syncthreads();
+            for (int b = b0 + warp; b < min(a.batch, b0 + kTileSeqs); b += kAttendTileThreads / 32) {
+                const TileSeq s(a, b);
+                long long n = 0;
+                for (int i = lane; i < s.items; i += 32) n += s.tiles(a, i);
+                n = warp_sum_ll(n);
+                if (lane == 0) sh.units[b - b0] = n;
+            }
+            __syncthreads();
+        };
+        long long head = 0;
+        for (int b0 = 0; b0 < a.batch; b0 += kTileSeqs) {
+            count(b0);
+            long long n = 0;
+            for (int i = lane; i < min(a.batch - b0, kTileSeqs); i += 32) n += sh.units[i];
+            head += warp_sum_ll(n);
         }
-        int upto = n;
-#pragma unroll
-        for (int m = 1; m < 32; m <<= 1) {
-            const int t = __shfl_up_sync(0xFFFFFFFFu, upto, m);
-            if (lane >= m) upto += t;
+        all = head * heads;
+        blocks = static_cast<int>(min(static_cast<long long>(gridDim.x), all));
+        if (tid == 0) work.rest[blockIdx.x].parts = 0;
+        if (static_cast<int>(blockIdx.x) >= blocks) return;
+        u0 = all * blockIdx.x / blocks, u1 = all * (blockIdx.x + 1) / blocks;
+        start.u = u0;
+        start.h = static_cast<int>(u0 / head);
+        long long rest = u0 - start.h * head;
+        int b = -1;
+        for (int b0 = 0; b < 0; b0 += kTileSeqs) {
+            if (a.batch > kTileSeqs) count(b0);
+            for (int i = 0; i < min(a.batch - b0, kTileSeqs) && b < 0; i += 32) {
+                const int l = warp_find(b0 + i + lane < a.batch && i + lane < kTileSeqs ? sh.units[i + lane] : 0, &rest, lane);
+                if (l >= 0) b = b0 + i + l;
+            }
         }
-        const unsigned who = __ballot_sync(0xFFFFFFFFu, before + upto > static_cast<int>(blockIdx.x));
-        if (who) {
-            const int l = __ffs(who) - 1;
-            b = b0 + l;
-            item = static_cast<int>(blockIdx.x) - before - __shfl_sync(0xFFFFFFFFu, upto - n, l);
-            break;
+        start.b = b;
+        start.s = TileSeq(a, b);
+        int item = -1;
+        for (int i = 0; item < 0; i += 32) {
+            const int l = warp_find(i + lane < start.s.items ? start.s.tiles(a, i + lane) : 0, &rest, lane);
+            if (l >= 0) item = i + l;
         }
-        before += __shfl_sync(0xFFFFFFFFu, upto, 31);
-    }
-    if (b < 0) return;
-    const StepSeq seq(a, b);
-    const int first = item * kTileRows, live = min(kTileRows, seq.rows * a.group - first);
-    // the last row sees the most
-    const int most = min(seq.len, a.lengths[b] - seq.rows + (first + live - 1) / a.group + 1);
-    const int tiles = most > 0 ? (most + kTileCols - 1) / kTileCols : 0;
-    const int32_t* table = a.tables + static_cast<long long>(b) * a.table_ld;
-    if (tiles == 0) {                         // rows that see nothing
-        for (int e = tid; e < live * (D / 8); e += kAttendTileThreads) {
-            const int r = first + e / (D / 8);
-            const long long row = (static_cast<long long>(seq.lo) + r / a.group) * heads * a.group + h * a.group + r % a.group;
-            *reinterpret_cast<uint4*>(a.out + row * D + e % (D / 8) * 8) = uint4{};
-            if (a.lse && e % (D / 8) == 0) a.lse[row] = -INFINITY;
-        }
-        return;
+        start.item = item;
+        start.x = static_cast<int>(rest);
+        start.tiles = start.s.tiles(a, item);
     }
 
     if (warp == 12) tmem_alloc(&sh.tmem, 512);
@@ -133,7 +215,6 @@ __global__ void __launch_bounds__(kAttendTileThreads, 1)
     if (warp < 8) {
         // ------------------------------------------------------------------------------------------------- softmax
         const int half = warp / 4, r = quarter * 32 + lane;
-        float scale = a.scale * 1.44269504f;
         int turn = 0;
         auto row_max = [&](float m) {
             float* x = &sh.xch[turn][quarter * 2][lane];
@@ -142,186 +223,227 @@ __global__ void __launch_bounds__(kAttendTileThreads, 1)
             turn ^= 1;
             return fmaxf(x[0], x[32]);
         };
-        {
-            // q's row, half of it, into TMEM: two values a column, scaled to a largest in [2^13, 2^14)
-            const int i = first + min(r, live - 1);
-            const __nv_bfloat16* src = a.q + (static_cast<long long>(seq.lo) + i / a.group) * a.ldq + (h * a.group + i % a.group) * D + half * (D / 2);
-            uint32_t top = 0;
+        int t0 = 0;                           // tiles so far
+#pragma unroll 1
+        for (TileCursor at = start;;) {
+            const TileSeq& seq = at.s;
+            const int first = at.item * kTileRows, live = min(kTileRows, seq.rows * a.group - first);
+            const int to = static_cast<int>(min(static_cast<long long>(at.tiles), at.x + (u1 - at.u)));
+            const int32_t* table = a.tables + static_cast<long long>(at.b) * a.table_ld;
+            float scale = a.scale * 1.44269504f;
+            {
+                // q's row, half of it, into TMEM: two values a column, scaled to a largest in [2^13, 2^14)
+                const int i = first + min(r, live - 1);
+                const __nv_bfloat16* src = a.q + (static_cast<long long>(seq.lo) + i / a.group) * a.ldq + (at.h * a.group + i % a.group) * D + half * (D / 2);
+                uint32_t top = 0;
 #pragma unroll 4
-            for (int e = 0; e < D / 2; e += 8) {
-                const uint4 y = *reinterpret_cast<const uint4*>(src + e);
-                top = __vmaxu2(__vmaxu2(top, y.x & 0x7FFF7FFFu), __vmaxu2(y.y & 0x7FFF7FFFu, __vmaxu2(y.z & 0x7FFF7FFFu, y.w & 0x7FFF7FFFu)));
-            }
-            const float2 f = scale_of(row_max(__uint_as_float(max(top & 0xFFFFu, top >> 16) << 16)));
-            scale *= f.y;
-#pragma unroll 1
-            for (int e = 0; e < D / 2; e += 32) {
-                uint32_t w[16];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const uint4 y = *reinterpret_cast<const uint4*>(src + e + j * 8);
-                    w[4 * j] = half2_of(mul2_rn(bf16x2_to_f2(y.x), f2(f.x, f.x))), w[4 * j + 1] = half2_of(mul2_rn(bf16x2_to_f2(y.y), f2(f.x, f.x)));
-                    w[4 * j + 2] = half2_of(mul2_rn(bf16x2_to_f2(y.z), f2(f.x, f.x))), w[4 * j + 3] = half2_of(mul2_rn(bf16x2_to_f2(y.w), f2(f.x, f.x)));
+                for (int e = 0; e < D / 2; e += 8) {
+                    const uint4 y = *reinterpret_cast<const uint4*>(src + e);
+                    top = __vmaxu2(__vmaxu2(top, y.x & 0x7FFF7FFFu), __vmaxu2(y.y & 0x7FFF7FFFu, __vmaxu2(y.z & 0x7FFF7FFFu, y.w & 0x7FFF7FFFu)));
                 }
-                tmem_st_x16(lanes + kTmQ + half * (D / 4) + e / 2, w);
-            }
-            tmem_wait_st();
-            tc_fence_before();
-            arrive(&sh.s_free);
-        }
-        const int seen = r < live ? min(seq.len, a.lengths[b] - seq.rows + (first + r) / a.group + 1) : 0;
-        const int least = min(seq.len, a.lengths[b] - seq.rows + first / a.group + 1);     // what the first row sees
-        float ref = -INFINITY, den = 0.0f;
-        // scales of this half's two runs of 16 rows: pages looked up two tiles ahead, scales fetched one ahead
-        int id[2];
-        float ks[2], vs[2];
-        bool in[2];
-        auto look_up = [&](int x) {
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int row = x * kTileCols + half * 32 + e * 16;
-                id[e] = x < tiles && row < seq.len ? table[row >> shift] : -1;
-            }
-        };
-        auto fetch = [&]() {
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                in[e] = id[e] >= 0 && id[e] < a.c.pages;
-                const long long at = static_cast<long long>(in[e] ? id[e] : 0) * heads + h;
-                ks[e] = in[e] ? a.c.k_scale[at] : 0.0f;
-                vs[e] = in[e] ? fmaxf(a.c.v_scale[at], 1e-30f) : 1.0f;
-            }
-        };
-        look_up(0);
-        fetch();
-        look_up(1);
+                const float2 f = scale_of(row_max(__uint_as_float(max(top & 0xFFFFu, top >> 16) << 16)));
+                scale *= f.y;
 #pragma unroll 1
-        for (int x = 0; x < tiles; ++x) {
-            const float f[2] = {ks[0] * scale, ks[1] * scale}, inv[2] = {__fdividef(1.0f, vs[0]), __fdividef(1.0f, vs[1])}, add[2] = {lg2f(vs[0]), lg2f(vs[1])};
-            const bool plain = in[0] && in[1] && x * kTileCols + half * 32 + 32 <= least;
-            const bool have[2] = {in[0], in[1]};
-            fetch();
-            look_up(x + 2);
-            wait(&sh.s_full, x & 1, kStatusTimeoutAccFull);
-            tc_fence_after();
-            uint32_t c[32];
-            tmem_ld_x32_sync(lanes + kTmScore + half * 32, c);
-            tc_fence_before();
-            arrive(&sh.s_free);
-            float t[32], m = -INFINITY;
+                for (int e = 0; e < D / 2; e += 32) {
+                    uint32_t w[16];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) t[i] = fmaf(__uint_as_float(c[i]), f[i / 16], add[i / 16]);
-            if (!plain) {
-                const int col = x * kTileCols + half * 32;
-#pragma unroll
-                for (int i = 0; i < 32; ++i) t[i] = col + i < seen && have[i / 16] ? t[i] : -INFINITY;
-            }
-#pragma unroll
-            for (int i = 0; i < 32; i += 2) m = fmaxf(m, fmaxf(t[i], t[i + 1]));
-            m = row_max(m);
-            // a new reference where the maximum is well above the old one; O is scaled then
-            const bool move = m > ref + 8.0f;           // (true from -inf)
-            if (__any_sync(0xFFFFFFFFu, move)) {
-                const float to = move ? m : ref, g = ref == -INFINITY ? 0.0f : ex2(ref - to);
-                if (x > 0) {
-                    wait(&sh.pv_done, (x - 1) & 1, kStatusTimeoutAccFull);
-                    tc_fence_after();
-#pragma unroll 1
-                    for (int e = half * (D / 2); e < (half + 1) * (D / 2); e += 16) {
-                        uint32_t o[16];
-                        tmem_ld_x16_sync(lanes + kTmO + e, o);
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * g);
-                        tmem_st_x16(lanes + kTmO + e, o);
+                    for (int j = 0; j < 4; ++j) {
+                        const uint4 y = *reinterpret_cast<const uint4*>(src + e + j * 8);
+                        w[4 * j] = half2_of(mul2_rn(bf16x2_to_f2(y.x), f2(f.x, f.x))), w[4 * j + 1] = half2_of(mul2_rn(bf16x2_to_f2(y.y), f2(f.x, f.x)));
+                        w[4 * j + 2] = half2_of(mul2_rn(bf16x2_to_f2(y.z), f2(f.x, f.x))), w[4 * j + 3] = half2_of(mul2_rn(bf16x2_to_f2(y.w), f2(f.x, f.x)));
                     }
-                    tmem_wait_st();
+                    tmem_st_x16(lanes + kTmQ + half * (D / 4) + e / 2, w);
                 }
-                den *= g;
-                ref = to;
+                tmem_wait_st();
+                tc_fence_before();
+                arrive(&sh.s_free);
             }
-            const float base = ref == -INFINITY ? 0.0f : ref;
-            float sum[2] = {};
+            const int seen = r < live ? min(seq.len, seq.before + (first + r) / a.group + 1) : 0;
+            const int least = min(seq.len, seq.before + first / a.group + 1);     // what the first row sees
+            float ref = -INFINITY, den = 0.0f;
+            // scales of this half's two runs of 16 rows: pages looked up two tiles ahead, scales fetched one ahead
+            int id[2];
+            float ks[2], vs[2];
+            bool in[2];
+            auto look_up = [&](int x) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-                t[i] = ex2(t[i] - base);
-                sum[i / 16] += t[i];
-            }
-            den += sum[0] * inv[0] + sum[1] * inv[1];
-            // P's place is free once O has taken the tile before
-            if (x > 0) wait(&sh.pv_done, (x - 1) & 1, kStatusTimeoutAccFull);
-            tc_fence_after();
-#pragma unroll
-            for (int e = 0; e < 32; e += 16) {
-                uint32_t hi[8], lo[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    // upper halves, and upper halves of what they leave
-                    const uint32_t y0 = __float_as_uint(t[e + 2 * i]), y1 = __float_as_uint(t[e + 2 * i + 1]);
-                    hi[i] = __byte_perm(y0, y1, 0x7632);
-                    const uint64_t rest = sub2_rn(u2(y0, y1), u2(y0 & 0xFFFF0000u, y1 & 0xFFFF0000u));
-                    lo[i] = __byte_perm(static_cast<uint32_t>(rest), static_cast<uint32_t>(rest >> 32), 0x7632);
+                for (int e = 0; e < 2; ++e) {
+                    const int row = x * kTileCols + half * 32 + e * 16;
+                    id[e] = x < to && row < seq.len ? table[row >> shift] : -1;
                 }
-                tmem_st_x8(lanes + kTmWeight + half * 16 + e / 2, hi);
-                tmem_st_x8(lanes + kTmWeight + 32 + half * 16 + e / 2, lo);
-            }
-            tmem_wait_st();
-            tc_fence_before();
-            arrive(&sh.p_full);
-        }
-        // out
-        sh.xch[turn][quarter * 2 + half][lane] = den;
-        named_bar_sync(1 + quarter, 64);
-        den = sh.xch[turn][quarter * 2][lane] + sh.xch[turn][quarter * 2 + 1][lane];
-        wait(&sh.pv_done, (tiles - 1) & 1, kStatusTimeoutAccFull);
-        tc_fence_after();
-        const float scale_out = den > 0.0f ? 1.0f / den : 0.0f;
-        const int i = first + r;
-        const long long row = (static_cast<long long>(seq.lo) + i / a.group) * heads * a.group + h * a.group + i % a.group;
+            };
+            auto fetch = [&]() {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    in[e] = id[e] >= 0 && id[e] < a.c.pages;
+                    const long long scales = static_cast<long long>(in[e] ? id[e] : 0) * heads + at.h;
+                    ks[e] = in[e] ? a.c.k_scale[scales] : 0.0f;
+                    vs[e] = in[e] ? fmaxf(a.c.v_scale[scales], 1e-30f) : 1.0f;
+                }
+            };
+            look_up(at.x);
+            fetch();
+            look_up(at.x + 1);
 #pragma unroll 1
-        for (int e = half * (D / 2); e < (half + 1) * (D / 2); e += 16) {
-            uint32_t o[16], w[8];
-            tmem_ld_x16_sync(lanes + kTmO + e, o);
+            for (int x = at.x; x < to; ++x, ++t0) {
+                const float f[2] = {ks[0] * scale, ks[1] * scale}, inv[2] = {__fdividef(1.0f, vs[0]), __fdividef(1.0f, vs[1])}, add[2] = {lg2f(vs[0]), lg2f(vs[1])};
+                const bool plain = in[0] && in[1] && x * kTileCols + half * 32 + 32 <= least;
+                const bool have[2] = {in[0], in[1]};
+                fetch();
+                look_up(x + 2);
+                wait(&sh.s_full, t0 & 1, kStatusTimeoutAccFull);
+                tc_fence_after();
+                uint32_t c[32];
+                tmem_ld_x32_sync(lanes + kTmScore + half * 32, c);
+                tc_fence_before();
+                if (x + 1 < to) arrive(&sh.s_free);
+                float t[32], m = -INFINITY;
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                w[j] = bf16x2_rn(f2(__uint_as_float(o[2 * j]) * scale_out, __uint_as_float(o[2 * j + 1]) * scale_out));
-            if (r < live) {
-                *reinterpret_cast<uint4*>(a.out + row * D + e) = uint4{w[0], w[1], w[2], w[3]};
-                *reinterpret_cast<uint4*>(a.out + row * D + e + 8) = uint4{w[4], w[5], w[6], w[7]};
+                for (int i = 0; i < 32; ++i) t[i] = fmaf(__uint_as_float(c[i]), f[i / 16], add[i / 16]);
+                if (!plain) {
+                    const int col = x * kTileCols + half * 32;
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) t[i] = col + i < seen && have[i / 16] ? t[i] : -INFINITY;
+                }
+#pragma unroll
+                for (int i = 0; i < 32; i += 2) m = fmaxf(m, fmaxf(t[i], t[i + 1]));
+                m = row_max(m);
+                // a new reference where the maximum is well above the old one; O is scaled then
+                const bool move = m > ref + 8.0f;           // (true from -inf)
+                if (__any_sync(0xFFFFFFFFu, move)) {
+                    const float to = move ? m : ref, g = ref == -INFINITY ? 0.0f : ex2(ref - to);
+                    if (x > at.x) {
+                        wait(&sh.pv_done, (t0 - 1) & 1, kStatusTimeoutAccFull);
+                        tc_fence_after();
+#pragma unroll 1
+                        for (int e = half * (D / 2); e < (half + 1) * (D / 2); e += 16) {
+                            uint32_t o[16];
+                            tmem_ld_x16_sync(lanes + kTmO + e, o);
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * g);
+                            tmem_st_x16(lanes + kTmO + e, o);
+                        }
+                        tmem_wait_st();
+                    }
+                    den *= g;
+                    ref = to;
+                }
+                const float base = ref == -INFINITY ? 0.0f : ref;
+                float sum[2] = {};
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    t[i] = ex2(t[i] - base);
+                    sum[i / 16] += t[i];
+                }
+                den += sum[0] * inv[0] + sum[1] * inv[1];
+                // P's place is free once O has taken the tile before
+                if (x > at.x) wait(&sh.pv_done, (t0 - 1) & 1, kStatusTimeoutAccFull);
+                tc_fence_after();
+#pragma unroll
+                for (int e = 0; e < 32; e += 16) {
+                    uint32_t hi[8], lo[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        // upper halves, and upper halves of what they leave
+                        const uint32_t y0 = __float_as_uint(t[e + 2 * i]), y1 = __float_as_uint(t[e + 2 * i + 1]);
+                        hi[i] = __byte_perm(y0, y1, 0x7632);
+                        const uint64_t rest = sub2_rn(u2(y0, y1), u2(y0 & 0xFFFF0000u, y1 & 0xFFFF0000u));
+                        lo[i] = __byte_perm(static_cast<uint32_t>(rest), static_cast<uint32_t>(rest >> 32), 0x7632);
+                    }
+                    tmem_st_x8(lanes + kTmWeight + half * 16 + e / 2, hi);
+                    tmem_st_x8(lanes + kTmWeight + 32 + half * 16 + e / 2, lo);
+                }
+                tmem_wait_st();
+                tc_fence_before();
+                arrive(&sh.p_full);
             }
+            // out
+            sh.xch[turn][quarter * 2 + half][lane] = den;
+            named_bar_sync(1 + quarter, 64);
+            den = sh.xch[turn][quarter * 2][lane] + sh.xch[turn][quarter * 2 + 1][lane];
+            turn ^= 1;
+            wait(&sh.pv_done, (t0 - 1) & 1, kStatusTimeoutAccFull);
+            tc_fence_after();
+            if (at.x > 0 || to < at.tiles) {
+                // a part: columns of 128 rows
+                const long long place = 2 * static_cast<long long>(blockIdx.x) + (at.x == 0);
+                float* sums = work.sums + place * D * kTileRows + r;
+#pragma unroll 1
+                for (int e = half * (D / 2); e < (half + 1) * (D / 2); e += 16) {
+                    uint32_t o[16];
+                    tmem_ld_x16_sync(lanes + kTmO + e, o);
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) sums[(e + j) * kTileRows] = __uint_as_float(o[j]);
+                }
+                if (half == 0) work.stats[place * 2 * kTileRows + r] = ref, work.stats[(place * 2 + 1) * kTileRows + r] = den;
+                if (tid == 0 && at.x == 0) {
+                    // the last block that has a part of it
+                    const long long last = at.u + at.tiles;
+                    work.rest[blockIdx.x] = {seq.lo, first, live, at.h, static_cast<int>((last * blocks - 1) / all) - static_cast<int>(blockIdx.x) + 1};
+                }
+            } else {
+                const float scale_out = den > 0.0f ? 1.0f / den : 0.0f;
+                const int i = first + r;
+                const long long row = (static_cast<long long>(seq.lo) + i / a.group) * heads * a.group + at.h * a.group + i % a.group;
+#pragma unroll 1
+                for (int e = half * (D / 2); e < (half + 1) * (D / 2); e += 16) {
+                    uint32_t o[16], w[8];
+                    tmem_ld_x16_sync(lanes + kTmO + e, o);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        w[j] = bf16x2_rn(f2(__uint_as_float(o[2 * j]) * scale_out, __uint_as_float(o[2 * j + 1]) * scale_out));
+                    if (r < live) {
+                        *reinterpret_cast<uint4*>(a.out + row * D + e) = uint4{w[0], w[1], w[2], w[3]};
+                        *reinterpret_cast<uint4*>(a.out + row * D + e + 8) = uint4{w[4], w[5], w[6], w[7]};
+                    }
+                }
+                if (a.lse && half == 0 && r < live) a.lse[row] = den > 0.0f ? 0.69314718f * (ref + log2f(den)) : -INFINITY;
+            }
+            at.u += to - at.x;
+            if (at.u >= u1) break;
+            at.next(a);
         }
-        if (a.lse && half == 0 && r < live) a.lse[row] = den > 0.0f ? 0.69314718f * (ref + log2f(den)) : -INFINITY;
     } else if (warp == 12) {
         // ---------------------------------------------------------------------------------------------------- MMAs
         if (lane == 0) {
             constexpr uint32_t id_s = idesc_f16_f32(128, kTileCols, false), id_o = idesc_bf16_ts(128, D, true);
+            int t0 = 0;                       // tiles before the item
 #pragma unroll 1
-            for (int x = 0; x <= tiles; ++x) {
-                if (x < tiles) {
-                    const int buf = x & 1;
-                    const uint64_t kd = sw128_kmajor_desc(smem_u32(sh.k[buf]));
-                    wait(&sh.k_full[buf], (x >> 1) & 1, kStatusTimeoutFull);
-                    wait(&sh.s_free, x & 1, kStatusTimeoutAccEmpty);       // (first: q is there)
-                    if (wait.dead) break;
-                    tc_fence_after();
+            for (TileCursor at = start; !wait.dead;) {
+                const int tiles = static_cast<int>(min(static_cast<long long>(at.tiles - at.x), u1 - at.u));
 #pragma unroll 1
-                    for (int ks = 0; ks < D / 16; ++ks)
-                        umma_f16_ts(tm + kTmScore, tm + kTmQ + ks * 8, kd + (ks / 4) * (kTileCols * 8) + (ks % 4) * 2, id_s, ks > 0);
-                    umma_commit(&sh.s_full);
-                    umma_commit(&sh.k_free[buf]);
+                for (int x = 0; x <= tiles; ++x) {
+                    if (x < tiles) {
+                        const int t = t0 + x, buf = t & 1;
+                        const uint64_t kd = sw128_kmajor_desc(smem_u32(sh.k[buf]));
+                        wait(&sh.k_full[buf], (t >> 1) & 1, kStatusTimeoutFull);
+                        wait(&sh.s_free, t & 1, kStatusTimeoutAccEmpty);       // (an item's first: q is there)
+                        if (wait.dead) break;
+                        tc_fence_after();
+#pragma unroll 1
+                        for (int ks = 0; ks < D / 16; ++ks)
+                            umma_f16_ts(tm + kTmScore, tm + kTmQ + ks * 8, kd + (ks / 4) * (kTileCols * 8) + (ks % 4) * 2, id_s, ks > 0);
+                        umma_commit(&sh.s_full);
+                        umma_commit(&sh.k_free[buf]);
+                    }
+                    if (x > 0) {
+                        const int t = t0 + x - 1, buf = t & 1;
+                        const uint64_t vd = sw128_mn_desc(smem_u32(sh.v[buf]), kTileCols * 128);
+                        wait(&sh.v_full[buf], (t >> 1) & 1, kStatusTimeoutFull);
+                        wait(&sh.p_full, t & 1, kStatusTimeoutEmpty);
+                        if (wait.dead) break;
+                        tc_fence_after();
+#pragma unroll 1
+                        for (int e = 0; e < 8; ++e)
+                            umma_f16_ts(tm + kTmO, tm + kTmWeight + (e / 4) * 32 + (e % 4) * 8, vd + (e % 4) * 128, id_o, x > 1 || e > 0);
+                        umma_commit(&sh.pv_done);
+                        umma_commit(&sh.v_free[buf]);
+                    }
                 }
-                if (x > 0) {
-                    const int y = x - 1, buf = y & 1;
-                    const uint64_t vd = sw128_mn_desc(smem_u32(sh.v[buf]), kTileCols * 128);
-                    wait(&sh.v_full[buf], (y >> 1) & 1, kStatusTimeoutFull);
-                    wait(&sh.p_full, y & 1, kStatusTimeoutEmpty);
-                    if (wait.dead) break;
-                    tc_fence_after();
-#pragma unroll 1
-                    for (int e = 0; e < 8; ++e)
-                        umma_f16_ts(tm + kTmO, tm + kTmWeight + (e / 4) * 32 + (e % 4) * 8, vd + (e % 4) * 128, id_o, y > 0 || e > 0);
-                    umma_commit(&sh.pv_done);
-                    umma_commit(&sh.v_free[buf]);
-                }
+                t0 += tiles;
+                at.u += tiles;
+                if (at.u >= u1) break;
+                at.next(a);
             }
             drain_mmas(&sh.drained);
         }
@@ -330,19 +452,20 @@ __global__ void __launch_bounds__(kAttendTileThreads, 1)
         // --------------------------------------------------------------------------------------------------- loads
         const uint64_t policy = l2_policy_evict_normal();
         int id = -1, loads[2] = {};
-        auto look_up = [&](int x) {           // lane l < 4: rows 16 l .. of the tile
-            const int row = x * kTileCols + lane * 16;
-            id = x < tiles && lane < 4 && row < seq.len ? table[row >> shift] : -1;
+        TileCursor at = start;
+        auto look_up = [&]() {                // lane l < 4: rows 16 l .. of the tile
+            const int row = at.x * kTileCols + lane * 16;
+            id = lane < 4 && row < at.s.len ? a.tables[static_cast<long long>(at.b) * a.table_ld + (row >> shift)] : -1;
         };
-        look_up(0);
+        look_up();
 #pragma unroll 1
-        for (int x = 0; x < tiles; ++x) {
+        for (int t = 0, n = static_cast<int>(u1 - u0); t < n; ++t) {
             const bool in = id >= 0 && id < a.c.pages;
-            const int at = (id * heads + h) * page + ((x * kTileCols + lane * 16) & (page - 1)), buf = x & 1;
+            const int from = (id * heads + at.h) * page + ((at.x * kTileCols + lane * 16) & (page - 1)), buf = t & 1;
             const uint32_t have = __popc(__ballot_sync(0xFFFFFFFFu, in));
 #pragma unroll 1
             for (int e = 0; e < 2; ++e) {     // k, then v
-                if (x > 1) wait(&sh.in_free[buf][e], ((x >> 1) - 1) & 1, kStatusTimeoutEmpty);
+                if (t > 1) wait(&sh.in_free[buf][e], ((t >> 1) - 1) & 1, kStatusTimeoutEmpty);
                 wait.dead = __any_sync(0xFFFFFFFFu, wait.dead);
                 if (lane == 0 && !wait.dead) {
                     fence_proxy_async_smem();
@@ -353,10 +476,13 @@ __global__ void __launch_bounds__(kAttendTileThreads, 1)
                 if (in && !wait.dead)
 #pragma unroll
                     for (int d = 0; d < D; d += 128)
-                        tma_load_2d(sh.codes[buf][e] + lane * 16 * D + d * 16, e ? &maps.v : &maps.k, &sh.in[buf][e], d, at, policy);
+                        tma_load_2d(sh.codes[buf][e] + lane * 16 * D + d * 16, e ? &maps.v : &maps.k, &sh.in[buf][e], d, from, policy);
                 __syncwarp();
             }
-            look_up(x + 1);
+            if (t + 1 < n) {
+                if (++at.x == at.tiles) at.next(a);
+                look_up();
+            }
         }
         // no copy may be in flight when the block ends
         if (lane == 0)
@@ -371,13 +497,13 @@ __global__ void __launch_bounds__(kAttendTileThreads, 1)
         const int from = D == 64 ? step_at<64>(lane % 8, lane / 8 * 16) : (lane % 8) * 128 + ((lane / 8) ^ (lane % 8)) * 16;
         const int into = (lane % 8) * 128 + ((lane / 8 * 2) ^ (lane % 8)) * 16;
 #pragma unroll 1
-        for (int x = 0; x < tiles; ++x) {
-            const int buf = x & 1;
+        for (int t = 0, n = static_cast<int>(u1 - u0); t < n; ++t) {
+            const int buf = t & 1;
 #pragma unroll 1
             for (int e = 0; e < 2; ++e) {
-                wait(&sh.in[buf][e], (x >> 1) & 1, kStatusTimeoutFull);
+                wait(&sh.in[buf][e], (t >> 1) & 1, kStatusTimeoutFull);
                 // K's place is free once the scores of the tile before last are there, V's once O has taken it
-                if (x > 1) wait(e ? &sh.v_free[buf] : &sh.k_free[buf], ((x >> 1) - 1) & 1, kStatusTimeoutEmpty);
+                if (t > 1) wait(e ? &sh.v_free[buf] : &sh.k_free[buf], ((t >> 1) - 1) & 1, kStatusTimeoutEmpty);
                 uint8_t* to = e ? sh.v[buf] : sh.k[buf];
                 // 8 rows by 4 pieces of 16 codes a warp and turn
                 auto convert = [&](auto pair) {
@@ -426,6 +552,83 @@ __global__ void __launch_bounds__(kAttendTileThreads, 1)
     if (warp == 12) {
         tmem_relinquish();
         tmem_dealloc(tm, 512);
+    }
+}
+
+// The join of items that blocks share.  A unit of it is 32 rows of some columns; 2, 4 or 8 warps (by the number of parts, so
+// that neither a few long items nor many short ones leave warps without work) take the parts in turn for 16 columns, and
+// their sums are added in the warps' order.
+constexpr int kJoinThreads = 8 * 32, kJoinBlocksPerSm = 4, kJoinCols = 16, kMostTileBlocks = 256;
+template <int D>
+__global__ void __launch_bounds__(kJoinThreads) kv8_join_kernel(const __grid_constant__ Kv8Attend a, const TileWork work, int blocks) {
+    __shared__ int upto[kMostTileBlocks];                     // units of the blocks' items, added up
+    __shared__ float xch[8][2 + kJoinCols][32];
+    const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
+    auto ways_of = [](int parts) { return parts > 4 ? 8 : parts > 2 ? 4 : 2; };
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (warp == 0) {
+        int before = 0;
+        for (int i = lane; i - lane < blocks; i += 32) {
+            const int parts = i < blocks ? work.rest[i].parts : 0;
+            int n = parts ? (work.rest[i].live + 31) / 32 * (D / kJoinCols / (8 / ways_of(parts))) : 0;
+#pragma unroll
+            for (int m = 1; m < 32; m <<= 1) {
+                const int t = __shfl_up_sync(0xFFFFFFFFu, n, m);
+                if (lane >= m) n += t;
+            }
+            if (i < blocks) upto[i] = before + n;
+            before += __shfl_sync(0xFFFFFFFFu, n, 31);
+        }
+    }
+    __syncthreads();
+    const int units = upto[blocks - 1];
+#pragma unroll 1
+    for (int u = blockIdx.x; u < units; u += gridDim.x) {
+        int i = 0;                                            // the first with upto[i] > u
+#pragma unroll
+        for (int m = kMostTileBlocks / 2; m > 0; m >>= 1)
+            if (i + m <= blocks && upto[i + m - 1] <= u) i += m;
+        const TileRest rest = work.rest[i];
+        const int ways = ways_of(rest.parts), across = D / kJoinCols / (8 / ways), slice = warp % ways;
+        const int unit = u - (i ? upto[i - 1] : 0), r = unit / across * 32 + lane;
+        const int col = (unit % across * (8 / ways) + warp / ways) * kJoinCols;
+        float top = -INFINITY, den = 0.0f, o[kJoinCols] = {};
+#pragma unroll 2
+        for (int p = slice; p < rest.parts; p += ways) {
+            const long long place = 2 * (static_cast<long long>(i) + p) + (p == 0);
+            const float ref = work.stats[place * 2 * kTileRows + r], d = work.stats[(place * 2 + 1) * kTileRows + r];
+            float y[kJoinCols];
+#pragma unroll
+            for (int e = 0; e < kJoinCols; ++e) y[e] = work.sums[(place * D + col + e) * kTileRows + r];
+            const float m = fmaxf(top, ref), base = m == -INFINITY ? 0.0f : m, f0 = ex2f(top - base), f1 = ex2f(ref - base);
+            top = m;
+            den = den * f0 + d * f1;
+#pragma unroll
+            for (int e = 0; e < kJoinCols; ++e) o[e] = o[e] * f0 + y[e] * f1;
+        }
+        __syncthreads();                                      // the unit before has been read
+        xch[warp][0][lane] = top, xch[warp][1][lane] = den;
+#pragma unroll
+        for (int e = 0; e < kJoinCols; ++e) xch[warp][2 + e][lane] = o[e];
+        __syncthreads();
+        if (slice > 0 || r >= rest.live) continue;
+        for (int w = 1; w < ways; ++w) {
+            const float ref = xch[warp + w][0][lane], m = fmaxf(top, ref), base = m == -INFINITY ? 0.0f : m;
+            const float f0 = ex2f(top - base), f1 = ex2f(ref - base);
+            top = m;
+            den = den * f0 + xch[warp + w][1][lane] * f1;
+#pragma unroll
+            for (int e = 0; e < kJoinCols; ++e) o[e] = o[e] * f0 + xch[warp + w][2 + e][lane] * f1;
+        }
+        const float scale = den > 0.0f ? 1.0f / den : 0.0f;
+        const int y = rest.first + r;
+        const long long row = (static_cast<long long>(rest.lo) + y / a.group) * a.c.heads * a.group + rest.h * a.group + y % a.group;
+        uint32_t w[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = bf16x2_rn(f2(o[2 * e] * scale, o[2 * e + 1] * scale));
+        *reinterpret_cast<uint4*>(a.out + row * D + col) = uint4{w[0], w[1], w[2], w[3]};
+        *reinterpret_cast<uint4*>(a.out + row * D + col + 8) = uint4{w[4], w[5], w[6], w[7]};
+        if (a.lse && col == 0) a.lse[row] = den > 0.0f ? 0.69314718f * (top + log2f(den)) : -INFINITY;
     }
 }
 

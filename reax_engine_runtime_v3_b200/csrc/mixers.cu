@@ -2,6 +2,7 @@
 // (declarations and contracts: include/reax_b200.h).  As in abi.cu, nothing here allocates or synchronizes.
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 #include <utility>
 
 #include "abi_shared.h"
@@ -140,18 +141,28 @@ int check_rows(const char* who, const int32_t* tables, const int32_t* lengths, c
 }
 
 // Workspace of the attention: counters (zero between calls), then the parts of items that blocks share.
-struct StepWorkspace {
-    reax::StepWork work;
+struct AttendWorkspace {
+    reax::StepWork step;
+    reax::TileWork tile;
     size_t bytes;
-    StepWorkspace(void* base, int sms) {
-        const size_t blocks = static_cast<size_t>(sms) * reax::kStepBlocksPerSm;
-        const size_t counters = (blocks * sizeof(int) + 255) / 256 * 256;
-        const size_t stats = blocks * 2 * 2 * reax::kStepRows * sizeof(float);
+    AttendWorkspace(void* base, int sms) {
         char* p = static_cast<char*>(base);
-        work.counters = reinterpret_cast<int*>(p);
-        work.stats = reinterpret_cast<float*>(p + counters);
-        work.parts = reinterpret_cast<float*>(p + counters + stats);
-        bytes = counters + stats + blocks * 2 * reax::kStepRows * 256 * sizeof(float);
+        size_t at = 0;
+        auto take = [&](auto*& to, size_t n) {
+            to = reinterpret_cast<std::remove_reference_t<decltype(to)>>(p + at);
+            at += (n * sizeof(*to) + 255) / 256 * 256;
+        };
+        const size_t blocks = static_cast<size_t>(sms) * reax::kStepBlocksPerSm;
+        take(step.counters, blocks);
+        const size_t shared = at;
+        take(step.stats, blocks * 2 * 2 * reax::kStepRows);
+        take(step.parts, blocks * 2 * reax::kStepRows * 256);
+        bytes = at;
+        at = shared;
+        take(tile.rest, sms);
+        take(tile.stats, static_cast<size_t>(sms) * 2 * 2 * reax::kTileRows);
+        take(tile.sums, static_cast<size_t>(sms) * 2 * reax::kTileRows * 256);
+        bytes = std::max(bytes, at);
     }
 };
 
@@ -159,16 +170,17 @@ struct StepWorkspace {
 constexpr int kStepMostRows = 32;
 
 template <int D>
-int attend_tiles(const char* who, const reax::Kv8Attend& a, const reax::Kv8Maps& maps, void* stream) {
+int attend_tiles(const char* who, const reax::Kv8Attend& a, const reax::Kv8Maps& maps, void* workspace, int sms, void* stream) {
     static std::atomic<bool> done[kMaxDevices];
     constexpr size_t smem = sizeof(reax::TileShared<D>) + 1024;
     static_assert(smem <= 227 * 1024, "shared memory of one block");
-    const int rc = allow_smem(reinterpret_cast<const void*>(reax::kv8_tile_kernel<D>), done, smem);
+    int rc = allow_smem(reinterpret_cast<const void*>(reax::kv8_tile_kernel<D>), done, smem);
     if (rc != REAX_OK) return rc;
-    // the most items that any split of the rows over the batch gives
-    const long long items = static_cast<long long>(a.rows) * a.group / reax::kTileRows + std::min(a.rows, a.batch);
-    return launch(who, reax::kv8_tile_kernel<D>, dim3(static_cast<unsigned>(items), a.c.heads), reax::kAttendTileThreads, smem, stream, a,
-                  maps, wait_ns());
+    const reax::TileWork work = AttendWorkspace(workspace, sms).tile;
+    const int blocks = std::min(sms, reax::kMostTileBlocks);
+    rc = launch(who, reax::kv8_tile_kernel<D>, dim3(blocks), reax::kAttendTileThreads, smem, stream, a, maps, work, wait_ns());
+    if (rc != REAX_OK) return rc;
+    return launch<true>(who, reax::kv8_join_kernel<D>, dim3(sms * reax::kJoinBlocksPerSm), reax::kJoinThreads, 0, stream, a, work, blocks);
 }
 
 template <int D>
@@ -178,7 +190,7 @@ int attend_step(const char* who, const reax::Kv8Attend& a, void* workspace, int 
     const int rc = allow_smem(reinterpret_cast<const void*>(reax::kv8_step_kernel<D>), done, smem);
     if (rc != REAX_OK) return rc;
     return launch(who, reax::kv8_step_kernel<D>, dim3(sms * reax::kStepBlocksPerSm), reax::kAttendStepThreads, smem, stream, a,
-                  StepWorkspace(workspace, sms).work);
+                  AttendWorkspace(workspace, sms).step);
 }
 
 }  // namespace
@@ -281,7 +293,7 @@ int reax_kv8_read(const int8_t* k_codes, const int8_t* v_codes, const float* k_s
 
 size_t reax_kv8_workspace_bytes(int device) {
     const int sms = reax_abi::device_sms(device);
-    return sms < 0 ? 0 : StepWorkspace(nullptr, sms).bytes;
+    return sms < 0 ? 0 : AttendWorkspace(nullptr, sms).bytes;
 }
 
 int reax_kv8_attend(const void* q, const int8_t* k_codes, const int8_t* v_codes, const float* k_scales,
@@ -303,9 +315,9 @@ int reax_kv8_attend(const void* q, const int8_t* k_codes, const int8_t* v_codes,
     if (!aligned(q, 16) || !aligned(out, 16) || ldq % 8)
         return fail(REAX_ERR_ALIGN, "%s: q and out must be 16-byte aligned, the row stride a multiple of 8", who);
     if ((rc = reax_abi::current_sms(&sms)) != REAX_OK) return rc;
-    if (!workspace || workspace_bytes < StepWorkspace(nullptr, sms).bytes)
+    if (!workspace || workspace_bytes < AttendWorkspace(nullptr, sms).bytes)
         return fail(REAX_ERR_WORKSPACE, "%s: workspace of %zu bytes, needs reax_kv8_workspace_bytes() = %zu", who, workspace_bytes,
-                    StepWorkspace(nullptr, sms).bytes);
+                    AttendWorkspace(nullptr, sms).bytes);
     if (!aligned(workspace, 256)) return fail(REAX_ERR_ALIGN, "%s: the workspace must be 256-byte aligned", who);
     if (static_cast<long long>(max_rows) * group > kStepMostRows) {
         const long long pool = static_cast<long long>(pages) * heads * page;
@@ -313,9 +325,9 @@ int reax_kv8_attend(const void* q, const int8_t* k_codes, const int8_t* v_codes,
         reax::Kv8Maps maps;
         if ((rc = reax_abi::encode_codes(&maps.k, k_codes, dim, std::max(pool, 16ll), 16)) != REAX_OK) return rc;
         if ((rc = reax_abi::encode_codes(&maps.v, v_codes, dim, std::max(pool, 16ll), 16)) != REAX_OK) return rc;
-        if (dim == 64) return attend_tiles<64>(who, a, maps, stream);
-        if (dim == 128) return attend_tiles<128>(who, a, maps, stream);
-        return attend_tiles<256>(who, a, maps, stream);
+        if (dim == 64) return attend_tiles<64>(who, a, maps, workspace, sms, stream);
+        if (dim == 128) return attend_tiles<128>(who, a, maps, workspace, sms, stream);
+        return attend_tiles<256>(who, a, maps, workspace, sms, stream);
     }
     if (dim == 64) return attend_step<64>(who, a, workspace, sms, stream);
     if (dim == 128) return attend_step<128>(who, a, workspace, sms, stream);
