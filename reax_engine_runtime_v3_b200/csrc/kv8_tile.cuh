@@ -491,8 +491,8 @@ __global__ void __launch_bounds__(kAttendTileThreads, 1)
         __syncwarp();
     } else {
         // ------------------------------------------------------------------------------------------- codes to bf16
-        // each scheduler gets a quarter of the work: warps 8 and 9 that of one, 10 and 14, 11 and 15 share that of one
-        const int begin = warp - 8, step = warp < 10 ? 4 : 8;
+        const int begin = warp < 12 ? warp - 8 : warp - 10;
+        constexpr int step = kConverters;
         // this lane's place in 8 rows of 64 codes as they come, and in the tile
         const int from = D == 64 ? step_at<64>(lane % 8, lane / 8 * 16) : (lane % 8) * 128 + ((lane / 8) ^ (lane % 8)) * 16;
         const int into = (lane % 8) * 128 + ((lane / 8 * 2) ^ (lane % 8)) * 16;
@@ -508,20 +508,19 @@ __global__ void __launch_bounds__(kAttendTileThreads, 1)
                 // 8 rows by 4 pieces of 16 codes a warp and turn
                 auto convert = [&](auto pair) {
                     // (the loads first: the compiler must not move one over a store that it cannot tell apart)
-                    constexpr int kAll = (kTileCols / 8) * (D / 64);
-#pragma unroll 1
-                    for (int u0 = begin; u0 < kAll; u0 += 4 * step) {
-                        uint4 y[4];
+                    constexpr int kAll = (kTileCols / 8) * (D / 64), kEach = (kAll + step - 1) / step;
+                    {
+                        uint4 y[kEach];
 #pragma unroll
-                        for (int n = 0; n < 4; ++n) {
-                            const int u = min(u0 + n * step, kAll - 1), rb = u / (D / 64), pb = u % (D / 64);
+                        for (int n = 0; n < kEach; ++n) {
+                            const int u = min(begin + n * step, kAll - 1), rb = u / (D / 64), pb = u % (D / 64);
                             y[n] = *reinterpret_cast<const uint4*>(
                                 D == 64 ? sh.codes[buf][e] + rb * 512 + from
                                         : sh.codes[buf][e] + (rb / 2) * (16 * D) + (rb % 2) * 1024 + (pb / 2) * 2048 + (from ^ (pb % 2 * 64)));
                         }
 #pragma unroll
-                        for (int n = 0; n < 4; ++n) {
-                            const int u = u0 + n * step, rb = u / (D / 64), pb = u % (D / 64);
+                        for (int n = 0; n < kEach; ++n) {
+                            const int u = begin + n * step, rb = u / (D / 64), pb = u % (D / 64);
                             if (u >= kAll) break;
                             uint8_t* row = to + pb * (kTileCols * 128) + rb * 1024;
                             uint32_t w[8];
