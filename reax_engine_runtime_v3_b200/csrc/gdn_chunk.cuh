@@ -865,7 +865,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) gdn_chunk_kernel(const __gri
                 if (wait.dead) break;
                 tc_fence_after();
                 // descriptor addresses count in units of 16 bytes
-#pragma unroll 4
+#pragma unroll
                 for (int e = 0; e < 2 * (DK / 16); ++e) {
                     const int ks = e % (DK / 16);
                     umma_f16_ts(tm + kTmXk, tm + kTmS + (e / (DK / 16)) * 64 + ks * 8, kq + (ks / 4) * 1024 + (ks % 4) * 2, id64, e > 0);
@@ -875,14 +875,14 @@ __global__ void __launch_bounds__(kChunkThreads, 1) gdn_chunk_kernel(const __gri
                 if (c > 0) wait(&sh.tiles_free[par ^ 1], ((c - 1) >> 1) & 1, kStatusTimeoutEmpty);
                 if (wait.dead) break;
                 tc_fence_after();
-#pragma unroll 4
+#pragma unroll
                 for (int ks = 0; ks < DK / 16; ++ks)
                     umma_f16_ts(tm + kTmXq, tm + kTmS + ks * 8, kq + 512 + (ks / 4) * 1024 + (ks % 4) * 2, id64, ks > 0);
                 wait(&sh.tiles_in[par], (c >> 1) & 1, kStatusTimeoutFull);
                 wait(&sh.r_ready, par, kStatusTimeoutEmpty);
                 if (wait.dead) break;
                 tc_fence_after();
-#pragma unroll 4
+#pragma unroll
                 for (int e = 0; e < 12; ++e) {
                     const int ks = e % 4, term = e / 4;      // hi hi, lo hi, hi lo
                     umma_f16_ts(tm + kTmV, tm + kTmR + (term == 1 ? 32 : 0) + ks * 8, (term == 2 ? tlo : thi) + ks * 2, id64, e > 0);
@@ -891,12 +891,12 @@ __global__ void __launch_bounds__(kChunkThreads, 1) gdn_chunk_kernel(const __gri
                 wait(&sh.v_ready, par, kStatusTimeoutEmpty);
                 if (wait.dead) break;
                 tc_fence_after();
-#pragma unroll 4
+#pragma unroll
                 for (int e = 0; e < 8; ++e)
                     umma_f16_ts(tm + kTmS, tm + kTmXk + (e / 4) * 32 + (e % 4) * 8, kmn + (e % 4) * 128, id_d, e > 0);
                 umma_commit(&sh.d_done);
                 umma_commit(&sh.kq_free[slot_k]);
-#pragma unroll 4
+#pragma unroll
                 for (int ks = 0; ks < 4; ++ks) umma_f16_ts(tm + kTmY, tm + kTmR + ks * 8, pd + ks * 2, id64, ks > 0);
                 umma_commit(&sh.y_done);
             }

@@ -420,7 +420,7 @@ __global__ void __launch_bounds__(kAttendTileThreads, 1)
                         wait(&sh.s_free, t & 1, kStatusTimeoutAccEmpty);       // (an item's first: q is there)
                         if (wait.dead) break;
                         tc_fence_after();
-#pragma unroll 1
+#pragma unroll
                         for (int ks = 0; ks < D / 16; ++ks)
                             umma_f16_ts(tm + kTmScore, tm + kTmQ + ks * 8, kd + (ks / 4) * (kTileCols * 8) + (ks % 4) * 2, id_s, ks > 0);
                         umma_commit(&sh.s_full);
@@ -433,7 +433,7 @@ __global__ void __launch_bounds__(kAttendTileThreads, 1)
                         wait(&sh.p_full, t & 1, kStatusTimeoutEmpty);
                         if (wait.dead) break;
                         tc_fence_after();
-#pragma unroll 1
+#pragma unroll
                         for (int e = 0; e < 8; ++e)
                             umma_f16_ts(tm + kTmO, tm + kTmWeight + (e / 4) * 32 + (e % 4) * 8, vd + (e % 4) * 128, id_o, x > 1 || e > 0);
                         umma_commit(&sh.pv_done);
