@@ -17,7 +17,9 @@
 // Scaling O (in TMEM) costs as much as a tile, so the reference that the exponents are taken from moves only when a maximum
 // exceeds it by 8 (in log2): weights stay below 2^8, which bf16 holds as well as any.
 //
-// Roles (16 warps): 0-7 softmax (thread = row and half of the columns), 8-11 and 14-15 codes to 16 bits, 12 MMAs, 13 loads.
+// Roles (17 warps): 0-7 softmax (thread = row and half of the columns), 8 loads, 12 MMAs of the scores, 16 those of O, the
+// others codes to 16 bits.  Waiting for and issuing both sorts of MMA takes one warp longer than the MMAs take (332 us for 2048
+// rows of four prompts, MEASURED with two); the two, and the loads, share a scheduler with softmax warps alone.
 #pragma once
 
 #include "common.cuh"
@@ -28,7 +30,7 @@
 namespace reax {
 
 constexpr int kTileRows = 128, kTileCols = 64;
-constexpr int kAttendTileThreads = 16 * 32;
+constexpr int kAttendTileThreads = 17 * 32;
 constexpr int kConverters = 6;                // warps
 constexpr uint32_t kTmO = 0, kTmQ = 256, kTmScore = 384, kTmWeight = 448;
 
@@ -44,7 +46,7 @@ struct TileShared {
     uint8_t codes[2][2][kTileCols * D];       // of k and v as they come, two tiles: 16 rows after 16 rows
     float xch[2][8][32];
     long long units[kTileSeqs];               // tiles of the sequences, for one cached head
-    uint64_t in[2][2], in_free[2][2], k_full[2], v_full[2], k_free[2], v_free[2], s_full, s_free, p_full, pv_done, drained;
+    uint64_t in[2][2], in_free[2][2], k_full[2], v_full[2], k_free[2], v_free[2], s_full, s_free, p_full, pv_done, drained[2];
     uint32_t tmem;
     uint32_t abort;
 };
@@ -54,13 +56,15 @@ __host__ __device__ constexpr uint32_t idesc_bf16_ts(int M, int N, bool b_mn) {
     return idesc_bf16_f32(M, N) | (b_mn ? 1u << 16 : 0u);
 }
 
-// Two codes (bytes of x picked by SEL into 16-bit lanes) as bf16: 128 + (c & 127) less 128 or 256.
+// Two codes (as bytes c + 128 of x, picked by SEL into 16-bit lanes) as bf16 times 2^-6: the bits c + 128 are (c + 128) 2^-133
+// there, subnormal or not, so that one multiplication by 2^127 and a subtraction give them, exactly.
+constexpr float kCodeUp = 64.0f;
 template <uint32_t SEL>
 REAX_DEVI uint32_t codes_bf162(uint32_t x) {
     const uint32_t y = __byte_perm(x, 0u, SEL);
-    const uint32_t a = (y & 0x007F007Fu) | 0x43004300u, b = (y & 0x00800080u) | 0x43004300u;
-    const __nv_bfloat162 h = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
-    return *reinterpret_cast<const uint32_t*>(&h);
+    uint32_t z;
+    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(z) : "r"(y), "r"(0x7F007F00u), "r"(0xC000C000u));
+    return z;
 }
 
 // What the blocks leave for the join: the item that block i begins and others go on with, and the parts of both ends of each
@@ -197,7 +201,7 @@ __global__ void __launch_bounds__(kAttendTileThreads, 1)
             mbar_init(&sh.k_full[i], kConverters), mbar_init(&sh.v_full[i], kConverters);
             mbar_init(&sh.k_free[i], 1), mbar_init(&sh.v_free[i], 1);
         }
-        mbar_init(&sh.s_full, 1), mbar_init(&sh.s_free, 8), mbar_init(&sh.p_full, 8), mbar_init(&sh.pv_done, 1), mbar_init(&sh.drained, 1);
+        mbar_init(&sh.s_full, 1), mbar_init(&sh.s_free, 8), mbar_init(&sh.p_full, 8), mbar_init(&sh.pv_done, 1), mbar_init(&sh.drained[0], 1), mbar_init(&sh.drained[1], 1);
         sh.abort = 0;
         fence_mbar_init();
     }
@@ -382,7 +386,7 @@ __global__ void __launch_bounds__(kAttendTileThreads, 1)
                     work.rest[blockIdx.x] = {seq.lo, first, live, at.h, static_cast<int>((last * blocks - 1) / all) - static_cast<int>(blockIdx.x) + 1};
                 }
             } else {
-                const float scale_out = den > 0.0f ? 1.0f / den : 0.0f;
+                const float scale_out = den > 0.0f ? kCodeUp / den : 0.0f;
                 const int i = first + r;
                 const long long row = (static_cast<long long>(seq.lo) + i / a.group) * heads * a.group + at.h * a.group + i % a.group;
 #pragma unroll 1
@@ -404,51 +408,51 @@ __global__ void __launch_bounds__(kAttendTileThreads, 1)
             at.next(a);
         }
     } else if (warp == 12) {
-        // ---------------------------------------------------------------------------------------------------- MMAs
+        // ---------------------------------------------------------------------------------------- MMAs of the scores
         if (lane == 0) {
-            constexpr uint32_t id_s = idesc_f16_f32(128, kTileCols, false), id_o = idesc_bf16_ts(128, D, true);
-            int t0 = 0;                       // tiles before the item
+            constexpr uint32_t id_s = idesc_f16_f32(128, kTileCols, false);
 #pragma unroll 1
-            for (TileCursor at = start; !wait.dead;) {
-                const int tiles = static_cast<int>(min(static_cast<long long>(at.tiles - at.x), u1 - at.u));
-#pragma unroll 1
-                for (int x = 0; x <= tiles; ++x) {
-                    if (x < tiles) {
-                        const int t = t0 + x, buf = t & 1;
-                        const uint64_t kd = sw128_kmajor_desc(smem_u32(sh.k[buf]));
-                        wait(&sh.k_full[buf], (t >> 1) & 1, kStatusTimeoutFull);
-                        wait(&sh.s_free, t & 1, kStatusTimeoutAccEmpty);       // (an item's first: q is there)
-                        if (wait.dead) break;
-                        tc_fence_after();
+            for (int t = 0, n = static_cast<int>(u1 - u0); t < n; ++t) {
+                const int buf = t & 1;
+                const uint64_t kd = sw128_kmajor_desc(smem_u32(sh.k[buf]));
+                wait(&sh.k_full[buf], (t >> 1) & 1, kStatusTimeoutFull);
+                wait(&sh.s_free, t & 1, kStatusTimeoutAccEmpty);       // (an item's first: q is there)
+                if (wait.dead) break;
+                tc_fence_after();
 #pragma unroll
-                        for (int ks = 0; ks < D / 16; ++ks)
-                            umma_f16_ts(tm + kTmScore, tm + kTmQ + ks * 8, kd + (ks / 4) * (kTileCols * 8) + (ks % 4) * 2, id_s, ks > 0);
-                        umma_commit(&sh.s_full);
-                        umma_commit(&sh.k_free[buf]);
-                    }
-                    if (x > 0) {
-                        const int t = t0 + x - 1, buf = t & 1;
-                        const uint64_t vd = sw128_mn_desc(smem_u32(sh.v[buf]), kTileCols * 128);
-                        wait(&sh.v_full[buf], (t >> 1) & 1, kStatusTimeoutFull);
-                        wait(&sh.p_full, t & 1, kStatusTimeoutEmpty);
-                        if (wait.dead) break;
-                        tc_fence_after();
-#pragma unroll
-                        for (int e = 0; e < 8; ++e)
-                            umma_f16_ts(tm + kTmO, tm + kTmWeight + (e / 4) * 32 + (e % 4) * 8, vd + (e % 4) * 128, id_o, x > 1 || e > 0);
-                        umma_commit(&sh.pv_done);
-                        umma_commit(&sh.v_free[buf]);
-                    }
-                }
-                t0 += tiles;
-                at.u += tiles;
-                if (at.u >= u1) break;
-                at.next(a);
+                for (int ks = 0; ks < D / 16; ++ks)
+                    umma_f16_ts(tm + kTmScore, tm + kTmQ + ks * 8, kd + (ks / 4) * (kTileCols * 8) + (ks % 4) * 2, id_s, ks > 0);
+                umma_commit(&sh.s_full);
+                umma_commit(&sh.k_free[buf]);
             }
-            drain_mmas(&sh.drained);
+            drain_mmas(&sh.drained[0]);
         }
         __syncwarp();
-    } else if (warp == 13) {
+    } else if (warp == 16) {
+        // ----------------------------------------------------------------------------------------------- MMAs of O
+        if (lane == 0) {
+            constexpr uint32_t id_o = idesc_bf16_ts(128, D, true);
+            TileCursor at = start;
+#pragma unroll 1
+            for (int t = 0, n = static_cast<int>(u1 - u0); t < n; ++t) {
+                const int buf = t & 1;
+                const uint64_t vd = sw128_mn_desc(smem_u32(sh.v[buf]), kTileCols * 128);
+                const bool more = t > 0 && at.x > 0;          // (not an item's first tile, nor this block's)
+                wait(&sh.v_full[buf], (t >> 1) & 1, kStatusTimeoutFull);
+                wait(&sh.p_full, t & 1, kStatusTimeoutEmpty);
+                if (wait.dead) break;
+                tc_fence_after();
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    umma_f16_ts(tm + kTmO, tm + kTmWeight + (e / 4) * 32 + (e % 4) * 8, vd + (e % 4) * 128, id_o, more || e > 0);
+                umma_commit(&sh.pv_done);
+                umma_commit(&sh.v_free[buf]);
+                if (t + 1 < n && ++at.x == at.tiles) at.next(a);
+            }
+            drain_mmas(&sh.drained[1]);
+        }
+        __syncwarp();
+    } else if (warp == 8) {
         // --------------------------------------------------------------------------------------------------- loads
         const uint64_t policy = l2_policy_evict_normal();
         int id = -1, loads[2] = {};
@@ -491,7 +495,7 @@ __global__ void __launch_bounds__(kAttendTileThreads, 1)
         __syncwarp();
     } else {
         // ------------------------------------------------------------------------------------------- codes to bf16
-        const int begin = warp < 12 ? warp - 8 : warp - 10;
+        const int begin = warp < 12 ? warp - 9 : warp - 10;
         constexpr int step = kConverters;
         // this lane's place in 8 rows of 64 codes as they come, and in the tile
         const int from = D == 64 ? step_at<64>(lane % 8, lane / 8 * 16) : (lane % 8) * 128 + ((lane / 8) ^ (lane % 8)) * 16;
@@ -531,7 +535,9 @@ __global__ void __launch_bounds__(kAttendTileThreads, 1)
                     }
                 };
                 if (e)
-                    convert([](uint32_t x, uint32_t& lo, uint32_t& hi) { lo = codes_bf162<0x4140>(x), hi = codes_bf162<0x4342>(x); });
+                    convert([](uint32_t x, uint32_t& lo, uint32_t& hi) {
+                        lo = codes_bf162<0x4140>(x ^ 0x80808080u), hi = codes_bf162<0x4342>(x ^ 0x80808080u);
+                    });
                 else
                     convert([](uint32_t x, uint32_t& lo, uint32_t& hi) {
                         lo = codes_half2<0x4140>(x ^ 0x80808080u), hi = codes_half2<0x4342>(x ^ 0x80808080u);
@@ -619,7 +625,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv8_join_kernel(const __grid_con
 #pragma unroll
             for (int e = 0; e < kJoinCols; ++e) o[e] = o[e] * f0 + xch[warp + w][2 + e][lane] * f1;
         }
-        const float scale = den > 0.0f ? 1.0f / den : 0.0f;
+        const float scale = den > 0.0f ? kCodeUp / den : 0.0f;
         const int y = rest.first + r;
         const long long row = (static_cast<long long>(rest.lo) + y / a.group) * a.c.heads * a.group + rest.h * a.group + y % a.group;
         uint32_t w[8];
