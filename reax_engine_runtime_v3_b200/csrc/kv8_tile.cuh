@@ -240,23 +240,24 @@ __global__ void __launch_bounds__(kAttendTileThreads, 1)
                 const int i = first + min(r, live - 1);
                 const __nv_bfloat16* src = a.q + (static_cast<long long>(seq.lo) + i / a.group) * a.ldq + (at.h * a.group + i % a.group) * D + half * (D / 2);
                 uint32_t top = 0;
-#pragma unroll 4
-                for (int e = 0; e < D / 2; e += 8) {
-                    const uint4 y = *reinterpret_cast<const uint4*>(src + e);
-                    top = __vmaxu2(__vmaxu2(top, y.x & 0x7FFF7FFFu), __vmaxu2(y.y & 0x7FFF7FFFu, __vmaxu2(y.z & 0x7FFF7FFFu, y.w & 0x7FFF7FFFu)));
-                }
+                uint4 y[D / 16];
+#pragma unroll
+                for (int e = 0; e < D / 16; ++e) y[e] = *reinterpret_cast<const uint4*>(src + e * 8);
+#pragma unroll
+                for (int e = 0; e < D / 16; ++e)
+                    top = __vmaxu2(__vmaxu2(top, y[e].x & 0x7FFF7FFFu), __vmaxu2(y[e].y & 0x7FFF7FFFu, __vmaxu2(y[e].z & 0x7FFF7FFFu, y[e].w & 0x7FFF7FFFu)));
                 const float2 f = scale_of(row_max(__uint_as_float(max(top & 0xFFFFu, top >> 16) << 16)));
                 scale *= f.y;
-#pragma unroll 1
-                for (int e = 0; e < D / 2; e += 32) {
+#pragma unroll
+                for (int e = 0; e < D / 16; e += 4) {
                     uint32_t w[16];
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        const uint4 y = *reinterpret_cast<const uint4*>(src + e + j * 8);
-                        w[4 * j] = half2_of(mul2_rn(bf16x2_to_f2(y.x), f2(f.x, f.x))), w[4 * j + 1] = half2_of(mul2_rn(bf16x2_to_f2(y.y), f2(f.x, f.x)));
-                        w[4 * j + 2] = half2_of(mul2_rn(bf16x2_to_f2(y.z), f2(f.x, f.x))), w[4 * j + 3] = half2_of(mul2_rn(bf16x2_to_f2(y.w), f2(f.x, f.x)));
+                        const uint4 z = y[e + j];
+                        w[4 * j] = half2_of(mul2_rn(bf16x2_to_f2(z.x), f2(f.x, f.x))), w[4 * j + 1] = half2_of(mul2_rn(bf16x2_to_f2(z.y), f2(f.x, f.x)));
+                        w[4 * j + 2] = half2_of(mul2_rn(bf16x2_to_f2(z.z), f2(f.x, f.x))), w[4 * j + 3] = half2_of(mul2_rn(bf16x2_to_f2(z.w), f2(f.x, f.x)));
                     }
-                    tmem_st_x16(lanes + kTmQ + half * (D / 4) + e / 2, w);
+                    tmem_st_x16(lanes + kTmQ + half * (D / 4) + e * 4, w);
                 }
                 tmem_wait_st();
                 tc_fence_before();
@@ -301,16 +302,18 @@ __global__ void __launch_bounds__(kAttendTileThreads, 1)
                 tmem_ld_x32_sync(lanes + kTmScore + half * 32, c);
                 tc_fence_before();
                 if (x + 1 < to) arrive(&sh.s_free);
-                float t[32], m = -INFINITY;
+                uint64_t t[16];
+                float m = -INFINITY;
 #pragma unroll
-                for (int i = 0; i < 32; ++i) t[i] = fmaf(__uint_as_float(c[i]), f[i / 16], add[i / 16]);
+                for (int i = 0; i < 16; ++i) t[i] = fma2_rn(u2(c[2 * i], c[2 * i + 1]), f2(f[i / 8], f[i / 8]), f2(add[i / 8], add[i / 8]));
                 if (!plain) {
                     const int col = x * kTileCols + half * 32;
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) t[i] = col + i < seen && have[i / 16] ? t[i] : -INFINITY;
+                    for (int i = 0; i < 16; ++i)
+                        t[i] = f2(col + 2 * i < seen && have[i / 8] ? f2_lo(t[i]) : -INFINITY, col + 2 * i + 1 < seen && have[i / 8] ? f2_hi(t[i]) : -INFINITY);
                 }
 #pragma unroll
-                for (int i = 0; i < 32; i += 2) m = fmaxf(m, fmaxf(t[i], t[i + 1]));
+                for (int i = 0; i < 16; ++i) m = fmaxf(m, fmaxf(f2_lo(t[i]), f2_hi(t[i])));
                 m = row_max(m);
                 // a new reference where the maximum is well above the old one; O is scaled then
                 const bool move = m > ref + 8.0f;           // (true from -inf)
@@ -333,13 +336,14 @@ __global__ void __launch_bounds__(kAttendTileThreads, 1)
                     ref = to;
                 }
                 const float base = ref == -INFINITY ? 0.0f : ref;
-                float sum[2] = {};
+                uint64_t sum[2] = {};
 #pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    t[i] = ex2(t[i] - base);
-                    sum[i / 16] += t[i];
+                for (int i = 0; i < 16; ++i) {
+                    const uint64_t y = sub2_rn(t[i], f2(base, base));
+                    t[i] = f2(ex2(f2_lo(y)), ex2(f2_hi(y)));
+                    sum[i / 8] = add2_rn(sum[i / 8], t[i]);
                 }
-                den += sum[0] * inv[0] + sum[1] * inv[1];
+                den += (f2_lo(sum[0]) + f2_hi(sum[0])) * inv[0] + (f2_lo(sum[1]) + f2_hi(sum[1])) * inv[1];
                 // P's place is free once O has taken the tile before
                 if (x > at.x) wait(&sh.pv_done, (t0 - 1) & 1, kStatusTimeoutAccFull);
                 tc_fence_after();
@@ -349,9 +353,9 @@ __global__ void __launch_bounds__(kAttendTileThreads, 1)
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         // upper halves, and upper halves of what they leave
-                        const uint32_t y0 = __float_as_uint(t[e + 2 * i]), y1 = __float_as_uint(t[e + 2 * i + 1]);
+                        const uint32_t y0 = static_cast<uint32_t>(t[e / 2 + i]), y1 = static_cast<uint32_t>(t[e / 2 + i] >> 32);
                         hi[i] = __byte_perm(y0, y1, 0x7632);
-                        const uint64_t rest = sub2_rn(u2(y0, y1), u2(y0 & 0xFFFF0000u, y1 & 0xFFFF0000u));
+                        const uint64_t rest = sub2_rn(t[e / 2 + i], u2(y0 & 0xFFFF0000u, y1 & 0xFFFF0000u));
                         lo[i] = __byte_perm(static_cast<uint32_t>(rest), static_cast<uint32_t>(rest >> 32), 0x7632);
                     }
                     tmem_st_x8(lanes + kTmWeight + half * 16 + e / 2, hi);
@@ -372,12 +376,12 @@ __global__ void __launch_bounds__(kAttendTileThreads, 1)
                 // a part: columns of 128 rows
                 const long long place = 2 * static_cast<long long>(blockIdx.x) + (at.x == 0);
                 float* sums = work.sums + place * D * kTileRows + r;
-#pragma unroll 1
-                for (int e = half * (D / 2); e < (half + 1) * (D / 2); e += 16) {
-                    uint32_t o[16];
-                    tmem_ld_x16_sync(lanes + kTmO + e, o);
+#pragma unroll 2
+                for (int e = half * (D / 2); e < (half + 1) * (D / 2); e += 32) {
+                    uint32_t o[32];
+                    tmem_ld_x32_sync(lanes + kTmO + e, o);
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) sums[(e + j) * kTileRows] = __uint_as_float(o[j]);
+                    for (int j = 0; j < 32; ++j) sums[(e + j) * kTileRows] = __uint_as_float(o[j]);
                 }
                 if (half == 0) work.stats[place * 2 * kTileRows + r] = ref, work.stats[(place * 2 + 1) * kTileRows + r] = den;
                 if (tid == 0 && at.x == 0) {
@@ -389,7 +393,7 @@ __global__ void __launch_bounds__(kAttendTileThreads, 1)
                 const float scale_out = den > 0.0f ? kCodeUp / den : 0.0f;
                 const int i = first + r;
                 const long long row = (static_cast<long long>(seq.lo) + i / a.group) * heads * a.group + at.h * a.group + i % a.group;
-#pragma unroll 1
+#pragma unroll 2
                 for (int e = half * (D / 2); e < (half + 1) * (D / 2); e += 16) {
                     uint32_t o[16], w[8];
                     tmem_ld_x16_sync(lanes + kTmO + e, o);
