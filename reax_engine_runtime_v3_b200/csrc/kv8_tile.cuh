@@ -9,17 +9,22 @@
 // instructions of bf16 to make from codes.  A weight is split into two bf16 numbers, hi + lo (cut, not rounded: 2^-15), whose exponents reach as far as
 // float32's: a single bf16 would lose half the output's bits again, and fp16 the weights below 2^-28 of the largest.
 //
-// What bounds it: 128 x 64 scores cost about 1000 tensor cycles at 256 values a head (an MMA of N = 64 takes 60 cycles with
-// its A operand in TMEM, and twice that with q read from shared memory beside the conversion's traffic: q lives in TMEM), O
-// another 1000 with both terms; the softmax, the split and the codes' conversion take the other pipes about as long.  The
-// roles overlap.
+// What bounds it: at 256 values a head a tile takes about 2650 cycles (1.55 us), of which the tensor cores work 2000 (128 x 64
+// scores cost 1000: an MMA of N = 64 takes 60 cycles with its A operand in TMEM, and twice that with q read from shared memory
+// beside the conversion's traffic, so q lives in TMEM; O costs another 1000 with both terms).  The softmax's chain from a
+// tile's scores to its weights takes 2600, the codes' conversion 2500.  The roles overlap.
 //
 // Scaling O (in TMEM) costs as much as a tile, so the reference that the exponents are taken from moves only when a maximum
 // exceeds it by 8 (in log2): weights stay below 2^8, which bf16 holds as well as any.
 //
+// Work.  The tiles of all items lie on one line, of which each block takes an equal part; parts of items that blocks share are
+// joined by a second kernel, in the blocks' order.  2048 rows of four prompts (19676 tiles) take 270 us; a block for each item
+// had left the longest for the end (510 us), and one sequence of 65536 cached rows and 16 new ones to four blocks (2305 us,
+// now 95).
+//
 // Roles (17 warps): 0-7 softmax (thread = row and half of the columns), 8 loads, 12 MMAs of the scores, 16 those of O, the
-// others codes to 16 bits.  Waiting for and issuing both sorts of MMA takes one warp longer than the MMAs take (332 us for 2048
-// rows of four prompts, MEASURED with two); the two, and the loads, share a scheduler with softmax warps alone.
+// others codes to 16 bits.  Waiting for and issuing both sorts of MMA takes one warp 3350 cycles a tile.  The two, and the
+// loads, share a scheduler with softmax warps alone.
 #pragma once
 
 #include "common.cuh"
@@ -49,6 +54,7 @@ struct TileShared {
     uint64_t in[2][2], in_free[2][2], k_full[2], v_full[2], k_free[2], v_free[2], s_full, s_free, p_full, pv_done, drained[2];
     uint32_t tmem;
     uint32_t abort;
+    bool more[2];                             // a tile's outputs are added to those of the item's tiles before
 };
 
 // fp32 sums of bf16 operands; b_mn: B is stored with N contiguous.
@@ -97,14 +103,21 @@ struct TileSeq {
     }
 };
 
-// A place on the line of tiles: of the cached heads one after the other, in each of the items of the sequences.
+// A place on the line of items: of the cached heads one after the other, in each those of the sequences.  An item is as long
+// as its tiles and kItemTiles more, which come first and stand for the time that it takes to begin and end one (its rows
+// of q, its outputs; measured 9 us): 2048 rows of four prompts take 290 us where only tiles are counted, 270 with it.
+constexpr int kItemTiles = 5;
 struct TileCursor {
-    long long u;
-    int h, b, item, x, tiles;
+    long long end;                            // the item's on the line
+    int h, b, item, x, to, tiles;             // [x, to): this block's of its tiles
     TileSeq s;
-    // Go on with the item at u (past `to - x` tiles), which is on the line.
-    REAX_DEVI void next(const Kv8Attend& a) {
-        x = 0;
+    REAX_DEVI void take(long long from, long long u1) {
+        x = static_cast<int>(max(tiles - (end - from), 0ll));
+        to = static_cast<int>(tiles - max(end - u1, 0ll));
+    }
+    // The next item of which this block has tiles.
+    REAX_DEVI bool next(const Kv8Attend& a, long long u1) {
+        if (end + kItemTiles >= u1) return false;
         if (++item >= s.items) {
             item = 0;
             do {
@@ -113,6 +126,10 @@ struct TileCursor {
             } while (s.items == 0);
         }
         tiles = s.tiles(a, item);
+        end += kItemTiles + tiles;
+        take(0, u1);
+        x = 0;
+        return true;
     }
 };
 
@@ -143,9 +160,9 @@ __global__ void __launch_bounds__(kAttendTileThreads, 1)
     const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32, quarter = warp % 4;
     const int heads = a.c.heads, page = a.c.page, shift = __ffs(page) - 1;
     asm volatile("griddepcontrol.launch_dependents;");        // (the join, which waits for the end of this grid)
-    // this block's stretch [u0, u1) of the line, and where it begins
+    // this block's stretch [u0, u1) of the line, and what it begins with
     long long u0 = 0, u1 = 0, all = 0;
-    int blocks = 0;
+    int blocks = 0, n = 0;                                    // n: its tiles
     TileCursor start;
     {
         auto count = [&](int b0) {
@@ -153,7 +170,7 @@ __global__ void __launch_bounds__(kAttendTileThreads, 1)
             for (int b = b0 + warp; b < min(a.batch, b0 + kTileSeqs); b += kAttendTileThreads / 32) {
                 const TileSeq s(a, b);
                 long long n = 0;
-                for (int i = lane; i < s.items; i += 32) n += s.tiles(a, i);
+                for (int i = lane; i < s.items; i += 32) n += kItemTiles + s.tiles(a, i);
                 n = warp_sum_ll(n);
                 if (lane == 0) sh.units[b - b0] = n;
             }
@@ -167,11 +184,10 @@ __global__ void __launch_bounds__(kAttendTileThreads, 1)
             head += warp_sum_ll(n);
         }
         all = head * heads;
-        blocks = static_cast<int>(min(static_cast<long long>(gridDim.x), all));
+        blocks = static_cast<int>(min(static_cast<long long>(gridDim.x), all / (kItemTiles + 1)));   // (each gets a tile)
         if (tid == 0) work.rest[blockIdx.x].parts = 0;
         if (static_cast<int>(blockIdx.x) >= blocks) return;
         u0 = all * blockIdx.x / blocks, u1 = all * (blockIdx.x + 1) / blocks;
-        start.u = u0;
         start.h = static_cast<int>(u0 / head);
         long long rest = u0 - start.h * head;
         int b = -1;
@@ -186,12 +202,16 @@ __global__ void __launch_bounds__(kAttendTileThreads, 1)
         start.s = TileSeq(a, b);
         int item = -1;
         for (int i = 0; item < 0; i += 32) {
-            const int l = warp_find(i + lane < start.s.items ? start.s.tiles(a, i + lane) : 0, &rest, lane);
+            const int l = warp_find(i + lane < start.s.items ? kItemTiles + start.s.tiles(a, i + lane) : 0, &rest, lane);
             if (l >= 0) item = i + l;
         }
         start.item = item;
-        start.x = static_cast<int>(rest);
         start.tiles = start.s.tiles(a, item);
+        start.end = u0 - rest + kItemTiles + start.tiles;
+        start.take(u0, u1);
+        TileCursor at = start;
+        do n += at.to - at.x;
+        while (at.next(a, u1));
     }
 
     if (warp == 12) tmem_alloc(&sh.tmem, 512);
@@ -232,7 +252,7 @@ __global__ void __launch_bounds__(kAttendTileThreads, 1)
         for (TileCursor at = start;;) {
             const TileSeq& seq = at.s;
             const int first = at.item * kTileRows, live = min(kTileRows, seq.rows * a.group - first);
-            const int to = static_cast<int>(min(static_cast<long long>(at.tiles), at.x + (u1 - at.u)));
+            const int to = at.to;
             const int32_t* table = a.tables + static_cast<long long>(at.b) * a.table_ld;
             float scale = a.scale * 1.44269504f;
             {
@@ -363,6 +383,7 @@ __global__ void __launch_bounds__(kAttendTileThreads, 1)
                 }
                 tmem_wait_st();
                 tc_fence_before();
+                if (tid == 0) sh.more[t0 & 1] = x > at.x;
                 arrive(&sh.p_full);
             }
             // out
@@ -386,8 +407,7 @@ __global__ void __launch_bounds__(kAttendTileThreads, 1)
                 if (half == 0) work.stats[place * 2 * kTileRows + r] = ref, work.stats[(place * 2 + 1) * kTileRows + r] = den;
                 if (tid == 0 && at.x == 0) {
                     // the last block that has a part of it
-                    const long long last = at.u + at.tiles;
-                    work.rest[blockIdx.x] = {seq.lo, first, live, at.h, static_cast<int>((last * blocks - 1) / all) - static_cast<int>(blockIdx.x) + 1};
+                    work.rest[blockIdx.x] = {seq.lo, first, live, at.h, static_cast<int>((at.end * blocks - 1) / all) - static_cast<int>(blockIdx.x) + 1};
                 }
             } else {
                 const float scale_out = den > 0.0f ? kCodeUp / den : 0.0f;
@@ -407,16 +427,14 @@ __global__ void __launch_bounds__(kAttendTileThreads, 1)
                 }
                 if (a.lse && half == 0 && r < live) a.lse[row] = den > 0.0f ? 0.69314718f * (ref + log2f(den)) : -INFINITY;
             }
-            at.u += to - at.x;
-            if (at.u >= u1) break;
-            at.next(a);
+            if (!at.next(a, u1)) break;
         }
     } else if (warp == 12) {
         // ---------------------------------------------------------------------------------------- MMAs of the scores
         if (lane == 0) {
             constexpr uint32_t id_s = idesc_f16_f32(128, kTileCols, false);
 #pragma unroll 1
-            for (int t = 0, n = static_cast<int>(u1 - u0); t < n; ++t) {
+            for (int t = 0; t < n; ++t) {
                 const int buf = t & 1;
                 const uint64_t kd = sw128_kmajor_desc(smem_u32(sh.k[buf]));
                 wait(&sh.k_full[buf], (t >> 1) & 1, kStatusTimeoutFull);
@@ -436,22 +454,20 @@ __global__ void __launch_bounds__(kAttendTileThreads, 1)
         // ----------------------------------------------------------------------------------------------- MMAs of O
         if (lane == 0) {
             constexpr uint32_t id_o = idesc_bf16_ts(128, D, true);
-            TileCursor at = start;
 #pragma unroll 1
-            for (int t = 0, n = static_cast<int>(u1 - u0); t < n; ++t) {
+            for (int t = 0; t < n; ++t) {
                 const int buf = t & 1;
                 const uint64_t vd = sw128_mn_desc(smem_u32(sh.v[buf]), kTileCols * 128);
-                const bool more = t > 0 && at.x > 0;          // (not an item's first tile, nor this block's)
                 wait(&sh.v_full[buf], (t >> 1) & 1, kStatusTimeoutFull);
                 wait(&sh.p_full, t & 1, kStatusTimeoutEmpty);
                 if (wait.dead) break;
                 tc_fence_after();
+                const bool more = sh.more[buf];
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
                     umma_f16_ts(tm + kTmO, tm + kTmWeight + (e / 4) * 32 + (e % 4) * 8, vd + (e % 4) * 128, id_o, more || e > 0);
                 umma_commit(&sh.pv_done);
                 umma_commit(&sh.v_free[buf]);
-                if (t + 1 < n && ++at.x == at.tiles) at.next(a);
             }
             drain_mmas(&sh.drained[1]);
         }
@@ -467,7 +483,7 @@ __global__ void __launch_bounds__(kAttendTileThreads, 1)
         };
         look_up();
 #pragma unroll 1
-        for (int t = 0, n = static_cast<int>(u1 - u0); t < n; ++t) {
+        for (int t = 0; t < n; ++t) {
             const bool in = id >= 0 && id < a.c.pages;
             const int from = (id * heads + at.h) * page + ((at.x * kTileCols + lane * 16) & (page - 1)), buf = t & 1;
             const uint32_t have = __popc(__ballot_sync(0xFFFFFFFFu, in));
@@ -488,7 +504,7 @@ __global__ void __launch_bounds__(kAttendTileThreads, 1)
                 __syncwarp();
             }
             if (t + 1 < n) {
-                if (++at.x == at.tiles) at.next(a);
+                if (++at.x == at.to) at.next(a, u1);
                 look_up();
             }
         }
@@ -505,7 +521,7 @@ __global__ void __launch_bounds__(kAttendTileThreads, 1)
         const int from = D == 64 ? step_at<64>(lane % 8, lane / 8 * 16) : (lane % 8) * 128 + ((lane / 8) ^ (lane % 8)) * 16;
         const int into = (lane % 8) * 128 + ((lane / 8 * 2) ^ (lane % 8)) * 16;
 #pragma unroll 1
-        for (int t = 0, n = static_cast<int>(u1 - u0); t < n; ++t) {
+        for (int t = 0; t < n; ++t) {
             const int buf = t & 1;
 #pragma unroll 1
             for (int e = 0; e < 2; ++e) {
