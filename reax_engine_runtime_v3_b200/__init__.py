@@ -12,6 +12,11 @@ Drop-in modules mirror the reference's import names and call signatures:
   reax_engine_runtime_v3_b200.runtime.mixed_origin_bf16      <- runtime/mixed_origin_bf16.py
   reax_engine_runtime_v3_b200.runtime.split_gated_projection <- runtime/split_gated_projection.py
 
+The token mixers beside them have names of their own:
+
+  reax_engine_runtime_v3_b200.gated_delta   the gated delta rule: prefill (packed prompts), decode (a row of each sequence)
+  reax_engine_runtime_v3_b200.kv_int8       Int8Cache: a paged INT8 cache (append, read) and attention over it
+
 ``install()`` registers them under the reference's own module names (``reaxv2.gate_up`` ...) so
 callers that import those names get this implementation.  Every kernel runs through the C ABI of
 ``libreax_b200.so``; there is no CPU or library fallback.

@@ -187,8 +187,8 @@ def noalloc_status(clear: bool = False) -> int:
 
 
 def mixer_status(clear: bool = False) -> int:
-    """Status word of the gated delta rule's prompt form on the current device, after the current stream's work
-    (synchronizes that stream); non-zero means a bounded wait expired."""
+    """Status word of the gated delta rule's prompt form and the attention of many rows on the current device, after the
+    current stream's work (synchronizes that stream); non-zero means a bounded wait expired."""
     v = C.c_uint(0)
     check(load().reax_mixer_status(C.byref(v), 1 if clear else 0, stream_handle()))
     return int(v.value)

@@ -818,8 +818,7 @@ int device_sms(int device) {
     return cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess ? sms : -1;
 }
 
-int encode_rows(CUtensorMap* map, const void* base, int cols, int rows, long long ld, int box_cols, int box_rows,
-                bool swizzle) {
+int encode_rows(CUtensorMap* map, const void* base, int cols, int rows, long long ld, int box_cols, int box_rows) {
     PFN_cuTensorMapEncodeTiled_v12000 enc;
     int rc = get_encoder(&enc);
     if (rc != REAX_OK) return rc;
@@ -828,8 +827,7 @@ int encode_rows(CUtensorMap* map, const void* base, int cols, int rows, long lon
     cuuint32_t box[2] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows)};
     cuuint32_t estr[2] = {1, 1};
     CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, estr,
-                     CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
-                     CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS)
         return fail(REAX_ERR_INVALID, "cuTensorMapEncodeTiled failed (%d) for %d rows of %d values, stride %lld",

@@ -1,8 +1,8 @@
 // Attention of few query rows over the paged INT8 cache: a step of the serving loop.
 //
 // What bounds it is the cache's bytes, read once: k and v codes of a page and head are copied into shared memory (16-byte
-// pieces xor-ed with their row's number, against bank conflicts), are turned into fp16 in registers (exact: |code| <= 128) and multiplied with mma.sync m16n8k16,
-// whose 16 rows hold the query rows and heads that share a cached head.  tcgen05 tiles would be 128 rows high, all but
+// pieces xor-ed with their row's number, against bank conflicts), are turned into fp16 in registers (exact: |code| <= 128) and
+// multiplied with mma.sync m16n8k16, whose 16 rows hold the query rows and heads that share a cached head.  tcgen05 tiles would be 128 rows high, all but
 // a few of them empty; at 16 rows the tensor cores need a third of the time that the bytes take.
 //
 // Scales.  A page's scale of k multiplies its scores.  A page's scale of v (s_v) would multiply the weights, whose fp16

@@ -20,7 +20,7 @@
 // Work.  The tiles of all items lie on one line, of which each block takes an equal part; parts of items that blocks share are
 // joined by a second kernel, in the blocks' order.  2048 rows of four prompts (19676 tiles) take 270 us; a block for each item
 // had left the longest for the end (510 us), and one sequence of 65536 cached rows and 16 new ones to four blocks (2305 us,
-// now 95).
+// now 73).
 //
 // Roles (17 warps): 0-7 softmax (thread = row and half of the columns), 8 loads, 12 MMAs of the scores, 16 those of O, the
 // others codes to 16 bits.  Waiting for and issuing both sorts of MMA takes one warp 3350 cycles a tile.  The two, and the

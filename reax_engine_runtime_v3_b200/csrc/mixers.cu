@@ -95,9 +95,9 @@ int gdn_chunks(const char* who, const reax::GdnParams& p, void* workspace, int s
     int rc = allow_smem(reinterpret_cast<const void*>(reax::gdn_chunk_kernel<DK, DV>), done, reax::gdn_chunk_smem());
     if (rc == REAX_OK) rc = allow_smem(reinterpret_cast<const void*>(reax::gdn_tiles_kernel<DK>), tiles_done, reax::gdn_tiles_smem());
     reax::GdnMaps maps;
-    if (rc == REAX_OK) rc = reax_abi::encode_rows(&maps.v, p.v, p.v_heads * DV, p.rows, p.ldv, DV, reax::kChunk, false);
+    if (rc == REAX_OK) rc = reax_abi::encode_rows(&maps.v, p.v, p.v_heads * DV, p.rows, p.ldv, DV, reax::kChunk);
     if (rc == REAX_OK)
-        rc = reax_abi::encode_rows(&maps.out, p.out, p.v_heads * DV, p.rows, static_cast<long long>(p.v_heads) * DV, 32, 32, false);
+        rc = reax_abi::encode_rows(&maps.out, p.out, p.v_heads * DV, p.rows, static_cast<long long>(p.v_heads) * DV, 32, 32);
     const long long most = gdn_most_chunks(p.rows, p.batch), slab = gdn_slab(p.rows, p.batch, p.k_heads, p.v_heads, DK);
     reax::GdnScratch scratch;
     scratch.tiles = static_cast<reax::GdnTiles*>(workspace);
@@ -166,8 +166,10 @@ struct AttendWorkspace {
     }
 };
 
-// Rows x heads of a sequence up to which the step form is used: it reads the cache once for each 16 of them.
-constexpr int kStepMostRows = 32;
+// Rows x heads of a sequence up to which the step form is used: it reads the cache once for each 16 of them.  Measured at 256
+// values a head, 4 cached heads of 64 sequences with 4096 cached rows: 16 rows x heads 150 us by it and 206 by the form for
+// many rows, 32 of them 262 and 208; of one sequence with 65536, 16: 84 and 73, 32: 104 and 73; of one with 4096, 8: 26 and 33.
+constexpr int kStepMostRows = reax::kStepRows;
 
 template <int D>
 int attend_tiles(const char* who, const reax::Kv8Attend& a, const reax::Kv8Maps& maps, void* workspace, int sms, void* stream) {
