@@ -207,6 +207,30 @@ def test_long_sequence():
     compare(out, state, *definition(*x, spans, [0]))
 
 
+def test_more_chunks_than_the_scratch_memory_holds():
+    """A batch that takes several launches gives what its sequences give alone, bit for bit."""
+    from reax_engine_runtime_v3_b200 import _native, gated_delta
+    heads, lens = 512, [2500, 0, 1300, 65]
+    n = sum(lens)
+    size = _native.load().reax_gdn_workspace_bytes
+    assert size(n, len(lens), heads, heads, 128) == size(2 * n, len(lens), heads, heads, 128)     # (one launch holds no more)
+    assert size(max(lens), 1, heads, heads, 128) < size(n, len(lens), heads, heads, 128)
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    rnd = lambda *s: torch.randn(*s, generator=gen, device="cuda")
+    q, k, v = rnd(n, heads, 128).bfloat16(), rnd(n, heads, 128).bfloat16(), rnd(n, heads, 64).bfloat16()
+    g, beta, state = -torch.rand(n, heads, generator=gen, device="cuda"), torch.rand(n, heads, generator=gen, device="cuda"), \
+        rnd(len(lens), heads, 128, 64)
+    alone, outs, at = state.clone(), [], 0
+    for b, m in enumerate(lens):
+        rows = slice(at, at + m)
+        if m:
+            outs.append(gated_delta.prefill(q[rows], k[rows], v[rows], g[rows], beta[rows], alone[b:b + 1]))
+        at += m
+    cu = torch.tensor([0, *torch.tensor(lens).cumsum(0).tolist()], dtype=torch.int32, device="cuda")
+    out = gated_delta.prefill(q, k, v, g, beta, state, cu_seqlens=cu)
+    assert torch.equal(out, torch.cat(outs)) and torch.equal(state, alone)
+
+
 def test_refusals():
     from reax_engine_runtime_v3_b200 import gated_delta
     x = [t.cuda() for t in inputs(17, 4, 2, 4, 128, 128, 4)]

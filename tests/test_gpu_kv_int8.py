@@ -114,6 +114,18 @@ def test_attend_rows_that_see_nothing():
     assert not out[:4].any() and (lse[:4] == -math.inf).all() and not out[9:13].any()
 
 
+@pytest.mark.parametrize("heads,group,rows,lens", [
+    (1, 4, [(5 * i) % 9 + 1 for i in range(300)], [(37 * i) % 150 + 9 for i in range(300)]),    # more sequences than are counted at once
+    (3, 1, [17] * 50, [17] * 50),                                                                # items of a tile each
+    (2, 4, [0, 40, 0, 0, 25, 0], [10, 900, 0, 64, 25, 3]),                                       # sequences without rows
+    (1, 2, [20], [30000]),                                                                       # one item for all blocks
+    (2, 5, [131, 3], [2500, 4000]),
+])
+def test_attend_blocks_share_the_tiles(heads, group, rows, lens):
+    cache, tables = filled(len(rows), lens, heads, 128, 32)
+    check_attend(cache, tables, rows, lens, group, seed=8, max_rows=1000)
+
+
 def test_attend_hint_does_not_change_results_beyond_rounding():
     """Every value of the hint has to be right, a wrong one too."""
     lens, rows = [300, 64, 1], [20, 3, 1]
