@@ -16,7 +16,7 @@
 // Loads.  Each warp fetches its own 16 rows of a tile into its own ring with asynchronous 16-byte copies, so that warps never
 // wait for one another but to join their parts, and all registers go to eight warps on an SM.  (A fifth warp for the loads
 // left 168 of 255 registers and the outputs of 256 columns spilled; boxes of 16 rows by TMA cost about 1100 cycles a tile to
-// issue: 141 us for 64 sequences with 261000 rows, where the copies take 134.)
+// issue: 141 us for 64 sequences with 261000 rows, where the copies took 134; the call takes 131 now, 4.1 TB/s.)
 //
 // Work.  Tiles of 64 cached rows of every (sequence, cached head, 16 query rows) lie on one line, of which each block takes
 // an equal part: lengths need not be known on the host and long ones are split by themselves.  A part of an item that
@@ -40,7 +40,7 @@ template <int D>
 struct StepShared {
     static constexpr int kStages = D == 256 ? 2 : 4;
     uint8_t kv[kStages][4][2][16 * D];        // a warp's 16 rows of codes of k and v
-    float o[kStepRows][D + 16];               // parts of the output added up (columns in the order of step_col)
+    float o[2][kStepRows][D + 16];            // outputs of warps 0 and 1, and of 2 and 3 (columns in the order of step_col)
     __half q[kStepRows][D + 8];
     float q_scale[kStepRows];
     float4 meta[kStages][4];                  // of each 16 rows: scale of k, log2 and inverse of that of v, 1 if in the cache
@@ -408,8 +408,8 @@ __global__ void __launch_bounds__(kAttendStepThreads, kStepBlocksPerSm)
             constexpr int W = D == 64 ? 8 : 16;
             const int live = min(kStepRows, s.rows * a.group - at);
 #pragma unroll 1
-            for (int w = 0; w < 4; ++w) {
-                if (warp == w) {
+            for (int w = 0; w < 2; ++w) {
+                if (warp % 2 == w) {
 #pragma unroll
                     for (int r = 0; r < 2; ++r)
                         if (g + 8 * r < live)
@@ -421,7 +421,7 @@ __global__ void __launch_bounds__(kAttendStepThreads, kStepBlocksPerSm)
                                     for (int j = 0; j < W; j += 4) {
                                         const float(*x)[4] = o + blk * W + j;
                                         const int k = 2 * r + e;
-                                        float4& y = *reinterpret_cast<float4*>(&sh.o[g + 8 * r][step_col(blk * 8 * W + (2 * q + e) * W + j)]);
+                                        float4& y = *reinterpret_cast<float4*>(&sh.o[warp / 2][g + 8 * r][step_col(blk * 8 * W + (2 * q + e) * W + j)]);
                                         float4 z = w == 0 ? float4{} : y;
                                         z.x += x[0][k] * f[r], z.y += x[1][k] * f[r], z.z += x[2][k] * f[r], z.w += x[3][k] * f[r];
                                         y = z;
@@ -448,6 +448,10 @@ __global__ void __launch_bounds__(kAttendStepThreads, kStepBlocksPerSm)
                     *reinterpret_cast<uint32_t*>(a.out + row * D + e * 64 + lane * 2) = bf16x2_rn(f2(y[2 * e] * inv, y[2 * e + 1] * inv));
                 if (lane == 0 && a.lse) a.lse[row] = d > 0.0f ? 0.69314718f * (m + log2f(d)) : -INFINITY;
             };
+            auto two_columns = [&](int r, int col) {
+                const float2 x = *reinterpret_cast<const float2*>(&sh.o[0][r][step_col(col)]), y = *reinterpret_cast<const float2*>(&sh.o[1][r][step_col(col)]);
+                return float2{x.x + y.x, x.y + y.y};
+            };
             if (whole) {
 #pragma unroll 1
                 for (int r = warp; r < live; r += 4) {
@@ -455,7 +459,7 @@ __global__ void __launch_bounds__(kAttendStepThreads, kStepBlocksPerSm)
                     row_stat(r, &m, &d);
 #pragma unroll
                     for (int e = 0; e < D / 64; ++e) {
-                        const float2 z = *reinterpret_cast<const float2*>(&sh.o[r][step_col(e * 64 + lane * 2)]);
+                        const float2 z = two_columns(r, e * 64 + lane * 2);
                         y[2 * e] = z.x, y[2 * e + 1] = z.y;
                     }
                     write_row(r, m, d, y);
@@ -477,7 +481,7 @@ __global__ void __launch_bounds__(kAttendStepThreads, kStepBlocksPerSm)
 #pragma unroll
                 for (int e = 0; e < D / 64; ++e)
                     __stcg(reinterpret_cast<float2*>(work.parts + (static_cast<long long>(part) * kStepRows + r) * D + e * 64 + lane * 2),
-                           *reinterpret_cast<const float2*>(&sh.o[r][step_col(e * 64 + lane * 2)]));
+                           two_columns(r, e * 64 + lane * 2));
             }
             __threadfence();
             __syncthreads();
@@ -492,6 +496,18 @@ __global__ void __launch_bounds__(kAttendStepThreads, kStepBlocksPerSm)
 #pragma unroll 1
                 for (int r = warp; r < live; r += 4) {
                     float m = -INFINITY, d = 0.0f, y[D / 32] = {};
+                    float2 z[16][D / 64];
+                    auto fetch = [&](int first) {             // 16 parts (past the end: factor 0)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+#pragma unroll
+                            for (int e = 0; e < D / 64; ++e) {
+                                const int w = min(first + i, w1), slot = 2 * w + (w == w0);
+                                z[i][e] = __ldcg(reinterpret_cast<const float2*>(
+                                    work.parts + (static_cast<long long>(slot) * kStepRows + r) * D + e * 64 + lane * 2));
+                            }
+                    };
+                    fetch(w0);
                     for (int w = w0 + lane; w <= w1; w += 32) m = fmaxf(m, __ldcg(&work.stats[(2 * w + (w == w0)) * 2 * kStepRows + r]));
                     m = warp_max(m);
                     // 32 parts at a time: a lane has the factor of one
@@ -508,21 +524,13 @@ __global__ void __launch_bounds__(kAttendStepThreads, kStepBlocksPerSm)
                         const int n_parts = min(32, w1 - first + 1);
 #pragma unroll 1
                         for (int i0 = 0; i0 < n_parts; i0 += 16) {
-                            float2 z[16][D / 64];
-#pragma unroll
-                            for (int i = 0; i < 16; ++i)
-#pragma unroll
-                                for (int e = 0; e < D / 64; ++e) {
-                                    const int w = min(first + i0 + i, w1), slot = 2 * w + (w == w0);     // (past the end: factor 0)
-                                    z[i][e] = __ldcg(reinterpret_cast<const float2*>(
-                                        work.parts + (static_cast<long long>(slot) * kStepRows + r) * D + e * 64 + lane * 2));
-                                }
 #pragma unroll
                             for (int i = 0; i < 16; ++i) {
                                 const float fw = __shfl_sync(0xFFFFFFFFu, f_lane, i0 + i);
 #pragma unroll
                                 for (int e = 0; e < D / 64; ++e) y[2 * e] += fw * z[i][e].x, y[2 * e + 1] += fw * z[i][e].y;
                             }
+                            if (first + i0 + 16 <= w1) fetch(first + i0 + 16);
                         }
                     }
                     write_row(r, m, d, y);
