@@ -121,7 +121,6 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const Kv8App
     const int b = s_seq, pg = s_page;
     if (b < 0 || pg >= a.table_ld) return;
     const int id = a.tables[static_cast<long long>(b) * a.table_ld + pg];
-    if (id < 0 || id >= a.c.pages) return;
     int lo, hi;
     kv8_span(a.cu, b, a.rows, &lo, &hi);
     const int len = max(a.lengths[b], 0), h = blockIdx.y, dim = a.c.dim;
@@ -130,24 +129,29 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const Kv8App
     const bool is_v = blockIdx.z != 0;
     const long long ld = is_v ? a.ldv : a.ldk;
     const __nv_bfloat16* src = (is_v ? a.v : a.k) + (lo + static_cast<long long>(pg) * a.c.page + from - len) * ld + h * dim;
+    const int per_row = dim / 8, row_shift = __ffs(per_row) - 1, total = (to - from) * per_row;       // pieces of 8 values
+    constexpr int kHeld = 64 * 256 / 8 / kAppendThreads;              // a whole page of the largest size
+    uint4 x[kHeld];                                                   // (asked for before the page's number is looked at)
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+        const int e = tid + i * kAppendThreads;
+        x[i] = e < total ? *reinterpret_cast<const uint4*>(src + (e >> row_shift) * ld + (e & (per_row - 1)) * 8) : uint4{};
+    }
+    if (id < 0 || id >= a.c.pages) return;
     const long long at = static_cast<long long>(id) * a.c.heads + h;
     int8_t* dst = (is_v ? a.c.v : a.c.k) + at * a.c.page * dim;
     float* scale = (is_v ? a.c.v_scale : a.c.k_scale) + at;
-    const int per_row = dim / 8, row_shift = __ffs(per_row) - 1, total = (to - from) * per_row;       // pieces of 8 values
-    constexpr int kHeld = 64 * 256 / 8 / kAppendThreads;              // a whole page of the largest size
-    uint4 x[kHeld];
+    const float was = from > 0 ? *scale : 0.0f;
     float m = 0.0f;
 #pragma unroll
     for (int i = 0; i < kHeld; ++i) {
         const int e = tid + i * kAppendThreads;
         if (e < total) {
-            x[i] = *reinterpret_cast<const uint4*>(src + (e >> row_shift) * ld + (e & (per_row - 1)) * 8);
             m = absmax_finite(absmax_finite(absmax_finite(absmax_finite(m, x[i].x), x[i].y), x[i].z), x[i].w);
         }
     }
     m = warp_max(m);
     if (lane == 0) s_max[tid / 32] = m;
-    const float was = from > 0 ? *scale : 0.0f;
     __syncthreads();
     m = s_max[0];
 #pragma unroll
