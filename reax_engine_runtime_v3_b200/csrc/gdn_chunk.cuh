@@ -155,14 +155,6 @@ REAX_DEVI float2 scale_of(float m) {
     return float2{__uint_as_float((267u - e) << 23), __uint_as_float((e - 13u) << 23)};
 }
 
-// (x0, x1) as fp16 pairs hi + lo.
-REAX_DEVI void split2(float x0, float x1, uint32_t& hi, uint32_t& lo) {
-    const __half2 h = __floats2half2_rn(x0, x1);
-    const float2 f = __half22float2(h);
-    const __half2 l = __floats2half2_rn(x0 - f.x, x1 - f.y);
-    hi = *reinterpret_cast<const uint32_t*>(&h);
-    lo = *reinterpret_cast<const uint32_t*>(&l);
-}
 REAX_DEVI uint32_t half2_bits(float x0, float x1) {
     const __half2 h = __floats2half2_rn(x0, x1);
     return *reinterpret_cast<const uint32_t*>(&h);
