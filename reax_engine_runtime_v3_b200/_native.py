@@ -93,6 +93,17 @@ def check(status: int) -> None:
         raise RuntimeError(f"REAX B200 status {status} ({ERRORS.get(status, 'unknown')}): {message}")
 
 
+def launch(device: torch.device, entry: str, *args) -> None:
+    """Call an entry with the tensors' device current (the library launches on the current one) and check its status.
+    The device is switched only where it has to be: a switch and back costs as much as a small launch."""
+    fn = getattr(load(), entry)
+    if device.index == torch.cuda.current_device():
+        check(fn(*args))
+    else:
+        with torch.cuda.device(device):
+            check(fn(*args))
+
+
 def ptr(t: torch.Tensor | None) -> int | None:
     """Device address of a tensor (None for a missing or empty optional operand)."""
     if t is None or t.numel() == 0:
@@ -186,11 +197,13 @@ def noalloc_status(clear: bool = False) -> int:
     return int(v.value)
 
 
-def mixer_status(clear: bool = False) -> int:
-    """Status word of the gated delta rule's prompt form and the attention of many rows on the current device, after the
-    current stream's work (synchronizes that stream); non-zero means a bounded wait expired."""
+def mixer_status(clear: bool = False, device: torch.device | None = None) -> int:
+    """Status word of the gated delta rule's prompt form and the attention of many rows on `device` (the current one if not
+    given), after the work of the stream that is current there (synchronizes it); non-zero means a bounded wait expired."""
+    if device is None:
+        device = torch.device("cuda", torch.cuda.current_device())
     v = C.c_uint(0)
-    check(load().reax_mixer_status(C.byref(v), 1 if clear else 0, stream_handle()))
+    launch(device, "reax_mixer_status", C.byref(v), 1 if clear else 0, stream_handle(device))
     return int(v.value)
 
 

@@ -69,15 +69,14 @@ def prefill(q, k, v, g, beta, state, *, cu_seqlens=None, slots=None, carry=True,
         assert cu_seqlens.dtype is torch.int32 and cu_seqlens.dim() == 1 and cu_seqlens.is_contiguous(), \
             "cu_seqlens is contiguous int32"
         _native.require_one_device(q, cu_seqlens)
-    lib = _native.load()
     # scratch memory of this call: torch's allocator keeps it for the next one on this stream
-    size = lib.reax_gdn_workspace_bytes(q.shape[0], batch, sizes[0], sizes[1], sizes[2])
+    size = _native.load().reax_gdn_workspace_bytes(q.shape[0], batch, sizes[0], sizes[1], sizes[2])
     scratch = torch.empty(size, dtype=torch.uint8, device=q.device)
-    _native.check(lib.reax_gdn_prefill(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), state.data_ptr(),
+    _native.launch(
+        q.device, "reax_gdn_prefill", q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), state.data_ptr(),
         None if cu_seqlens is None else cu_seqlens.data_ptr(), None if slots is None else slots.data_ptr(), out.data_ptr(),
         q.shape[0], batch, *sizes, *strides, sizes[2] ** -0.5 if scale is None else scale, normalize, carry,
-        scratch.data_ptr(), size, _native.stream_handle(q.device)))
+        scratch.data_ptr(), size, _native.stream_handle(q.device))
     return out
 
 
@@ -85,8 +84,8 @@ def decode(q, k, v, g, beta, state, *, slots=None, scale=None, normalize=True, o
     """One row of each sequence, from the states kept: arguments and result as ``prefill``, row b is sequence b's."""
     n = q.shape[0]
     out, strides, sizes = _check(q, k, v, g, beta, state, slots, out, n)
-    _native.check(_native.load().reax_gdn_decode(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), state.data_ptr(),
+    _native.launch(
+        q.device, "reax_gdn_decode", q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), state.data_ptr(),
         None if slots is None else slots.data_ptr(), out.data_ptr(), n, *sizes, *strides,
-        sizes[2] ** -0.5 if scale is None else scale, normalize, _native.stream_handle(q.device)))
+        sizes[2] ** -0.5 if scale is None else scale, normalize, _native.stream_handle(q.device))
     return out

@@ -73,10 +73,10 @@ class Int8Cache:
         assert n == v.shape[0], "k and v have the same rows"
         batch, width = self._sequences(tables, lengths, cu_seqlens, n, "lengths")
         _native.require_one_device(self.k, k, v, tables, lengths, cu_seqlens)
-        _native.check(_native.load().reax_kv8_append(
-            k.data_ptr(), v.data_ptr(), *self._cache(), tables.data_ptr(), lengths.data_ptr(),
+        _native.launch(
+            k.device, "reax_kv8_append", k.data_ptr(), v.data_ptr(), *self._cache(), tables.data_ptr(), lengths.data_ptr(),
             None if cu_seqlens is None else cu_seqlens.data_ptr(), n, batch, width, self.pages, self.heads, self.page, self.dim,
-            ldk, ldv, _native.stream_handle(k.device)))
+            ldk, ldv, _native.stream_handle(k.device))
 
     def read(self, tables, starts, cu_seqlens, rows):
         """Sequence b's rows ``starts[b]`` on, ``cu_seqlens[b + 1] - cu_seqlens[b]`` of them and ``rows`` in all, as bf16
@@ -86,9 +86,9 @@ class Int8Cache:
         _native.require_one_device(self.k, tables, starts, cu_seqlens)
         k = torch.empty((rows, self.heads, self.dim), dtype=torch.bfloat16, device=self.k.device)
         v = torch.empty_like(k)
-        _native.check(_native.load().reax_kv8_read(
-            *self._cache(), tables.data_ptr(), starts.data_ptr(), cu_seqlens.data_ptr(), k.data_ptr(), v.data_ptr(), rows, batch,
-            width, self.pages, self.heads, self.page, self.dim, _native.stream_handle(self.k.device)))
+        _native.launch(
+            k.device, "reax_kv8_read", *self._cache(), tables.data_ptr(), starts.data_ptr(), cu_seqlens.data_ptr(), k.data_ptr(),
+            v.data_ptr(), rows, batch, width, self.pages, self.heads, self.page, self.dim, _native.stream_handle(k.device))
         return k, v
 
     def attend(self, q, tables, lengths, *, cu_seqlens=None, max_rows=None, scale=None, return_lse=False, out=None):
@@ -112,9 +112,9 @@ class Int8Cache:
         if max_rows is None:
             max_rows = 1 if cu_seqlens is None else n
         ws = _native.kv8_workspace(q.device)
-        _native.check(_native.load().reax_kv8_attend(
-            q.data_ptr(), *self._cache(), tables.data_ptr(), lengths.data_ptr(),
+        _native.launch(
+            q.device, "reax_kv8_attend", q.data_ptr(), *self._cache(), tables.data_ptr(), lengths.data_ptr(),
             None if cu_seqlens is None else cu_seqlens.data_ptr(), out.data_ptr(), None if lse is None else lse.data_ptr(), n,
             max_rows, batch, width, self.pages, self.heads, heads_q // self.heads, self.page, self.dim, ldq,
-            self.dim ** -0.5 if scale is None else scale, ws.data_ptr(), ws.numel(), _native.stream_handle(q.device)))
+            self.dim ** -0.5 if scale is None else scale, ws.data_ptr(), ws.numel(), _native.stream_handle(q.device))
         return (out, lse) if return_lse else out
