@@ -288,10 +288,11 @@ REAX_API size_t reax_kv8_workspace_bytes(int device);
 
 /* Softmax attention of q (bf16 [rows, heads * group, dim], row stride ldq) over the cache.  Sequence b has lengths[b]
  * cached rows, of which its cu_seqlens[b + 1] - cu_seqlens[b] query rows (cu_seqlens NULL: one) are the last: query row
- * i of n sees cached rows 0 .. lengths[b] - n + i.  A row that sees none gives zeros, and -inf in lse.  Query head h
- * reads cached head h / group.  out bf16 [rows, heads * group, dim]; lse float32 [rows, heads * group] (may be NULL):
- * the natural log of the sum of exp(scale q.k).  max_rows: at least the most query rows of a sequence (a hint for the
- * launch; the result does not depend on it).  The workspace (reax_kv8_workspace_bytes(), zeroed once; one for each
+ * i of n sees cached rows 0 .. lengths[b] - n + i.  A row that sees none gives zeros, and -inf in lse.  One that does,
+ * and holds a NaN or an infinity or sees a place of a page whose scale of k or v is one, gives NaN in out and lse; no
+ * other row is touched by it.  Query head h reads cached head h / group.  out bf16 [rows, heads * group, dim]; lse
+ * float32 [rows, heads * group] (may be NULL): the natural log of the sum of exp(scale q.k).  max_rows: at least the
+ * most query rows of a sequence (a hint for the launch; the result does not depend on it).  The workspace (reax_kv8_workspace_bytes(), zeroed once; one for each
  * stream, as the GEMMs') holds the parts of rows whose cache several blocks share. */
 REAX_API int reax_kv8_attend(const void* q, const int8_t* k_codes, const int8_t* v_codes, const float* k_scales,
                              const float* v_scales, const int32_t* tables, const int32_t* lengths,

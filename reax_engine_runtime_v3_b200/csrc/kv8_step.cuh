@@ -13,6 +13,11 @@
 // differ by more than 19, it multiplies such weights in passes of their own, times 2^29 each, and the outputs so far with
 // them: every weight then counts with its 11 bits, down to 2^-115 of the largest.
 //
+// Not finite.  A query row that holds a NaN or an infinity gets NaN as its scale, and so does a page with such a scale of k or v
+// as its scale of k: the scores that either meets are NaN.  The maximum passes over them (it is never NaN) and the weights'
+// comparisons drop them, so the denominator alone carries them to the outputs and the log-sum-exp; 0 is left to rows that
+// see nothing.
+//
 // Loads.  Each warp fetches its own 16 rows of a tile into its own ring with asynchronous 16-byte copies, so that warps never
 // wait for one another but to join their parts, and all registers go to eight warps on an SM.  (A fifth warp for the loads
 // left 168 of 255 registers and the outputs of 256 columns spilled; boxes of 16 rows by TMA cost about 1100 cycles a tile to
@@ -125,6 +130,15 @@ REAX_DEVI float lg2f(float x) {
     return y;
 }
 
+constexpr uint32_t kNanBits = 0x7FFFFFFFu;
+
+// A page's scale of k, NaN where it or the page's scale of v is not finite.
+REAX_DEVI float kv8_score_scale(float k_scale, float v_scale) { return __fmaf_rn(0.0f, v_scale, __fmaf_rn(0.0f, k_scale, k_scale)); }
+// A row's factor from its denominator: 0 where that is (nothing seen), NaN where that is.
+REAX_DEVI float kv8_inverse(float x, float den) { return den == 0.0f ? 0.0f : x / den; }
+// ... and its log-sum-exp.
+REAX_DEVI float kv8_lse(float reference, float den) { return den == 0.0f ? -INFINITY : 0.69314718f * (reference + log2f(den)); }
+
 template <int D>
 __global__ void __launch_bounds__(kAttendStepThreads, kStepBlocksPerSm)
     kv8_step_kernel(const __grid_constant__ Kv8Attend a, const StepWork work) {
@@ -184,7 +198,10 @@ __global__ void __launch_bounds__(kAttendStepThreads, kStepBlocksPerSm)
         id = row < ahead.s.len ? a.tables[static_cast<long long>(ahead.b) * a.table_ld + (row >> shift)] : -1;
     };
     auto put_down = [&]() {
-        if (put >= 0 && lane == 0) sh.meta[put][warp] = float4{ks, lg2f(vs), __fdividef(1.0f, vs), in ? 1.0f : 0.0f};
+        if (put >= 0 && lane == 0) {
+            const float v = fmaxf(vs, 1e-30f);
+            sh.meta[put][warp] = float4{kv8_score_scale(ks, vs), lg2f(v), __fdividef(1.0f, v), in ? 1.0f : 0.0f};
+        }
         put = -1;
     };
     auto load = [&]() {
@@ -195,7 +212,7 @@ __global__ void __launch_bounds__(kAttendStepThreads, kStepBlocksPerSm)
             if (in) {
                 const long long at = static_cast<long long>(id) * heads + ahead.h;
                 ks = a.c.k_scale[at];
-                vs = fmaxf(a.c.v_scale[at], 1e-30f);
+                vs = a.c.v_scale[at];
                 const long long first = ((at << shift) + ((ahead.x * kStepTile + warp * 16) & (page - 1))) * D + lane * 16;
 #pragma unroll
                 for (int e = 0; e < 16 * D; e += 512) {
@@ -235,19 +252,22 @@ __global__ void __launch_bounds__(kAttendStepThreads, kStepBlocksPerSm)
                 const __nv_bfloat16* src = a.q + static_cast<long long>(s.lo + (real ? (at + r) / a.group : 0)) * a.ldq +
                                            (h * a.group + (real ? (at + r) % a.group : 0)) * D;
                 float x[D / 32], m = 0.0f;
+                bool finite = true;
 #pragma unroll
                 for (int i = 0; i < D / 64; ++i) {
                     const uint32_t w = real ? *reinterpret_cast<const uint32_t*>(src + i * 64 + lane * 2) : 0u;
                     x[2 * i] = __uint_as_float(w << 16), x[2 * i + 1] = __uint_as_float(w & 0xFFFF0000u);
                     m = fmaxf(m, fmaxf(fabsf(x[2 * i]), fabsf(x[2 * i + 1])));
+                    finite = finite && fabsf(x[2 * i]) < INFINITY && fabsf(x[2 * i + 1]) < INFINITY;
                 }
                 m = warp_max(m);
+                finite = __all_sync(0xFFFFFFFFu, finite);
                 const uint32_t e = max(__float_as_uint(m) >> 23, 14u);
                 const float f = __uint_as_float((267u - e) << 23);
 #pragma unroll
                 for (int i = 0; i < D / 64; ++i)
                     *reinterpret_cast<__half2*>(&sh.q[r][i * 64 + lane * 2]) = __floats2half2_rn(x[2 * i] * f, x[2 * i + 1] * f);
-                if (lane == 0) sh.q_scale[r] = __uint_as_float((e - 13u) << 23) * a.scale * 1.44269504f;
+                if (lane == 0) sh.q_scale[r] = finite ? __uint_as_float((e - 13u) << 23) * a.scale * 1.44269504f : __uint_as_float(kNanBits);
             }
             __syncthreads();
             const float qs[2] = {sh.q_scale[g], sh.q_scale[g + 8]};
@@ -437,16 +457,16 @@ __global__ void __launch_bounds__(kAttendStepThreads, kStepBlocksPerSm)
                 *d = 0.0f;
 #pragma unroll
                 for (int w = 0; w < 4; ++w)
-                    if (sh.stat[0][w][r] != -INFINITY) *d += sh.stat[1][w][r] * ex2f(sh.stat[0][w][r] - *m);
+                    *d += sh.stat[1][w][r] * (sh.stat[0][w][r] == -INFINITY ? 0.0f : ex2f(sh.stat[0][w][r] - *m));
             };
             auto write_row = [&](int r, float m, float d, const float (&y)[D / 32]) {
                 const int i = (at + r) / a.group, hq = h * a.group + (at + r) % a.group;
                 const long long row = static_cast<long long>(s.lo + i) * heads * a.group + hq;
-                const float inv = d > 0.0f ? 1.0f / d : 0.0f;
+                const float inv = kv8_inverse(1.0f, d);
 #pragma unroll
                 for (int e = 0; e < D / 64; ++e)
                     *reinterpret_cast<uint32_t*>(a.out + row * D + e * 64 + lane * 2) = bf16x2_rn(f2(y[2 * e] * inv, y[2 * e + 1] * inv));
-                if (lane == 0 && a.lse) a.lse[row] = d > 0.0f ? 0.69314718f * (m + log2f(d)) : -INFINITY;
+                if (lane == 0 && a.lse) a.lse[row] = kv8_lse(m, d);
             };
             auto two_columns = [&](int r, int col) {
                 const float2 x = *reinterpret_cast<const float2*>(&sh.o[0][r][step_col(col)]), y = *reinterpret_cast<const float2*>(&sh.o[1][r][step_col(col)]);

@@ -14,6 +14,9 @@
 // beside the conversion's traffic, so q lives in TMEM; O costs another 1000 with both terms).  The softmax's chain from a
 // tile's scores to its weights takes 2600, the codes' conversion 2500.  The roles overlap.
 //
+// Values that are not finite go as in the step form: a NaN as the scale of the row or of the page's scores, carried to the
+// outputs by the denominator.
+//
 // Scaling O (in TMEM) costs as much as a tile, so the reference that the exponents are taken from moves only when a maximum
 // exceeds it by 8 (in log2): weights stay below 2^8, which bf16 holds as well as any.
 //
@@ -266,8 +269,10 @@ __global__ void __launch_bounds__(kAttendTileThreads, 1)
 #pragma unroll
                 for (int e = 0; e < D / 16; ++e)
                     top = __vmaxu2(__vmaxu2(top, y[e].x & 0x7FFF7FFFu), __vmaxu2(y[e].y & 0x7FFF7FFFu, __vmaxu2(y[e].z & 0x7FFF7FFFu, y[e].w & 0x7FFF7FFFu)));
-                const float2 f = scale_of(row_max(__uint_as_float(max(top & 0xFFFFu, top >> 16) << 16)));
-                scale *= f.y;
+                // (a NaN counts as an infinity, which the maximum keeps)
+                const float most = row_max(__uint_as_float(min(max(top & 0xFFFFu, top >> 16), 0x7F80u) << 16));
+                const float2 f = scale_of(most);
+                scale = most < INFINITY ? scale * f.y : __uint_as_float(kNanBits);
 #pragma unroll
                 for (int e = 0; e < D / 16; e += 4) {
                     uint32_t w[16];
@@ -303,7 +308,7 @@ __global__ void __launch_bounds__(kAttendTileThreads, 1)
                     in[e] = id[e] >= 0 && id[e] < a.c.pages;
                     const long long scales = static_cast<long long>(in[e] ? id[e] : 0) * heads + at.h;
                     ks[e] = in[e] ? a.c.k_scale[scales] : 0.0f;
-                    vs[e] = in[e] ? fmaxf(a.c.v_scale[scales], 1e-30f) : 1.0f;
+                    vs[e] = in[e] ? a.c.v_scale[scales] : 1.0f;
                 }
             };
             look_up(at.x);
@@ -311,7 +316,8 @@ __global__ void __launch_bounds__(kAttendTileThreads, 1)
             look_up(at.x + 1);
 #pragma unroll 1
             for (int x = at.x; x < to; ++x, ++t0) {
-                const float f[2] = {ks[0] * scale, ks[1] * scale}, inv[2] = {__fdividef(1.0f, vs[0]), __fdividef(1.0f, vs[1])}, add[2] = {lg2f(vs[0]), lg2f(vs[1])};
+                const float v[2] = {fmaxf(vs[0], 1e-30f), fmaxf(vs[1], 1e-30f)}, inv[2] = {__fdividef(1.0f, v[0]), __fdividef(1.0f, v[1])};
+                const float f[2] = {kv8_score_scale(ks[0], vs[0]) * scale, kv8_score_scale(ks[1], vs[1]) * scale}, add[2] = {lg2f(v[0]), lg2f(v[1])};
                 const bool plain = in[0] && in[1] && x * kTileCols + half * 32 + 32 <= least;
                 const bool have[2] = {in[0], in[1]};
                 fetch();
@@ -410,7 +416,7 @@ __global__ void __launch_bounds__(kAttendTileThreads, 1)
                     work.rest[blockIdx.x] = {seq.lo, first, live, at.h, static_cast<int>((at.end * blocks - 1) / all) - static_cast<int>(blockIdx.x) + 1};
                 }
             } else {
-                const float scale_out = den > 0.0f ? kCodeUp / den : 0.0f;
+                const float scale_out = kv8_inverse(kCodeUp, den);
                 const int i = first + r;
                 const long long row = (static_cast<long long>(seq.lo) + i / a.group) * heads * a.group + at.h * a.group + i % a.group;
 #pragma unroll 2
@@ -425,7 +431,7 @@ __global__ void __launch_bounds__(kAttendTileThreads, 1)
                         *reinterpret_cast<uint4*>(a.out + row * D + e + 8) = uint4{w[4], w[5], w[6], w[7]};
                     }
                 }
-                if (a.lse && half == 0 && r < live) a.lse[row] = den > 0.0f ? 0.69314718f * (ref + log2f(den)) : -INFINITY;
+                if (a.lse && half == 0 && r < live) a.lse[row] = kv8_lse(ref, den);
             }
             if (!at.next(a, u1)) break;
         }
@@ -645,7 +651,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv8_join_kernel(const __grid_con
 #pragma unroll
             for (int e = 0; e < kJoinCols; ++e) o[e] = o[e] * f0 + xch[warp + w][2 + e][lane] * f1;
         }
-        const float scale = den > 0.0f ? kCodeUp / den : 0.0f;
+        const float scale = kv8_inverse(kCodeUp, den);
         const int y = rest.first + r;
         const long long row = (static_cast<long long>(rest.lo) + y / a.group) * a.c.heads * a.group + rest.h * a.group + y % a.group;
         uint32_t w[8];
@@ -653,7 +659,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv8_join_kernel(const __grid_con
         for (int e = 0; e < 8; ++e) w[e] = bf16x2_rn(f2(o[2 * e] * scale, o[2 * e + 1] * scale));
         *reinterpret_cast<uint4*>(a.out + row * D + col) = uint4{w[0], w[1], w[2], w[3]};
         *reinterpret_cast<uint4*>(a.out + row * D + col + 8) = uint4{w[4], w[5], w[6], w[7]};
-        if (a.lse && col == 0) a.lse[row] = den > 0.0f ? 0.69314718f * (top + log2f(den)) : -INFINITY;
+        if (a.lse && col == 0) a.lse[row] = kv8_lse(top, den);
     }
 }
 
