@@ -292,8 +292,10 @@ REAX_API size_t reax_kv8_workspace_bytes(int device);
  * and holds a NaN or an infinity or sees a place of a page whose scale of k or v is one, gives NaN in out and lse; no
  * other row is touched by it.  Query head h reads cached head h / group.  out bf16 [rows, heads * group, dim]; lse
  * float32 [rows, heads * group] (may be NULL): the natural log of the sum of exp(scale q.k).  max_rows: at least the
- * most query rows of a sequence (a hint for the launch; the result does not depend on it).  The workspace (reax_kv8_workspace_bytes(), zeroed once; one for each
- * stream, as the GEMMs') holds the parts of rows whose cache several blocks share. */
+ * most query rows of a sequence (a hint for the launch; the result does not depend on it).
+ * The workspace (reax_kv8_workspace_bytes(), zeroed once) holds the parts of rows whose cache several blocks share.
+ * Calls that can run at the same time have one each: one for each stream, and one for each captured graph.  Calls that are
+ * captured need not find it zeroed. */
 REAX_API int reax_kv8_attend(const void* q, const int8_t* k_codes, const int8_t* v_codes, const float* k_scales,
                              const float* v_scales, const int32_t* tables, const int32_t* lengths,
                              const int32_t* cu_seqlens, void* out, float* lse, int rows, int max_rows, int batch,

@@ -169,8 +169,22 @@ def _stream_workspace(device: torch.device, kind: str) -> torch.Tensor:
     return ws
 
 
+def _capturing(device: torch.device) -> bool:
+    """Whether the stream that is current on `device` is being captured."""
+    if device.index == torch.cuda.current_device():
+        return torch.cuda.is_current_stream_capturing()
+    with torch.cuda.device(device):
+        return torch.cuda.is_current_stream_capturing()
+
+
 def kv8_workspace(device: torch.device) -> torch.Tensor:
-    """Zero-initialised workspace of the attention over the INT8 cache for (device, current stream)."""
+    """Workspace of the attention over the INT8 cache: zero-initialised, one for each (device, current stream).
+
+    A captured call gets memory of its graph instead (a captured call clears the counters itself): graphs captured on one
+    stream may be replayed on several, in any order and beside calls on the stream that captured them.
+    """
+    if _capturing(device):
+        return torch.empty(load().reax_kv8_workspace_bytes(device.index), dtype=torch.uint8, device=device)
     return _stream_workspace(device, "reax_kv8_workspace_bytes")
 
 

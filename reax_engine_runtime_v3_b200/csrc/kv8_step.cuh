@@ -130,6 +130,12 @@ REAX_DEVI float lg2f(float x) {
     return y;
 }
 
+// Clears the counters before a step whose workspace may hold anything; the step, a dependent launch, waits for it.
+__global__ void __launch_bounds__(kAttendStepThreads) kv8_clear_kernel(const StepWork work, int blocks) {
+    asm volatile("griddepcontrol.launch_dependents;");
+    for (int i = threadIdx.x; i < blocks; i += kAttendStepThreads) work.counters[i] = 0;
+}
+
 constexpr uint32_t kNanBits = 0x7FFFFFFFu;
 
 // A page's scale of k, NaN where it or the page's scale of v is not finite.
@@ -161,7 +167,10 @@ __global__ void __launch_bounds__(kAttendStepThreads, kStepBlocksPerSm)
     for (int i = 0; i < kAttendStepThreads / 32; ++i) total += sh.sum[i];
     const long long each = max((total + gridDim.x - 1) / gridDim.x, 2ll);
     const long long u0 = min(each * blockIdx.x, total), u1 = min(u0 + each, total);
-    if (u0 >= u1) return;
+    if (u0 >= u1) {
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        return;
+    }
     // the tile u0 (each warp looks for itself)
     StepCursor at_u;
     long long u = u0, start = 0;              // start: tiles of the sequences before
@@ -230,6 +239,7 @@ __global__ void __launch_bounds__(kAttendStepThreads, kStepBlocksPerSm)
     look_up();
 #pragma unroll 1
     for (int i = 0; i < kStages; ++i) load();
+    asm volatile("griddepcontrol.wait;" ::: "memory");        // the counters are clear (what comes before that, comes before the inputs)
     put_down();
     __syncwarp();
 
