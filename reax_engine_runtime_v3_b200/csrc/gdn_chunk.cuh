@@ -23,6 +23,11 @@
 // have 8 bits and are exact in one.  X_k, V' and D, which the state depends on, take all terms down to 2^-22; X_q and Y
 // only reach the bf16 output and take the hi terms.  Sums are float32.
 //
+// Not finite.  The products run over whole chunks, where 0 times NaN would reach the rows before.  So the first kernel finds a
+// chunk's first row whose k, g or beta is not finite, leaves the rows from there on out of T (as if their beta were 0) and
+// marks them in c_x; the second takes R of the rows from a column's first that is not finite on as 0 (by the mark, by v or by
+// the state) and puts NaN into the outputs and the state that follow from it.  A q that is not finite stays in its row.
+//
 // Two kernels.  What a chunk needs that does not depend on the state (k and q as fp16 tiles, T, P and the rows' factors) is
 // found by gdn_tiles_kernel for all chunks at once, a block of four warps for each chunk and key head, and kept in scratch
 // memory; gdn_chunk_kernel then carries the states along, a block for each sequence and value head, which reads those tiles
@@ -51,6 +56,7 @@ constexpr int kTilesThreads = 4 * 32;
 constexpr int kKqSlots = 3;                   // chunks of k and q tiles in flight
 constexpr int kGdnSorted = 256;               // sequences up to which blocks take them in the order of their lengths
 constexpr float kGdnDown = 0x1p-20f, kGdnUp = 0x1p20f;
+constexpr uint32_t kGdnNan = 0x7FFFFFFFu;
 
 // TMEM columns.  S hi and lo (64 each) share the columns of D, and the decayed V' hi and lo those of X_k, V' hi those of R:
 // each is written after the other has been read.
@@ -90,6 +96,7 @@ struct GdnTilesShared {
     float a11[32 * 32], a22[32 * 32];         // -A's diagonal blocks; 16-byte pieces of a row xor-ed with row % 8
     float g_hi[4][kChunk], g_lo[4][kChunk], beta[4][kChunk];   // of four value heads: G in log2, as hi + lo
     float row_k[kChunk], row_q[kChunk];       // scales of the rows of k and q
+    int bad_k[2], bad[4];                     // first row of k (of either half) and of four value heads that is not finite, or 64
     uint64_t kk_done, z_done, drained[2];
     uint32_t tmem;
     uint32_t abort;
@@ -229,6 +236,13 @@ REAX_DEVI void split2(uint64_t x, uint64_t f, uint32_t& hi, uint32_t& lo) {
 }
 REAX_DEVI uint32_t half2_of(uint64_t x) { return half2_bits(f2_lo(x), f2_hi(x)); }
 REAX_DEVI float max3(float m, uint64_t x) { return fmaxf(m, fmaxf(fabsf(f2_lo(x)), fabsf(f2_hi(x)))); }
+// ... that a NaN is not lost in.
+REAX_DEVI float max3_nan(float m, uint64_t x) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(fabsf(f2_lo(x))), "f"(fabsf(f2_hi(x))));
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(m), "f"(y));
+    return y;
+}
 
 REAX_DEVI uint64_t u2(uint32_t lo, uint32_t hi) { return (static_cast<uint64_t>(hi) << 32) | lo; }
 REAX_DEVI void tmem_st_x8(uint32_t taddr, const uint32_t (&r)[8]) {
@@ -309,6 +323,7 @@ __global__ void __launch_bounds__(kTilesThreads, 4) gdn_tiles_kernel(const __gri
         // row's number turns, so that the eight lanes of a shared-memory pass meet all banks.
         constexpr int kPieces = DK / 8, kTurns = kPieces / 4;
         const int r8 = lane / 4;
+        int bad = kChunk;
         uint4 raw[4][kTurns];
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
@@ -334,6 +349,10 @@ __global__ void __launch_bounds__(kTilesThreads, 4) gdn_tiles_kernel(const __gri
             float sq = f2_lo(sum[0]) + f2_hi(sum[0]);
             sq += __shfl_xor_sync(0xFFFFFFFFu, sq, 1);
             sq += __shfl_xor_sync(0xFFFFFFFFu, sq, 2);
+            // a row of k that is not finite (its sum of squares is not) is left out
+            const bool out_of_k = warp < 2 && !(sq < INFINITY);
+            const unsigned who = __ballot_sync(0xFFFFFFFFu, out_of_k);
+            if (who) bad = min(bad, warp * 32 + u * 8 + (__ffs(who) - 1) / 4);
             // 2^(k - 1) <= norm < 2^k
             const int k = static_cast<int>((max(__float_as_uint(sq) >> 23, 7u) + 1) >> 1) - 63;
             const float f = __uint_as_float(static_cast<uint32_t>(127 + 14 - k) << 23);
@@ -342,14 +361,16 @@ __global__ void __launch_bounds__(kTilesThreads, 4) gdn_tiles_kernel(const __gri
 #pragma unroll
             for (int x = 0; x < kTurns; ++x) {
                 const int at = ((x + r8) % kTurns) * 4 + lane % 4;
+                if (out_of_k) raw[u][x] = uint4{};
                 const uint32_t y[4] = {raw[u][x].x, raw[u][x].y, raw[u][x].z, raw[u][x].w};
                 uint32_t o[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) o[j] = half2_of(mul2_rn(bf16x2_to_f2(y[j]), f2(f, f)));
                 *reinterpret_cast<uint4*>(sh.kq[at / 8] + r * 128 + ((at % 8) ^ r8) * 16) = uint4{o[0], o[1], o[2], o[3]};
             }
-            if (lane % 4 == 0) (r < 64 ? sh.row_k : sh.row_q - 64)[r] = r % 64 >= left ? 0.0f : r < 64 ? back : back * p.scale;
+            if (lane % 4 == 0) (r < 64 ? sh.row_k : sh.row_q - 64)[r] = r % 64 >= left || out_of_k ? 0.0f : r < 64 ? back : back * p.scale;
         }
+        if (warp < 2 && lane == 0) sh.bad_k[warp] = bad;
         fence_proxy_async_smem();
     }
     tc_fence_before();
@@ -388,13 +409,23 @@ __global__ void __launch_bounds__(kTilesThreads, 4) gdn_tiles_kernel(const __gri
             // so that differences of far running sums keep their low bits; decays below 2^-128 count as 0
             if (head > 0) __syncthreads();
             if (head + warp < heads) {
-                float hi[2], lo[2], be[2];
+                float hi[2], lo[2], be[2], y[2];
+                int bad = min(sh.bad_k[0], sh.bad_k[1]);
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     const bool real = lane * 2 + j < left;
                     const long long at = (static_cast<long long>(r0) + (real ? lane * 2 + j : 0)) * p.v_heads + hk * group + head0 + head + warp;
-                    const float y = real ? p.g[at] * 1.44269504f : 0.0f, x = y < -128.0f ? -128.0f : y;
+                    y[j] = real ? p.g[at] * 1.44269504f : 0.0f;
                     be[j] = real ? p.beta[at] : 0.0f;
+                    // (a decay of e^-inf is finite)
+                    const unsigned who = __ballot_sync(0xFFFFFFFFu, !(y[j] < 128.0f) || !(fabsf(be[j]) < INFINITY));
+                    if (who) bad = min(bad, 2 * (__ffs(who) - 1) + j);
+                }
+                if (lane == 0) sh.bad[warp] = bad;
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    if (lane * 2 + j >= bad) y[j] = be[j] = 0.0f;
+                    const float x = y[j] < -128.0f ? -128.0f : y[j];
                     hi[j] = rintf(x * 256.0f) * 0.00390625f;
                     lo[j] = x - hi[j];
                 }
@@ -542,7 +573,7 @@ __global__ void __launch_bounds__(kTilesThreads, 4) gdn_tiles_kernel(const __gri
 #pragma unroll
             for (int j = 0; j < 16; ++j) m = max3(max3(m, z[j]), z1[j]);
             const float2 f = scale_of(m);
-            st.c_x[i] = -row_k * beta * ex2(g_hi + g_lo);
+            st.c_x[i] = i >= sh.bad[head % 4] ? __uint_as_float(kGdnNan) : -row_k * beta * ex2(g_hi + g_lo);
             st.c_b[i] = beta;
             st.c_v[i] = row_k * ex2((g_hi_s[kChunk - 1] - g_hi) + (g_lo_s[kChunk - 1] - g_lo)) * f.y;
             st.c_u[i] = row_k * f.y;
@@ -680,6 +711,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) gdn_chunk_kernel(const __gri
         auto pair_of = [](const float* f) { return *reinterpret_cast<const uint64_t*>(f); };
         const uint16_t* vcol = reinterpret_cast<const uint16_t*>(sh.v[0]) + part * 32 * DV + (n < DV ? n : 0);
         float sq = 0.0f, sv = 0.0f;          // scales of the S behind X_q and the V' behind Y
+        int bad = kChunk;                     // the chunk's first row whose R is not finite in this column
 #pragma unroll 1
         for (int c = 0;; ++c) {                // (c counts from the first chunk of this launch)
             const uint32_t par = c & 1;
@@ -728,6 +760,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1) gdn_chunk_kernel(const __gri
                 }
                 tc_fence_before();
                 arrive(&sh.tiles_free[par ^ 1]);
+#pragma unroll 1
+                for (int i = max(bad - part * 32, 0); i < 32; ++i) o[i * 32] = kGdnNan >> 16;
+                __syncwarp();
                 const int row = (c - 1) * kChunk + part * 32, left = rows - row;
                 if (quarter * 32 < DV) {
                     if (left >= 32) {
@@ -772,8 +807,26 @@ __global__ void __launch_bounds__(kChunkThreads, 1) gdn_chunk_kernel(const __gri
                     }
                 arrive(&sh.v_free[par]);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) m = max3(m, r[i]);
-                const float2 rs = scale_of(row_max(m));
+                for (int i = 0; i < 16; ++i) m = max3_nan(m, r[i]);
+                float most = row_max(m < INFINITY ? m : INFINITY);
+                bad = kChunk;
+                if (__any_sync(0xFFFFFFFFu, most == INFINITY)) {      // (in both warps of a quarter)
+#pragma unroll
+                    for (int i = 15; i >= 0; --i) {
+                        if (!(fabsf(f2_hi(r[i])) < INFINITY)) bad = part * 32 + 2 * i + 1;
+                        if (!(fabsf(f2_lo(r[i])) < INFINITY)) bad = part * 32 + 2 * i;
+                    }
+                    bad = kChunk - static_cast<int>(row_max(static_cast<float>(kChunk - bad)));
+                    m = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const int at = part * 32 + 2 * i;
+                        r[i] = f2(at < bad ? f2_lo(r[i]) : 0.0f, at + 1 < bad ? f2_hi(r[i]) : 0.0f);
+                        m = max3(m, r[i]);
+                    }
+                    most = row_max(m);
+                }
+                const float2 rs = scale_of(most);
                 sv = rs.y;
 #pragma unroll
                 for (int e = 0; e < 16; e += 8) {
@@ -823,7 +876,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) gdn_chunk_kernel(const __gri
             tc_fence_before();
             arrive(&sh.v_ready);
             // (R's scale is that of V' until here)
-            const float back = vs.y * sv, gamma = st.gamma;
+            const float back = vs.y * sv, gamma = bad < kChunk ? __uint_as_float(kGdnNan) : st.gamma;
             sv *= us.y;
             // D -> S
 #pragma unroll
