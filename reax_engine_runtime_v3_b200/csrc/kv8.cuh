@@ -257,6 +257,7 @@ struct Kv8Attend {
     __nv_bfloat16* out;       // [rows, heads * group, dim]
     float* lse;               // [rows, heads * group] or NULL
     int rows, batch, table_ld, group;
+    int capacity;             // rows that a table has places for, at most 2^31 - 64
     float scale;
 };
 

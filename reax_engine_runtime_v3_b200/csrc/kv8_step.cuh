@@ -68,7 +68,7 @@ struct StepSeq {
         int hi;
         kv8_span(a.cu, b, a.rows, &lo, &hi);
         rows = hi - lo;
-        len = min(max(a.lengths[b], 0), a.table_ld * a.c.page);
+        len = min(max(a.lengths[b], 0), a.capacity);
         tiles = max((len + kStepTile - 1) / kStepTile, 1);
         items = (rows * a.group + kStepRows - 1) / kStepRows;
     }

@@ -95,7 +95,7 @@ struct TileSeq {
         kv8_span(a.cu, b, a.rows, &lo, &hi);
         rows = hi - lo;
         const int all = max(a.lengths[b], 0);
-        len = min(all, a.table_ld * a.c.page);
+        len = min(all, a.capacity);
         before = all - rows;
         items = (rows * a.group + kTileRows - 1) / kTileRows;
     }

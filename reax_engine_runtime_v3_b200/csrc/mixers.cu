@@ -314,10 +314,11 @@ int reax_kv8_attend(const void* q, const int8_t* k_codes, const int8_t* v_codes,
                     void* out, float* lse, int rows, int max_rows, int batch, int table_ld, int pages, int heads, int group,
                     int page, int dim, long long ldq, float scale, void* workspace, size_t workspace_bytes, void* stream) {
     const char* who = "reax_kv8_attend";
+    const int capacity = static_cast<int>(std::min(std::max(table_ld, 0) * static_cast<long long>(page), 0x7FFFFFC0ll));
     const reax::Kv8Attend a = {{const_cast<int8_t*>(k_codes), const_cast<int8_t*>(v_codes), const_cast<float*>(k_scales),
                                 const_cast<float*>(v_scales), pages, heads, page, dim},
                                static_cast<const __nv_bfloat16*>(q), ldq, tables, lengths, cu_seqlens,
-                               static_cast<__nv_bfloat16*>(out), lse, rows, batch, table_ld, group, scale};
+                               static_cast<__nv_bfloat16*>(out), lse, rows, batch, table_ld, group, capacity, scale};
     int rc = check_rows(who, tables, lengths, cu_seqlens, rows, batch, table_ld), sms = 0;
     if (rc != REAX_OK || rows == 0 || batch == 0) return rc;
     if ((rc = check_cache(who, a.c)) != REAX_OK) return rc;
