@@ -258,9 +258,9 @@ REAX_API int reax_gdn_decode(const void* q, const void* k, const void* v, const 
                              int Dv, int n_slots, long long ldq, long long ldk, long long ldv, float scale,
                              int normalize, void* stream);
 
-/* Status word of the gated delta rule's prompt form on the current device, after the work queued on `stream` so far (this
- * call synchronizes `stream`): 0, or the REAX_STATUS_* bits of waits inside its kernels that expired, whose outputs are
- * then invalid.  `clear` != 0 clears it after reading. */
+/* Status word of the gated delta rule's prompt form and of reax_kv8_attend for many rows on the current device, after the
+ * work queued on `stream` so far (this call synchronizes `stream`): 0, or the REAX_STATUS_* bits of waits inside their
+ * kernels that expired (reax_set_wait_timeout_ns, here at most 4 s), whose outputs are then invalid.  `clear` != 0 clears it after reading. */
 REAX_API int reax_mixer_status(unsigned* status, int clear, void* stream);
 
 /* ---- paged INT8 cache of keys and values ------------------------------------------------------------------
