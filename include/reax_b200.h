@@ -234,9 +234,9 @@ REAX_API int reax_sliced_i8_static(const int8_t* A, const int8_t* W, const void*
  * place; out bf16 [rows, v_heads, Dv].  Sequence b keeps its state in slot slots[b] (int32 [batch]; NULL: b); a
  * slot outside [0, n_slots) marks a sequence that keeps none: its outputs are zeros.  No two sequences of a call
  * may share a slot.  Dk and Dv are 64 or 128 each.
- * A value that is not finite touches no row before its own: one in q makes its row's outputs NaN; one in k (or a sum of a
- * row's squares above float32), g (-infinity aside: a decay to 0) or beta makes the head's outputs from its row on and the
- * state not finite, one in v or the state those of its column.
+ * A value that is not finite touches no row before its own: one in q makes its row's outputs NaN; one in k, g (-infinity
+ * aside: a decay to 0) or beta makes the head's outputs from its row on and the state not finite, one in v or the state
+ * those of its column.  With `normalize` a row of q or k whose sum of squares passes float32 counts as not finite.
  *
  * reax_gdn_prefill: sequence b has rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1 (int32 [batch + 1] on the device;
  * NULL: one sequence of all rows); one without rows keeps its state as it is, or gets zeros when `carry` is 0.
@@ -260,7 +260,8 @@ REAX_API int reax_gdn_decode(const void* q, const void* k, const void* v, const 
 
 /* Status word of the gated delta rule's prompt form and of reax_kv8_attend for many rows on the current device, after the
  * work queued on `stream` so far (this call synchronizes `stream`): 0, or the REAX_STATUS_* bits of waits inside their
- * kernels that expired (reax_set_wait_timeout_ns, here at most 4 s), whose outputs are then invalid.  `clear` != 0 clears it after reading. */
+ * kernels that expired (reax_set_wait_timeout_ns, here at most 4 s), whose outputs are then invalid.  `clear` != 0 clears
+ * it after reading. */
 REAX_API int reax_mixer_status(unsigned* status, int clear, void* stream);
 
 /* ---- paged INT8 cache of keys and values ------------------------------------------------------------------

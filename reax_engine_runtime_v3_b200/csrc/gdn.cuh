@@ -33,6 +33,9 @@ REAX_DEVI float warp_sum(float v) {
     return v;
 }
 
+// What a row with that sum of squares is multiplied by to be normalized: NaN, not 0, where the sum passes float32.
+REAX_DEVI float gdn_rsqrt(float sum) { return rsqrtf(__fmaf_rn(0.0f, sum, sum + kGdnNormEps)); }
+
 // State slot of sequence b, or -1 for one that keeps none (its outputs are zeros).
 REAX_DEVI int gdn_slot(const GdnParams& p, int b) {
     const int s = p.slots ? p.slots[b] : b;
@@ -93,8 +96,8 @@ __global__ void __launch_bounds__(kStepThreads) gdn_step_kernel(const GdnParams 
     float qq = 0, kk = 0, qk = 0;
 #pragma unroll
     for (int i = 0; i < DK / 32; ++i) qq += s_red[0][i], kk += s_red[1][i], qk += s_red[2][i];
-    const float rq = p.normalize ? p.scale * rsqrtf(qq + kGdnNormEps) : p.scale;
-    const float rk = p.normalize ? rsqrtf(kk + kGdnNormEps) : 1.0f;
+    const float rq = p.normalize ? p.scale * gdn_rsqrt(qq) : p.scale;
+    const float rk = p.normalize ? gdn_rsqrt(kk) : 1.0f;
     const float decay = expf(p.g[at]), beta = p.beta[at];
     const uint2 vw = *reinterpret_cast<const uint2*>(p.v + b * p.ldv + hv * DV + c * 4);
     __syncthreads();

@@ -113,3 +113,22 @@ def test_several_rows_and_heads():
     bad = torch.zeros_like(fine)
     bad[0, 0, :, 3] = bad[0, 0, :, 4] = bad[0, 3] = True
     assert torch.equal(fine, ~bad)
+
+
+@pytest.mark.parametrize("form", ["prefill", "decode"])
+def test_rows_whose_squares_pass_float32(form):
+    """Normalizing such a row must not turn it into zeros: its outputs, and of k the state, are not finite."""
+    from reax_engine_runtime_v3_b200 import gated_delta
+    x = inputs(37, 3, 2, 2, D, D, 3)
+    x[0][0, 0] *= 2.0 ** 70
+    x[1][1, 1] *= 2.0 ** 70
+    on = [t.cuda() for t in x]
+    if form == "decode":
+        out = gated_delta.decode(*on)
+    else:
+        out = gated_delta.prefill(*on, cu_seqlens=torch.arange(4, dtype=torch.int32).cuda())
+    out, state = out.cpu().isfinite(), on[5].cpu().isfinite()
+    for fine, row, head in ((out, 0, 0), (out, 1, 1), (state, 1, 1)):
+        assert not fine[row, head].any()
+        fine[row, head] = True
+    assert out.all() and state.all()
