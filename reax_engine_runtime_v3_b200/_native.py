@@ -93,15 +93,20 @@ def check(status: int) -> None:
         raise RuntimeError(f"REAX B200 status {status} ({ERRORS.get(status, 'unknown')}): {message}")
 
 
-def launch(device: torch.device, entry: str, *args) -> None:
-    """Call an entry with the tensors' device current (the library launches on the current one) and check its status.
-    The device is switched only where it has to be: a switch and back costs as much as a small launch."""
-    fn = getattr(load(), entry)
-    if device.index == torch.cuda.current_device():
-        check(fn(*args))
-    else:
-        with torch.cuda.device(device):
-            check(fn(*args))
+# The current device, and the handle of the stream that is current on a device, without what torch's own functions do around
+# them: a Stream object takes longer to make than a small launch.
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def launch(index: int, entry: str, *args) -> None:
+    """Call an entry whose last argument is the stream with device `index` current (the library launches on the current one)
+    and that device's current stream, and check its status.  The device is switched only where it has to be: a switch and
+    back costs as much as a small launch."""
+    if index != _current_device():
+        with torch.cuda.device(index):
+            return launch(index, entry, *args)
+    check(getattr(load(), entry)(*args, _raw_stream(index)))
 
 
 def ptr(t: torch.Tensor | None) -> int | None:
@@ -111,13 +116,10 @@ def ptr(t: torch.Tensor | None) -> int | None:
     return t.data_ptr()
 
 
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-
-
 def stream_handle(device: torch.device | None = None) -> int:
     """The current torch stream, as the reference passes it to cuLaunchKernel (reaxv2/gate_up.py:25-26)."""
-    if _raw_stream is not None and device is not None and device.index is not None:
-        return _raw_stream(device.index)      # the handle alone: a Stream object takes longer to make than a small launch
+    if device is not None and device.index is not None:
+        return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
 
 
@@ -139,13 +141,14 @@ def require_cuda(*tensors: torch.Tensor) -> None:
             raise RuntimeError("REAX B200 kernels take CUDA tensors only (no CPU path)")
 
 
-def require_one_device(*tensors: torch.Tensor) -> None:
-    """All tensors (None aside) on one GPU."""
+def require_one_device(*tensors: torch.Tensor) -> int:
+    """All tensors (None aside) on one GPU, whose index is returned."""
     index = tensors[0].get_device()
     for t in tensors:
         if t is not None and (t.get_device() != index or index < 0):
             require_cuda(*tensors)
             raise RuntimeError("REAX B200 kernels take tensors of one device")
+    return index
 
 
 # ------------------------------------------------------------------------------------------------------ workspace
@@ -171,7 +174,7 @@ def _stream_workspace(device: torch.device, kind: str) -> torch.Tensor:
 
 def _capturing(device: torch.device) -> bool:
     """Whether the stream that is current on `device` is being captured."""
-    if device.index == torch.cuda.current_device():
+    if device.index == _current_device():
         return torch.cuda.is_current_stream_capturing()
     with torch.cuda.device(device):
         return torch.cuda.is_current_stream_capturing()
@@ -214,10 +217,8 @@ def noalloc_status(clear: bool = False) -> int:
 def mixer_status(clear: bool = False, device: torch.device | None = None) -> int:
     """Status word of the gated delta rule's prompt form and the attention of many rows on `device` (the current one if not
     given), after the work of the stream that is current there (synchronizes it); non-zero means a bounded wait expired."""
-    if device is None:
-        device = torch.device("cuda", torch.cuda.current_device())
     v = C.c_uint(0)
-    launch(device, "reax_mixer_status", C.byref(v), 1 if clear else 0, stream_handle(device))
+    launch(torch.cuda.current_device() if device is None else device.index, "reax_mixer_status", C.byref(v), 1 if clear else 0)
     return int(v.value)
 
 

@@ -30,7 +30,7 @@ def _rows(x, name):
 
 def _check(q, k, v, g, beta, state, slots, out, batch):
     """The checks that both forms share: shapes, types and layouts the kernels take.  Returns the output, the row strides
-    of q, k and v and the sizes."""
+    of q, k and v, the sizes and the device."""
     n, k_heads, dk = q.shape
     n_v, v_heads, dv = v.shape
     assert k.shape == q.shape and n_v == n, "q, k [rows, k_heads, Dk] and v [rows, v_heads, Dv] disagree"
@@ -53,8 +53,8 @@ def _check(q, k, v, g, beta, state, slots, out, batch):
     else:
         assert out.dtype is torch.bfloat16 and out.shape == v.shape and out.is_contiguous(), \
             "out is contiguous bf16 [rows, v_heads, Dv]"
-    _native.require_one_device(q, k, v, g, beta, state, slots, out)
-    return out, strides, (k_heads, v_heads, dk, dv, n_slots)
+    index = _native.require_one_device(q, k, v, g, beta, state, slots, out)
+    return out, strides, (k_heads, v_heads, dk, dv, n_slots), index
 
 
 def prefill(q, k, v, g, beta, state, *, cu_seqlens=None, slots=None, carry=True, scale=None, normalize=True, out=None):
@@ -64,7 +64,7 @@ def prefill(q, k, v, g, beta, state, *, cu_seqlens=None, slots=None, carry=True,
     ``normalize``: divide q and k by the root of their sum of squares first; ``scale`` is Dk ** -0.5 if not given.
     Returns out bf16 [rows, v_heads, Dv]; the states are updated in place."""
     batch = 1 if cu_seqlens is None else cu_seqlens.shape[0] - 1
-    out, strides, sizes = _check(q, k, v, g, beta, state, slots, out, batch)
+    out, strides, sizes, index = _check(q, k, v, g, beta, state, slots, out, batch)
     if cu_seqlens is not None:
         assert cu_seqlens.dtype is torch.int32 and cu_seqlens.dim() == 1 and cu_seqlens.is_contiguous(), \
             "cu_seqlens is contiguous int32"
@@ -73,19 +73,19 @@ def prefill(q, k, v, g, beta, state, *, cu_seqlens=None, slots=None, carry=True,
     size = _native.load().reax_gdn_workspace_bytes(q.shape[0], batch, sizes[0], sizes[1], sizes[2])
     scratch = torch.empty(size, dtype=torch.uint8, device=q.device)
     _native.launch(
-        q.device, "reax_gdn_prefill", q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), state.data_ptr(),
+        index, "reax_gdn_prefill", q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), state.data_ptr(),
         None if cu_seqlens is None else cu_seqlens.data_ptr(), None if slots is None else slots.data_ptr(), out.data_ptr(),
         q.shape[0], batch, *sizes, *strides, sizes[2] ** -0.5 if scale is None else scale, normalize, carry,
-        scratch.data_ptr(), size, _native.stream_handle(q.device))
+        scratch.data_ptr(), size)
     return out
 
 
 def decode(q, k, v, g, beta, state, *, slots=None, scale=None, normalize=True, out=None):
     """One row of each sequence, from the states kept: arguments and result as ``prefill``, row b is sequence b's."""
     n = q.shape[0]
-    out, strides, sizes = _check(q, k, v, g, beta, state, slots, out, n)
+    out, strides, sizes, index = _check(q, k, v, g, beta, state, slots, out, n)
     _native.launch(
-        q.device, "reax_gdn_decode", q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), state.data_ptr(),
+        index, "reax_gdn_decode", q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), state.data_ptr(),
         None if slots is None else slots.data_ptr(), out.data_ptr(), n, *sizes, *strides,
-        sizes[2] ** -0.5 if scale is None else scale, normalize, _native.stream_handle(q.device))
+        sizes[2] ** -0.5 if scale is None else scale, normalize)
     return out

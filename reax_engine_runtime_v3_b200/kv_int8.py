@@ -72,23 +72,23 @@ class Int8Cache:
         n = k.shape[0]
         assert n == v.shape[0], "k and v have the same rows"
         batch, width = self._sequences(tables, lengths, cu_seqlens, n, "lengths")
-        _native.require_one_device(self.k, k, v, tables, lengths, cu_seqlens)
+        index = _native.require_one_device(self.k, k, v, tables, lengths, cu_seqlens)
         _native.launch(
-            k.device, "reax_kv8_append", k.data_ptr(), v.data_ptr(), *self._cache(), tables.data_ptr(), lengths.data_ptr(),
+            index, "reax_kv8_append", k.data_ptr(), v.data_ptr(), *self._cache(), tables.data_ptr(), lengths.data_ptr(),
             None if cu_seqlens is None else cu_seqlens.data_ptr(), n, batch, width, self.pages, self.heads, self.page, self.dim,
-            ldk, ldv, _native.stream_handle(k.device))
+            ldk, ldv)
 
     def read(self, tables, starts, cu_seqlens, rows):
         """Sequence b's rows ``starts[b]`` on, ``cu_seqlens[b + 1] - cu_seqlens[b]`` of them and ``rows`` in all, as bf16
         k and v [rows, heads, dim]."""
         batch, width = self._sequences(tables, starts, cu_seqlens, rows, "starts")
         assert cu_seqlens is not None, "read needs cu_seqlens"
-        _native.require_one_device(self.k, tables, starts, cu_seqlens)
+        index = _native.require_one_device(self.k, tables, starts, cu_seqlens)
         k = torch.empty((rows, self.heads, self.dim), dtype=torch.bfloat16, device=self.k.device)
         v = torch.empty_like(k)
         _native.launch(
-            k.device, "reax_kv8_read", *self._cache(), tables.data_ptr(), starts.data_ptr(), cu_seqlens.data_ptr(), k.data_ptr(),
-            v.data_ptr(), rows, batch, width, self.pages, self.heads, self.page, self.dim, _native.stream_handle(k.device))
+            index, "reax_kv8_read", *self._cache(), tables.data_ptr(), starts.data_ptr(), cu_seqlens.data_ptr(), k.data_ptr(),
+            v.data_ptr(), rows, batch, width, self.pages, self.heads, self.page, self.dim)
         return k, v
 
     def attend(self, q, tables, lengths, *, cu_seqlens=None, max_rows=None, scale=None, return_lse=False, out=None):
@@ -108,14 +108,14 @@ class Int8Cache:
         else:
             assert out.dtype is torch.bfloat16 and out.shape == q.shape and out.is_contiguous(), \
                 "out is contiguous bf16 like q"
-        _native.require_one_device(self.k, q, tables, lengths, cu_seqlens, out)
+        index = _native.require_one_device(self.k, q, tables, lengths, cu_seqlens, out)
         lse = torch.empty((n, heads_q), dtype=torch.float32, device=q.device) if return_lse else None
         if max_rows is None:
             max_rows = 1 if cu_seqlens is None else n
         ws = _native.kv8_workspace(q.device)
         _native.launch(
-            q.device, "reax_kv8_attend", q.data_ptr(), *self._cache(), tables.data_ptr(), lengths.data_ptr(),
+            index, "reax_kv8_attend", q.data_ptr(), *self._cache(), tables.data_ptr(), lengths.data_ptr(),
             None if cu_seqlens is None else cu_seqlens.data_ptr(), out.data_ptr(), None if lse is None else lse.data_ptr(), n,
             max_rows, batch, width, self.pages, self.heads, heads_q // self.heads, self.page, self.dim, ldq,
-            self.dim ** -0.5 if scale is None else scale, ws.data_ptr(), ws.numel(), _native.stream_handle(q.device))
+            self.dim ** -0.5 if scale is None else scale, ws.data_ptr(), ws.numel())
         return (out, lse) if return_lse else out

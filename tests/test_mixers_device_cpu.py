@@ -38,7 +38,8 @@ class Machine:
         monkeypatch.setattr(torch.cuda, "device", self.device)
         monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
         monkeypatch.setattr(_native, "load", lambda: self.library)
-        monkeypatch.setattr(_native, "stream_handle", lambda device=None: 0)
+        monkeypatch.setattr(_native, "_current_device", lambda: self.current)
+        monkeypatch.setattr(_native, "_raw_stream", lambda index: 0)
         monkeypatch.setattr(_native, "_workspaces", {})
 
     @contextlib.contextmanager
