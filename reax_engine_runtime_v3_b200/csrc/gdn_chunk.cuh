@@ -998,6 +998,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1) gdn_chunk_kernel(const __gri
 
 constexpr size_t gdn_chunk_smem() { return sizeof(GdnShared) + 1024; }
 constexpr size_t gdn_tiles_smem() { return sizeof(GdnTilesShared) + 1024; }
+// A block of the second kernel takes all of its SM's tensor memory and then waits for the first kernel's end, so that no block of
+// the first may share an SM with it: it would wait for tensor memory for good.  Their shared memory keeps them apart.
+static_assert(gdn_chunk_smem() + gdn_tiles_smem() + 2 * 1024 > 228 * 1024, "blocks of both kernels fit one SM");
 static_assert(gdn_chunk_smem() <= 227 * 1024 && 4 * (gdn_tiles_smem() + 1024) <= 228 * 1024, "shared memory of one SM");
 
 }  // namespace reax
