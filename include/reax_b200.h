@@ -239,7 +239,8 @@ REAX_API int reax_sliced_i8_static(const int8_t* A, const int8_t* W, const void*
  * those of its column.  With `normalize` a row of q or k whose sum of squares passes float32 counts as not finite.
  *
  * reax_gdn_prefill: sequence b has rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1 (int32 [batch + 1] on the device;
- * NULL: one sequence of all rows); one without rows keeps its state as it is, or gets zeros when `carry` is 0.
+ * NULL: one sequence of all rows); one without rows keeps its state as it is, or gets zeros when `carry` is 0.  A call with
+ * rows = 0 does nothing at all, whatever `carry` is.  Rows of no sequence are not written.
  * carry: 1 = start from the states kept, 0 = from zeros, and the states are only written. */
 REAX_API int reax_gdn_prefill(const void* q, const void* k, const void* v, const float* g, const float* beta,
                               float* state, const int32_t* cu_seqlens, const int32_t* slots, void* out, int rows,
@@ -296,7 +297,8 @@ REAX_API size_t reax_kv8_workspace_bytes(int device);
  * and holds a NaN or an infinity or sees a place of a page whose scale of k or v is one, gives NaN in out and lse; no
  * other row is touched by it.  Query head h reads cached head h / group.  out bf16 [rows, heads * group, dim]; lse
  * float32 [rows, heads * group] (may be NULL): the natural log of the sum of exp(scale q.k).  max_rows: at least the
- * most query rows of a sequence (a hint for the launch; the result does not depend on it).
+ * most query rows of a sequence (a hint for the launch; the result does not depend on it).  Rows of no sequence are not
+ * written.
  * The workspace (reax_kv8_workspace_bytes(), zeroed once) holds the parts of rows whose cache several blocks share.
  * Calls that can run at the same time have one each: one for each stream, and one for each captured graph.  Calls that are
  * captured need not find it zeroed. */

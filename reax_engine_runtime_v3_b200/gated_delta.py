@@ -62,7 +62,8 @@ def prefill(q, k, v, g, beta, state, *, cu_seqlens=None, slots=None, carry=True,
     beta float32 [rows, v_heads]; sequence b has rows ``cu_seqlens[b]`` up to ``cu_seqlens[b + 1]`` (int32 on the
     device; without it all rows are one sequence).  ``carry``: start from the states kept, else from zeros.
     ``normalize``: divide q and k by the root of their sum of squares first; ``scale`` is Dk ** -0.5 if not given.
-    Returns out bf16 [rows, v_heads, Dv]; the states are updated in place."""
+    A sequence without rows keeps its state, or gets zeros without ``carry``; a call without any rows does nothing.  Returns
+    out bf16 [rows, v_heads, Dv] (rows of no sequence are not written); the states are updated in place."""
     batch = 1 if cu_seqlens is None else cu_seqlens.shape[0] - 1
     out, strides, sizes, index = _check(q, k, v, g, beta, state, slots, out, batch)
     if cu_seqlens is not None:
