@@ -195,8 +195,8 @@ def workspace(device: torch.device) -> torch.Tensor:
     """Zero-initialised GEMM workspace for (device, current stream), created once and reused.
 
     The kernels leave it zeroed, so it is never cleared again (where the first call on a stream is a captured one, the
-    zeroing belongs to that graph: replay it first, or run a call on the stream before the capture); one workspace per stream keeps two
-    lanes replaying graphs concurrently apart (the reference keys its workspaces by stream too,
+    zeroing belongs to that graph: replay it first, or run a call on the stream before the capture);
+    one workspace per stream keeps two lanes replaying graphs concurrently apart (the reference keys its workspaces by stream too,
     runtime/native_core.py:102-115).
     """
     return _stream_workspace(device, "reax_workspace_bytes")

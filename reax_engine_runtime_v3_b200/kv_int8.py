@@ -98,8 +98,8 @@ class Int8Cache:
         rows 0 .. lengths[b] - n + i.  A row that sees none gives zeros (and -inf), one that holds a NaN or an infinity
         gives NaN (in both).  ``max_rows``: at least the most query rows of a sequence, where the caller knows it (a hint: it
         picks the kernel, not the result; without it ``cu_seqlens`` means the form for many rows, the slow one where each
-        sequence has one).  Rows of no sequence are not written.  Returns out bf16 [rows, heads * group, dim], with the float32 log-sum-exp
-        [rows, heads * group] beside it if asked."""
+        sequence has one).  Rows of no sequence are not written.  Returns out bf16 [rows, heads * group, dim], with the
+        float32 log-sum-exp [rows, heads * group] beside it if asked."""
         assert q.dim() == 3 and q.shape[1] % self.heads == 0, "the query heads are a multiple of the cached heads"
         n, heads_q, _ = q.shape
         ldq = _rows(q, heads_q, self.dim, "q")
