@@ -241,7 +241,8 @@ REAX_API int reax_sliced_i8_static(const int8_t* A, const int8_t* W, const void*
  * reax_gdn_prefill: sequence b has rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1 (int32 [batch + 1] on the device;
  * NULL: one sequence of all rows); one without rows keeps its state as it is, or gets zeros when `carry` is 0.  A call with
  * rows = 0 does nothing at all, whatever `carry` is.  Rows of no sequence are not written.
- * carry: 1 = start from the states kept, 0 = from zeros, and the states are only written. */
+ * carry: 1 = start from the states kept, 0 = from zeros, and the states are only written.  g may be above 0 as long as
+ * no 64 rows grow a state by more than 2^8 (its operands have 16 bits; reax_gdn_decode has no such bound). */
 REAX_API int reax_gdn_prefill(const void* q, const void* k, const void* v, const float* g, const float* beta,
                               float* state, const int32_t* cu_seqlens, const int32_t* slots, void* out, int rows,
                               int batch, int k_heads, int v_heads, int Dk, int Dv, int n_slots, long long ldq,
