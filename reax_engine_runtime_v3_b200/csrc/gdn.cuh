@@ -55,7 +55,7 @@ REAX_DEVI void gdn_rows(const GdnParams& p, int b, int* begin, int* end) {
 // One block a sequence and head: the block's threads hold the whole state, 4 columns of DV and DK / kGroups
 // rows each, so each value is read and written once and both sums over k (k^T S and q^T S) take one pass:
 // o = e^g q^T S + (q.k) u needs no second one.  Bound by the state's bytes: 512 sequences of 32 heads of 128 x 128 (2.1 GB read
-// and written) take 327 us, 6.6 TB/s; one takes 4 us, most of it the launch.
+// and written) take 327 to 338 us, 6.4 to 6.6 TB/s; one takes 4 us, most of it the launch.
 constexpr int kStepThreads = 256;
 
 template <int DK, int DV>

@@ -32,13 +32,15 @@
 // found by gdn_tiles_kernel for all chunks at once, a block of four warps for each chunk and key head, and kept in scratch
 // memory; gdn_chunk_kernel then carries the states along, a block for each sequence and value head, which reads those tiles
 // as they are.  Of one kernel with warps for each part, a chunk took 6.5 us of a block, most of it waiting for the solve of
-// the next one, where the second kernel takes 4.1: 8192 rows of one sequence and 32 value heads 860 -> 608 us, 32768 rows of
-// 16 sequences 836 -> 804 us, 4001 of 8 155 -> 136 us, 96 rows 22.5 -> 24.6 us.
+// the next one, where the second kernel takes 4.0: 8192 rows of one sequence and 32 value heads 860 us then and 590 now,
+// 32768 rows of 16 sequences 836 and 776, 4001 of 8 155 and 130, 96 rows 22.5 and 23.2.
 //
 // What bounds the second: the chain of a chunk.  Its three products take 3700 cycles from operands ready to results ready (of
-// which 2500 are MMAs) and the steps between them 4100.  Sixteen warps of a quarter column each in place of eight of a half
-// took as long (645 us for the 8192 rows).  The first (270 us of the 804): four blocks of four warps an SM, which its registers
-// and shared memory allow, fill 35% of its issue slots; the rest is waiting for the rows of k below 32, whose solve is longest.
+// which 2500 are MMAs) and the steps between them about 3900.  Sixteen warps of a quarter column each in place of eight of a
+// half took as long (645 us for the 8192 rows, 628 then by eight).  With DV = 64 half of the lanes carry zeros and a chunk
+// takes as long as with 128 (8192 rows 587 us).  The first (265 us of the 776, 298 alone): four blocks of four warps an SM, which
+// its registers and shared memory allow, fill 35% of its issue slots; the rest is waiting for the rows of k below 32, whose solve
+// is longest.
 //
 // Roles of the second (10 warps): 0-7 carry the state; 8 issues the MMAs; 9 loads.
 #pragma once

@@ -80,8 +80,8 @@ REAX_DEVI uint32_t kv8_codes(float x0, float x1, float x2, float x3, float scale
 // One block writes the new rows of one page, one head, of k (blockIdx.z = 0) or v (1).  Block x is the x-th
 // page touched, counted over the sequences in order: a warp's prefix sum over the batch finds whose it is,
 // so the host need not know the lengths.  Bound by bytes in the long run (rows read once, in registers for both the page's
-// maximum and its codes): 8191 rows of 4 heads of 256 appended and read back take 33 us
-// on the device, where their bytes take 16: two rounds of blocks, each a chain of loads that need each other.
+// maximum and its codes): 8192 rows of 4 heads of 256 take 21 us to append and 12 to read back, where their bytes take 8 each:
+// two rounds of blocks here and a search for each row there, chains of loads that need each other.
 constexpr int kAppendThreads = 256;
 
 __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(const Kv8Append a) {

@@ -21,7 +21,7 @@
 // exceeds it by 8 (in log2): weights stay below 2^8, which bf16 holds as well as any.
 //
 // Work.  The tiles of all items lie on one line, of which each block takes an equal part; parts of items that blocks share are
-// joined by a second kernel, in the blocks' order.  2048 rows of four prompts (19676 tiles) take 270 us; a block for each item
+// joined by a second kernel, in the blocks' order.  2048 rows of four prompts (19676 tiles) take 267 to 287 us; a block for each item
 // had left the longest for the end (510 us), and one sequence of 65536 cached rows and 16 new ones to four blocks (2305 us,
 // now 73).
 //
@@ -108,7 +108,8 @@ struct TileSeq {
 
 // A place on the line of items: of the cached heads one after the other, in each those of the sequences.  An item is as long
 // as its tiles and kItemTiles more, which come first and stand for the time that it takes to begin and end one (its rows
-// of q, its outputs; measured 9 us): 2048 rows of four prompts take 290 us where only tiles are counted, 270 with it.
+// of q, its outputs; measured 9 us, at 256 values a head): 2048 rows of four prompts took 290 us where only tiles are counted
+// and 270 with it, side by side.
 constexpr int kItemTiles = 5;
 struct TileCursor {
     long long end;                            // the item's on the line

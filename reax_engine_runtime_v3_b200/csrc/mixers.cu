@@ -166,9 +166,17 @@ struct AttendWorkspace {
     }
 };
 
-// Rows x heads of a sequence up to which the step form is used: it reads the cache once for each 16 of them.  Measured at 256
-// values a head, 4 cached heads of 64 sequences with 4096 cached rows: 16 rows x heads 150 us by it and 206 by the form for
-// many rows, 32 of them 262 and 208; of one sequence with 65536, 16: 84 and 73, 32: 104 and 73; of one with 4096, 8: 26 and 33.
+// Rows x heads of a sequence up to which the step form is used: it reads the cache once for each 16 of them.  Measured (us on
+// the device, by it / by the form for many rows, 4 cached heads):
+//   values a head                            64          128          256
+//   64 sequences of 4096 rows, 16:      78 / 152     92 / 164    144 / 208
+//                              32:     134 / 153    162 / 165    253 / 207
+//   16 sequences of 1024 rows, 16:      18 / 26      21 / 28      31 / 35
+//                              32:      26 / 26      30 / 29      42 / 36
+//   one of 65536 rows,         16:      46 / 51      52 / 55      73 / 67
+//                              32:      53 / 52      62 / 56      91 / 69
+//   one of 4096 rows,          16:      19 / 21      21 / 22      26 / 26
+//                              32:      19 / 21      22 / 22      29 / 27
 constexpr int kStepMostRows = reax::kStepRows;
 
 template <int D>
