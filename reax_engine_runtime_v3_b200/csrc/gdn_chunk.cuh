@@ -109,7 +109,7 @@ struct GdnShared {
     GdnTiles tiles[2];
     __nv_bfloat16 v[2][kChunk * 128];         // rows of DV values
     __nv_bfloat16 out[8][32 * 32];            // a warp's 32 rows of 32 output columns
-    float xch[2][8][32];
+    float xch[2][8][32], mu[8][32];
     uint64_t kq_in[kKqSlots], kq_free[kKqSlots], v_in[2], v_free[2], tiles_in[2], tiles_free[2];
     uint64_t s_ready, r_ready, v_ready, x_done, v_done, d_done, y_done, drained;
     int length[kGdnSorted], sequence, before;
@@ -702,7 +702,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1) gdn_chunk_kernel(const __gri
             s[i] = from_state && n < DV ? f2(at[0], at[DV]) : 0;
         }
         int turn = 0;
-        // Largest of both parts of this thread's row (the two warps of a quarter meet).
+        // Largest of both parts of this thread's row (the two warps of a quarter meet).  Both get the same value whatever else has
+        // happened, expired waits included: a place is written again only behind the barrier after the one it was read behind.
         auto row_max = [&](float m) {
             float* x = &sh.xch[turn][quarter * 2][lane];
             x[part * 32] = m;
@@ -854,9 +855,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1) gdn_chunk_kernel(const __gri
                 m = max3(m, mul2_rn(u2(x[2 * i], x[2 * i + 1]), pair_of(st.c_v + at)));
                 mu = max3(mu, mul2_rn(u2(x[2 * i], x[2 * i + 1]), pair_of(st.c_u + at)));
             }
-            sh.xch[turn ^ 1][quarter * 2 + part][lane] = mu;      // read behind row_max's barrier
+            sh.mu[quarter * 2 + part][lane] = mu;                 // read behind row_max's barrier
             const float2 vs = scale_of(row_max(m));
-            const float2 us = scale_of(fmaxf(sh.xch[turn][quarter * 2][lane], sh.xch[turn][quarter * 2 + 1][lane]));
+            const float2 us = scale_of(fmaxf(sh.mu[quarter * 2][lane], sh.mu[quarter * 2 + 1][lane]));
 #pragma unroll
             for (int e = 0; e < 16; e += 8) {
                 uint32_t hi[8], lo[8];
