@@ -21,7 +21,7 @@
 // exceeds it by 8 (in log2): weights stay below 2^8, which bf16 holds as well as any.
 //
 // Work.  The tiles of all items lie on one line, of which each block takes an equal part; parts of items that blocks share are
-// joined by a second kernel, in the blocks' order.  2048 rows of four prompts (19676 tiles) take 267 to 287 us; a block for each item
+// joined by a second kernel, in the blocks' order.  2048 rows of four prompts (19676 tiles) take 267 to 292 us; a block for each item
 // had left the longest for the end (510 us), and one sequence of 65536 cached rows and 16 new ones to four blocks (2305 us,
 // now 73).
 //
